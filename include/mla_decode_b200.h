@@ -349,6 +349,100 @@ int32_t mla_decode_ext_fp8kv(const void* q, const void* q_pe, const void* kv_fp8
                              const MlaCfg* cfg, void* stream);
 
 /*
+ * Decode over a latent cache held in 4 bits.  No counterpart in the reference.
+ * A latent row's 512 dims are 16 groups of 32; group g has a float16 scale s and a
+ * dim's code n (0..15) stands for (n - 8) s:
+ *   kv_codes   [..., kv_heads, 256] bytes: dims 8 w .. 8 w + 7 share 32-bit word w,
+ *              whose nibbles, lowest first, are dims 0 2 4 6 1 3 5 7 of the eight
+ *   kv_scales  [..., kv_heads, 16] float16
+ *   k_pe_cache [..., kv_heads, 64] in `dtype`
+ * 416 bytes a row instead of 1,152.  Everything else (q, q_pe, out, lse, paging, lengths,
+ * query positions, KV heads, cfg) as in mla_decode_ext.  Rows past a sequence's length
+ * are not read; a row on a page outside [0, num_pages) reads as zeros.
+ * Workspace: mla_decode_int4kv_workspace_bytes (256-byte aligned, zero before the first
+ * call with it, left ready by every call); 0 with no error text means none is needed.
+ */
+size_t mla_decode_int4kv_workspace_bytes(int32_t batch, int32_t q_len, int32_t heads, int32_t kv_heads,
+                                         int32_t max_seqlen_kv, int32_t dtype, const MlaCfg* cfg);
+int32_t mla_decode_ext_int4kv(const void* q, const void* q_pe, const void* kv_codes, const void* kv_scales,
+                              const void* k_pe_cache, const int32_t* block_table, const int32_t* cache_seqlens,
+                              void* out, float* lse, void* workspace, size_t workspace_bytes, int32_t batch,
+                              int32_t q_len, int32_t heads, int32_t kv_heads, int32_t max_seqlen_kv,
+                              int32_t page_size, int32_t num_pages, int32_t max_pages_per_seq, int32_t dtype,
+                              const MlaCfg* cfg, void* stream);
+
+/*
+ * Block tables and slots of a paged cache from request lengths, on the device.  No
+ * counterpart in the reference (its cache is contiguous).
+ * Request i holds L = cache_seqlens[i] rows (clamped to [0, max_pages x page_size]) in
+ * ceil(L / page_size) pages of its table row and gets n = new_lens[i] more (negative: 0).
+ * Pages it lacks come from free_pages[*free_pos ...], in request order; their ids are
+ * written into block_table (other entries are left as they are).
+ *   new_seqlens  [batch] rows held afterwards: L + n, or less when the table row or the
+ *                free list is full (rows that found no place are dropped)
+ *   new_free_pos [1] first free-list entry not handed out
+ *   slots        [num_tokens] cache row (page x page_size + row in page) of every new row,
+ *                -1 where there is none (padding, no place, a page id outside
+ *                [0, num_pages))
+ *   positions    [num_tokens] index of every new row in its sequence (0: padding)
+ *   cu_new       [batch + 1] first new row of every request (optional)
+ * q_len 0: new rows are packed, request after request (rows past num_tokens are not
+ * added); q_len > 0: num_tokens = batch x q_len, n is at most q_len and request i's rows
+ * are the last n of [i q_len, (i + 1) q_len), as mla_decode_ext's causal rule has a step's
+ * rows.  new_seqlens may be cache_seqlens and new_free_pos may be free_pos (in place);
+ * otherwise no two arrays overlap.  Workspace: mla_block_tables_workspace_bytes (16-byte
+ * aligned; 0 with no error text: none).
+ */
+size_t mla_block_tables_workspace_bytes(int32_t batch, int32_t num_tokens);
+int32_t mla_extend_block_tables(int32_t* block_table, const int32_t* cache_seqlens, const int32_t* new_lens,
+                                const int32_t* free_pages, const int32_t* free_pos, int32_t* new_seqlens,
+                                int32_t* new_free_pos, int32_t* slots, int32_t* positions, int32_t* cu_new,
+                                void* workspace, size_t workspace_bytes, int32_t batch, int32_t max_pages,
+                                int32_t page_size, int32_t num_pages, int32_t num_free, int32_t num_tokens,
+                                int32_t q_len, void* stream);
+
+/*
+ * Rotary positions.  No counterpart in the reference (its inputs come rotated).
+ * x, out [tokens, heads, head_dim] (last dim contiguous, other strides in elements;
+ * dtype 0, 1 or 2 = float32); dims [offset, offset + rot_dim) of every head are rotated,
+ * the others copied.  Pair i of the rot_dim / 2 (dims 2 i, 2 i + 1 with `interleaved`, else
+ * i, i + rot_dim / 2) turns by positions[token] x turns[i] turns (turns: float64
+ * [rot_dim / 2], frequency / 2 pi) and is multiplied by `gain`; negative positions turn
+ * back.  out may be x (same strides); else they must not overlap.  rot_dim is even, at
+ * most 1024.
+ */
+int32_t mla_rotary(const void* x, void* out, const int32_t* positions, const double* turns, float gain,
+                   int32_t tokens, int32_t heads, int32_t head_dim, int32_t rot_dim, int32_t offset,
+                   int32_t interleaved, int64_t x_token_stride, int64_t x_head_stride, int64_t out_token_stride,
+                   int64_t out_head_stride, int32_t dtype, void* stream);
+
+/*
+ * Rows into a latent cache (contiguous or paged: cache_rows rows in all) and back.  No
+ * counterpart in the reference.  Row t of kv [tokens, kv_heads, 512] and k_pe
+ * [tokens, kv_heads, 64] (strides in elements, multiples of 8; last dim contiguous) goes
+ * to cache row slots[t]; a slot outside [0, cache_rows) is skipped, distinct slots are the
+ * caller's (of two tokens with one slot, either's values may remain).
+ *   form MLA_CACHE_MODEL: kv_cache holds `dtype`; MLA_CACHE_FP8: e4m3 codes of kv / kv_scale
+ *   (round to nearest, saturating); MLA_CACHE_INT4: kv_cache holds codes and kv_scales
+ *   their scales as in mla_decode_ext_int4kv, with s = half(max |kv| / 7) (at most 65504)
+ *   and n = clamp(rint(kv / s), -8, 7) + 8; NaN stores as 0.
+ * With `positions` (int32 [tokens]) k_pe is rotated on the way (64 dims, turns / gain /
+ * interleaved as in mla_rotary).
+ * mla_cache_gather reads rows back: kv[t], k_pe[t] = what cache row slots[t] stands for,
+ * rounded to `dtype`; zeros for a slot outside [0, cache_rows).
+ */
+enum MlaCacheForm { MLA_CACHE_MODEL = 0, MLA_CACHE_FP8 = 1, MLA_CACHE_INT4 = 2 };
+int32_t mla_cache_append(const void* kv, const void* k_pe, const int32_t* slots, void* kv_cache, void* kv_scales,
+                         void* k_pe_cache, float kv_scale, const int32_t* positions, const double* turns, float gain,
+                         int32_t interleaved, int64_t tokens, int32_t kv_heads, int64_t cache_rows,
+                         int64_t kv_token_stride, int64_t kv_head_stride, int64_t pe_token_stride,
+                         int64_t pe_head_stride, int32_t form, int32_t dtype, void* stream);
+int32_t mla_cache_gather(const int32_t* slots, const void* kv_cache, const void* kv_scales, const void* k_pe_cache,
+                         float kv_scale, void* kv, void* k_pe, int64_t tokens, int32_t kv_heads, int64_t cache_rows,
+                         int64_t kv_token_stride, int64_t kv_head_stride, int64_t pe_token_stride,
+                         int64_t pe_head_stride, int32_t form, int32_t dtype, void* stream);
+
+/*
  * mla_decode_fwd without a workspace argument, for callers that cannot
  * allocate device memory where they decode (code running under CUDA-graph
  * capture, servers that reserve all memory up front and forbid allocation on

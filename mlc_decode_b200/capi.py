@@ -30,7 +30,14 @@ EXPORTED_SYMBOLS = ("mla_abi_version", "mla_last_error", "mla_split_plan",
                     "mla_decode_fp8kv", "mla_decode_ext_fp8kv", "mla_selftest_wait_timeout",
                     "mla_noalloc_init", "mla_noalloc_status", "mla_combine_strided",
                     "mla_seqsplit_buffer_bytes", "mla_ipc_export", "mla_ipc_import", "mla_ipc_close",
-                    "mla_seqsplit_exchange", "mla_seqsplit_decode", "mla_seqsplit_merge")
+                    "mla_seqsplit_exchange", "mla_seqsplit_decode", "mla_seqsplit_merge",
+                    "mla_decode_int4kv_workspace_bytes", "mla_decode_ext_int4kv",
+                    "mla_block_tables_workspace_bytes", "mla_extend_block_tables", "mla_rotary",
+                    "mla_cache_append", "mla_cache_gather")
+
+MLA_CACHE_MODEL = 0
+MLA_CACHE_FP8 = 1
+MLA_CACHE_INT4 = 2
 
 MLA_SELFTEST_STATUS = 0x1FF   # status word written by mla_selftest_wait_timeout
 
@@ -144,6 +151,24 @@ def load(build_if_missing: bool = True):
         lib.mla_seqsplit_decode.restype = i32
         lib.mla_seqsplit_merge.argtypes = [pvp, i32, i32, ctypes.c_uint32, i32, i32, vp, vp, i32, vp]
         lib.mla_seqsplit_merge.restype = i32
+        i64, f32 = ctypes.c_int64, ctypes.c_float
+        lib.mla_decode_int4kv_workspace_bytes.argtypes = [i32, i32, i32, i32, i32, i32, ctypes.POINTER(MlaCfg)]
+        lib.mla_decode_int4kv_workspace_bytes.restype = sz
+        lib.mla_decode_ext_int4kv.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32, i32,
+                                              i32, i32, i32, i32, ctypes.POINTER(MlaCfg), vp]
+        lib.mla_decode_ext_int4kv.restype = i32
+        lib.mla_block_tables_workspace_bytes.argtypes = [i32, i32]
+        lib.mla_block_tables_workspace_bytes.restype = sz
+        lib.mla_extend_block_tables.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32,
+                                                i32, i32, i32, vp]
+        lib.mla_extend_block_tables.restype = i32
+        lib.mla_rotary.argtypes = [vp, vp, vp, vp, f32, i32, i32, i32, i32, i32, i32, i64, i64, i64, i64, i32, vp]
+        lib.mla_rotary.restype = i32
+        lib.mla_cache_append.argtypes = [vp, vp, vp, vp, vp, vp, f32, vp, vp, f32, i32, i64, i32, i64, i64, i64, i64,
+                                         i64, i32, i32, vp]
+        lib.mla_cache_append.restype = i32
+        lib.mla_cache_gather.argtypes = [vp, vp, vp, vp, f32, vp, vp, i64, i32, i64, i64, i64, i64, i64, i32, i32, vp]
+        lib.mla_cache_gather.restype = i32
         _lib = lib
         return lib
 
@@ -373,3 +398,66 @@ def seqsplit_merge(bufs, world, rank, epoch, batch, heads, out, lse, dtype, stre
     arr = bufs if isinstance(bufs, ctypes.Array) else (ctypes.c_void_p * len(bufs))(*bufs)
     check(load().mla_seqsplit_merge(arr, int(world), int(rank), int(epoch), int(batch), int(heads), out, lse,
                                     int(dtype), stream))
+
+
+def int4kv_workspace_bytes(batch, q_len, heads, kv_heads, max_seqlen_kv, dtype, cfg: MlaCfg) -> int:
+    n = load().mla_decode_int4kv_workspace_bytes(int(batch), int(q_len), int(heads), int(kv_heads),
+                                                 int(max_seqlen_kv), int(dtype), ctypes.byref(cfg))
+    if n == 0:
+        msg = last_error()
+        if msg:
+            raise MlaError(1, msg)
+    return int(n)
+
+
+def decode_ext_int4kv(q, q_pe, kv_codes, kv_scales, k_pe_cache, block_table, cache_seqlens, out, lse, ws, ws_bytes,
+                      batch, q_len, heads, kv_heads, max_seqlen_kv, page_size, num_pages, max_pages, dtype,
+                      cfg: MlaCfg, stream) -> None:
+    """mla_decode_ext_int4kv: mla_decode_ext over a latent cache held in 4 bits."""
+    check(load().mla_decode_ext_int4kv(q, q_pe, kv_codes, kv_scales, k_pe_cache, block_table, cache_seqlens, out, lse,
+                                       ws, ws_bytes, int(batch), int(q_len), int(heads), int(kv_heads),
+                                       int(max_seqlen_kv), int(page_size), int(num_pages), int(max_pages),
+                                       int(dtype), ctypes.byref(cfg), stream))
+
+
+def block_tables_workspace_bytes(batch, num_tokens) -> int:
+    n = load().mla_block_tables_workspace_bytes(int(batch), int(num_tokens))
+    if n == 0:
+        msg = last_error()
+        if msg:
+            raise MlaError(1, msg)
+    return int(n)
+
+
+def extend_block_tables(block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens, new_free_pos, slots,
+                        positions, cu_new, ws, ws_bytes, batch, max_pages, page_size, num_pages, num_free, num_tokens,
+                        q_len, stream) -> None:
+    """mla_extend_block_tables (pointers are device addresses)."""
+    check(load().mla_extend_block_tables(block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens,
+                                         new_free_pos, slots, positions, cu_new, ws, ws_bytes, int(batch),
+                                         int(max_pages), int(page_size), int(num_pages), int(num_free),
+                                         int(num_tokens), int(q_len), stream))
+
+
+def rotary(x, out, positions, turns, gain, tokens, heads, head_dim, rot_dim, offset, interleaved, x_strides,
+           out_strides, dtype, stream) -> None:
+    """mla_rotary; strides are (token, head) in elements."""
+    check(load().mla_rotary(x, out, positions, turns, float(gain), int(tokens), int(heads), int(head_dim),
+                            int(rot_dim), int(offset), int(bool(interleaved)), *map(int, x_strides),
+                            *map(int, out_strides), int(dtype), stream))
+
+
+def cache_append(kv, k_pe, slots, kv_cache, kv_scales, k_pe_cache, kv_scale, positions, turns, gain, interleaved,
+                 tokens, kv_heads, cache_rows, kv_strides, pe_strides, form, dtype, stream) -> None:
+    """mla_cache_append; strides are (token, head) in elements."""
+    check(load().mla_cache_append(kv, k_pe, slots, kv_cache, kv_scales, k_pe_cache, float(kv_scale), positions, turns,
+                                  float(gain), int(bool(interleaved)), int(tokens), int(kv_heads), int(cache_rows),
+                                  *map(int, kv_strides), *map(int, pe_strides), int(form), int(dtype), stream))
+
+
+def cache_gather(slots, kv_cache, kv_scales, k_pe_cache, kv_scale, kv, k_pe, tokens, kv_heads, cache_rows, kv_strides,
+                 pe_strides, form, dtype, stream) -> None:
+    """mla_cache_gather; strides are (token, head) in elements."""
+    check(load().mla_cache_gather(slots, kv_cache, kv_scales, k_pe_cache, float(kv_scale), kv, k_pe, int(tokens),
+                                  int(kv_heads), int(cache_rows), *map(int, kv_strides), *map(int, pe_strides),
+                                  int(form), int(dtype), stream))

@@ -10,6 +10,8 @@ allocated on first use and reused, and passes it through the C ABI.
 """
 from __future__ import annotations
 
+import contextlib
+import math
 import os
 import threading
 
@@ -36,6 +38,16 @@ def _check_tensor(name, t, shape, dtype, device):
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
     if not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
+
+
+@contextlib.contextmanager
+def _on_device(device):
+    """The current stream of ``device`` (its handle), with that device current."""
+    if torch.cuda.current_device() == device.index:
+        yield torch.cuda.current_stream(device).cuda_stream
+    else:
+        with torch.cuda.device(device):
+            yield torch.cuda.current_stream(device).cuda_stream
 
 
 class MlaDecodeKernel:
@@ -449,3 +461,150 @@ class MlaPagedDecodeKernel:
             capi.decode_ext(q.data_ptr(), q_pe.data_ptr(), kv_cache.data_ptr(), k_pe_cache.data_ptr(), bt_ptr,
                             sl_ptr, out.data_ptr(), lse_ptr, ws.data_ptr(), ws.numel(), b, ql, h, kvh, smax,
                             page_size, num_pages, max_pages, _DTYPES[dtype], self._ccfg, stream)
+
+    def decode_int4(self, q, q_pe, kv_codes, kv_scales, k_pe_cache, cache_seqlens, out, lse=None, block_table=None):
+        """``__call__`` over a latent cache held in 4 bits (mla_decode_ext_int4kv).
+
+        ``kv_codes`` uint8 [..., kv_heads, 256] and ``kv_scales`` float16 [..., kv_heads, 16]
+        (leading dims as ``__call__``'s kv_cache) hold the rows as ``cache_append`` writes
+        them: 16 groups of 32 dims, each dim (code - 8) x its group's scale.  q, q_pe,
+        k_pe_cache and out keep the model's type; bfloat16 queries must lie within fp16's
+        range (the scores are fp16 products with fp32 sums).
+        """
+        b, h, smax, ql, kvh = self.batch, self.heads, self.max_seqlen_kv, self.q_len, self.kv_heads
+        dtype = q.dtype if isinstance(q, torch.Tensor) else None
+        if dtype not in _DTYPES:
+            raise ValueError(f"q must be float16 or bfloat16, got {dtype}")
+        dev = q.device
+        qshape = (b, h) if ql == 1 else (b, ql, h)
+        _check_tensor("q", q, (*qshape, DIM), dtype, None)
+        _check_tensor("q_pe", q_pe, (*qshape, PE_DIM), dtype, dev)
+        _check_tensor("out", out, (*qshape, DIM), dtype, dev)
+        if lse is not None:
+            _check_tensor("lse", lse, qshape, torch.float32, dev)
+        if cache_seqlens is not None:
+            _check_tensor("cache_seqlens", cache_seqlens, (b,), torch.int32, dev)
+        if block_table is None:
+            lead, page_size, num_pages, max_pages = (b, smax, kvh), 0, 0, 0
+        else:
+            if not isinstance(kv_codes, torch.Tensor) or kv_codes.dim() != 4:
+                raise ValueError(f"kv_codes must be [num_pages, page_size, {kvh}, 256]")
+            num_pages, page_size = int(kv_codes.shape[0]), int(kv_codes.shape[1])
+            if block_table.dim() != 2 or block_table.shape[0] != b:
+                raise ValueError(f"block_table must be [batch, max_pages], got {tuple(block_table.shape)}")
+            max_pages = int(block_table.shape[1])
+            _check_tensor("block_table", block_table, (b, max_pages), torch.int32, dev)
+            lead = (num_pages, page_size, kvh)
+        _check_tensor("kv_codes", kv_codes, (*lead, DIM // 2), torch.uint8, dev)
+        _check_tensor("kv_scales", kv_scales, (*lead, DIM // 32), torch.float16, dev)
+        _check_tensor("k_pe_cache", k_pe_cache, (*lead, PE_DIM), dtype, dev)
+        with _on_device(dev) as stream:
+            ws = self._int4_workspace(dev, dtype)
+            capi.decode_ext_int4kv(q.data_ptr(), q_pe.data_ptr(), kv_codes.data_ptr(), kv_scales.data_ptr(),
+                                   k_pe_cache.data_ptr(), None if block_table is None else block_table.data_ptr(),
+                                   None if cache_seqlens is None else cache_seqlens.data_ptr(), out.data_ptr(),
+                                   None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), b, ql, h, kvh,
+                                   smax, page_size, num_pages, max_pages, _DTYPES[dtype], self._ccfg, stream)
+
+    def _int4_workspace(self, device, dtype):
+        key = (device.index, dtype, "int4")
+        ws = self._ws.get(key)
+        if ws is None:
+            with self._lock:
+                ws = self._ws.get(key)
+                if ws is None:
+                    n = capi.int4kv_workspace_bytes(self.batch, self.q_len, self.heads, self.kv_heads,
+                                                    self.max_seqlen_kv, _DTYPES[dtype], self._ccfg)
+                    ws = self._ws[key] = torch.zeros(max(n, 1), dtype=torch.uint8, device=device)
+        return ws
+
+    def step(self, q, q_pe, kv, k_pe, kv_cache, k_pe_cache, block_table, cache_seqlens, free_pages, free_pos, out,
+             lse=None, new_lens=None, rotary=None, kv_scale=None, kv_scales=None):
+        """One decode step over a paged cache of any form: extend the block tables, write the
+        step's rows to the cache, decode.
+
+        q, q_pe, out, lse as in ``__call__``; kv [batch, kv_heads, 512] and k_pe [batch,
+        kv_heads, 64] ([batch, q_len, ...] for q_len > 1) are the step's new rows, of which
+        request i keeps its last ``new_lens[i]`` (int32 [batch] on the device; None: all q_len).
+        The cache is 16-bit, e4m3 (``kv_scale``) or 4-bit (``kv_scales``), as ``cache_append``
+        has it.  ``block_table``, ``cache_seqlens`` and ``free_pos`` (see
+        ``extend_block_tables``) are updated in place; a request whose table row or free list
+        is full keeps its length.  With ``rotary`` q_pe (into this object's scratch, q_pe
+        itself stays) and k_pe turn to their rows' positions.  Like the workspace, the scratch
+        is this object's: calls of one object are serialised by the caller.
+        """
+        from . import paged
+
+        b, ql, kvh = self.batch, self.q_len, self.kv_heads
+        dtype = q.dtype if isinstance(q, torch.Tensor) else None
+        if dtype not in _DTYPES:
+            raise ValueError(f"q must be float16 or bfloat16, got {dtype}")
+        dev = q.device
+        qshape = (b, self.heads) if ql == 1 else (b, ql, self.heads)
+        rshape = (b, kvh) if ql == 1 else (b, ql, kvh)
+        # everything is checked before the first launch: a refused step changes nothing
+        _check_tensor("q", q, (*qshape, DIM), dtype, None)
+        _check_tensor("q_pe", q_pe, (*qshape, PE_DIM), dtype, dev)
+        _check_tensor("out", out, (*qshape, DIM), dtype, dev)
+        if lse is not None:
+            _check_tensor("lse", lse, qshape, torch.float32, dev)
+        _check_tensor("kv", kv, (*rshape, DIM), dtype, dev)
+        _check_tensor("k_pe", k_pe, (*rshape, PE_DIM), dtype, dev)
+        paged._check_cache(kv_cache, k_pe_cache, kv_scale, kv_scales, dtype, dev)
+        if kv_cache.shape[2] != kvh:
+            raise ValueError(f"the cache has {kv_cache.shape[2]} KV heads, expected {kvh}")
+        if kv_cache.shape[1] % 64 or kv_cache.shape[1] < 64:
+            raise ValueError(f"page_size must be a positive multiple of 64, got {kv_cache.shape[1]}")
+        if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
+            raise ValueError("block_table must be an int32 tensor [batch, max_pages]")
+        _check_tensor("block_table", block_table, (b, block_table.shape[1]), torch.int32, dev)
+        _check_tensor("cache_seqlens", cache_seqlens, (b,), torch.int32, dev)
+        if new_lens is not None:
+            _check_tensor("new_lens", new_lens, (b,), torch.int32, dev)
+        if rotary is not None and rotary.rot_dim != PE_DIM:
+            raise ValueError(f"rotary must turn {PE_DIM} dims, not {rotary.rot_dim}")
+        if block_table.shape[1] * kv_cache.shape[1] > self.max_seqlen_kv:
+            raise ValueError(f"block_table covers {block_table.shape[1] * kv_cache.shape[1]} rows, more than "
+                             f"max_seqlen_kv = {self.max_seqlen_kv}")
+        num_pages, page_size = kv_cache.shape[:2]
+        if num_pages * page_size >= (1 << 31) - 256:
+            raise ValueError(f"the cache must hold fewer than 2^31 - 256 rows, got {num_pages * page_size}")
+        if kv_scale is not None and not (kv_scale > 0 and math.isfinite(kv_scale)):
+            raise ValueError(f"kv_scale must be finite and > 0, got {kv_scale}")
+        for name, t in (("q", q), ("q_pe", q_pe), ("out", out), ("kv", kv), ("k_pe", k_pe), ("kv_cache", kv_cache),
+                        ("k_pe_cache", k_pe_cache), ("kv_scales", kv_scales)):
+            if t is not None and t.data_ptr() % 16:
+                raise ValueError(f"{name} must start on a 16-byte boundary")
+        scale = self._ccfg.softmax_scale
+        if not (scale >= 0 and math.isfinite(scale)):
+            raise ValueError(f"softmax_scale must be finite and > 0, got {scale}")
+        self._int4_workspace(dev, dtype) if kv_scales is not None else self._workspace(dev, dtype)
+        slots, positions, all_new, turned = self._step_scratch(dev, dtype)
+        paged.extend_block_tables(block_table, cache_seqlens, all_new if new_lens is None else new_lens, free_pages,
+                                  free_pos, cache_seqlens, free_pos, slots, positions,
+                                  page_size=page_size, num_pages=num_pages, q_len=ql)
+        paged.cache_append(kv.view(b * ql, kvh, DIM), k_pe.view(b * ql, kvh, PE_DIM), slots, kv_cache, k_pe_cache,
+                           kv_scale=kv_scale, kv_scales=kv_scales, rotary=rotary,
+                           positions=None if rotary is None else positions)
+        if rotary is not None:
+            rotary(q_pe.view(b * ql, self.heads, PE_DIM), positions, turned)
+            q_pe = turned.view(*qshape, PE_DIM)
+        if kv_scales is not None:
+            self.decode_int4(q, q_pe, kv_cache, kv_scales, k_pe_cache, cache_seqlens, out, lse,
+                             block_table=block_table)
+        else:
+            self(q, q_pe, kv_cache, k_pe_cache, cache_seqlens, out, lse, block_table=block_table, kv_scale=kv_scale)
+
+    def _step_scratch(self, device, dtype):
+        key = (device.index, dtype, "step")
+        s = self._ws.get(key)
+        if s is None:
+            with self._lock:
+                s = self._ws.get(key)
+                if s is None:
+                    n = self.batch * self.q_len
+                    s = self._ws[key] = (torch.empty(n, dtype=torch.int32, device=device),
+                                         torch.empty(n, dtype=torch.int32, device=device),
+                                         torch.full((self.batch,), self.q_len, dtype=torch.int32, device=device),
+                                         torch.empty(n, self.heads, PE_DIM, dtype=dtype, device=device))
+        return s

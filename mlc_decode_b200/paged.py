@@ -1,0 +1,299 @@
+"""The paged latent cache around a decode call: block tables and slots from request
+lengths, rotary positions, and latent rows into and out of the cache.
+
+Everything is enqueued on the current stream of the tensors' device, allocates at most
+small temporaries, never synchronises the host and can be captured into a CUDA graph.
+No counterpart in the reference, whose cache is one contiguous tensor per call and whose
+inputs come rotated (baseline_mla.py:167-191).  C entry points: mla_extend_block_tables,
+mla_rotary, mla_cache_append, mla_cache_gather (include/mla_decode_b200.h).
+"""
+from __future__ import annotations
+
+import math
+import threading
+
+import torch
+
+from . import capi
+from .decode import _DTYPES, _FP8, DIM, PE_DIM, _check_tensor, _on_device
+
+INT4_GROUP = 32                      # dims per scale of the 4-bit form
+INT4_GROUPS = DIM // INT4_GROUP      # scales per row
+INT4_BYTES = DIM // 2                # code bytes per row
+
+_ROTARY_DTYPES = {**_DTYPES, torch.float32: capi.MLA_DTYPE_F32}
+
+
+def extend_block_tables(block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens, new_free_pos, slots,
+                        positions, page_size, num_pages, cu_new=None, q_len=0):
+    """Give every request ``new_lens[i]`` more cache rows (mla_extend_block_tables).
+
+    All tensors int32 on one device.  ``block_table`` [batch, max_pages] is extended in
+    place with page ids taken from ``free_pages[free_pos[0]:]`` in request order;
+    ``cache_seqlens`` [batch] are the rows held.  Written: ``new_seqlens`` [batch] (rows held
+    afterwards; fewer than asked for when the table row or the free list is full),
+    ``new_free_pos`` [1], ``slots`` [num_tokens] (cache row of every new row, -1 where there is
+    none), ``positions`` [num_tokens] (index in its sequence) and ``cu_new`` [batch + 1]
+    (first new row of every request; optional).  New rows are packed, request after request,
+    or, with ``q_len``, the last rows of each request's q_len.  ``new_seqlens`` may be
+    ``cache_seqlens`` and ``new_free_pos`` may be ``free_pos``; nothing else may overlap.
+    """
+    if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
+        raise ValueError("block_table must be an int32 tensor [batch, max_pages]")
+    b, max_pages = block_table.shape
+    dev = block_table.device
+    i32 = torch.int32
+    _check_tensor("block_table", block_table, (b, max_pages), i32, None)
+    n, nf = (t.numel() if isinstance(t, torch.Tensor) else -1 for t in (slots, free_pages))
+    for name, t, shape in (("cache_seqlens", cache_seqlens, (b,)), ("new_lens", new_lens, (b,)),
+                           ("free_pages", free_pages, (nf,)), ("free_pos", free_pos, (1,)),
+                           ("new_seqlens", new_seqlens, (b,)), ("new_free_pos", new_free_pos, (1,)),
+                           ("slots", slots, (n,)), ("positions", positions, (n,))):
+        if not (type(t) is torch.Tensor and t.dtype == i32 and t.device == dev and t.shape == shape
+                and t.is_contiguous()):
+            _check_tensor(name, t, shape, i32, dev)
+    if cu_new is not None:
+        _check_tensor("cu_new", cu_new, (b + 1,), i32, dev)
+    with _on_device(dev) as stream:
+        nbytes = capi.block_tables_workspace_bytes(b, n)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+        capi.extend_block_tables(block_table.data_ptr(), cache_seqlens.data_ptr(), new_lens.data_ptr(),
+                                 free_pages.data_ptr(), free_pos.data_ptr(), new_seqlens.data_ptr(),
+                                 new_free_pos.data_ptr(), slots.data_ptr(), positions.data_ptr(),
+                                 None if cu_new is None else cu_new.data_ptr(),
+                                 None if ws is None else ws.data_ptr(), nbytes, b, max_pages, page_size, num_pages,
+                                 nf, n, q_len, stream)
+
+
+def rotary_frequencies(rot_dim, base=10000.0, scaling=None):
+    """(angles per position of the rot_dim / 2 pairs, gain on cos and sin) in 64 bits.
+
+    Unscaled: base ** (-2 i / rot_dim), gain 1.  ``scaling`` (a dict) stretches them for
+    contexts longer than the trained one:
+      {"type": "linear", "factor": f}   every frequency / f
+      {"type": "ntk", "factor": f}      base * f ** (rot_dim / (rot_dim - 2))
+      {"type": "yarn", "factor": f, "original_max_position": n, "beta_fast": 32, "beta_slow": 1,
+       "gain": ...}                     pairs that turn more than beta_fast times in n positions
+                                        stay, those below beta_slow turns are / f, a linear ramp
+                                        between them; gain defaults to 0.1 ln f + 1
+    """
+    if rot_dim < 2 or rot_dim % 2 or not base > 1.0 or not math.isfinite(base):
+        raise ValueError(f"rot_dim must be even and >= 2 and base finite and > 1 (got {rot_dim}, {base})")
+    s = dict(scaling or {})
+    kind = s.get("type")
+    if kind not in (None, "linear", "ntk", "yarn"):
+        raise ValueError(f"unknown rotary scaling {kind!r}")
+    known = {None: set(), "linear": {"factor"}, "ntk": {"factor"},
+             "yarn": {"factor", "original_max_position", "beta_fast", "beta_slow", "gain"}}[kind]
+    if set(s) - known - {"type"}:
+        raise ValueError(f"unknown rotary scaling parameters {sorted(set(s) - known - {'type'})}")
+    factor = float(s.get("factor", 1.0))
+    if not factor >= 1.0 or not math.isfinite(factor):
+        raise ValueError(f"rotary scaling factor must be finite and >= 1, got {factor}")
+    if kind == "ntk":
+        if rot_dim == 2:
+            raise ValueError("ntk scaling needs rot_dim > 2")
+        base = base * factor ** (rot_dim / (rot_dim - 2))
+    freq = [base ** (-2.0 * i / rot_dim) for i in range(rot_dim // 2)]
+    if kind == "linear":
+        return [f / factor for f in freq], 1.0
+    if kind != "yarn":
+        return freq, 1.0
+    trained = float(s.get("original_max_position", 0))
+    fast, slow = float(s.get("beta_fast", 32.0)), float(s.get("beta_slow", 1.0))
+    if not trained >= 1 or not fast >= slow > 0:
+        raise ValueError("yarn needs original_max_position >= 1 and beta_fast >= beta_slow > 0")
+
+    def pair_of(turns):   # the (fractional) pair that makes `turns` turns in the trained context
+        return rot_dim * math.log(trained / (turns * 2 * math.pi)) / (2 * math.log(base))
+
+    low, high = max(math.floor(pair_of(fast)), 0), min(math.ceil(pair_of(slow)), rot_dim - 1)
+    out = []
+    for i, f in enumerate(freq):
+        ramp = min(max((i - low) / max(high - low, 0.001), 0.0), 1.0)
+        out.append(f * (1.0 - ramp) + f / factor * ramp)
+    return out, float(s.get("gain", 0.1 * math.log(factor) + 1.0))
+
+
+class Rotary:
+    """Rotary positions of ``rot_dim`` dims of every head (mla_rotary).
+
+    ``rot(x, positions, out, offset=0)``: x, out [tokens, heads, head_dim] in float16,
+    bfloat16 or float32 (any token and head strides, last dim contiguous), positions int32
+    [tokens]; dims [offset, offset + rot_dim) turn, the others are copied; out may be x.
+    ``interleaved``: pairs are dims (2 i, 2 i + 1), else (i, i + rot_dim / 2).  ``scaling``: see
+    ``rotary_frequencies``.  The frequencies are uploaded by the first call on a device (make
+    it, or ``rot.turns(device)``, before a graph capture).
+    """
+
+    def __init__(self, rot_dim=PE_DIM, base=10000.0, interleaved=True, scaling=None):
+        self.rot_dim, self.base, self.interleaved = int(rot_dim), float(base), bool(interleaved)
+        self.scaling = dict(scaling) if scaling else None
+        freq, self.gain = rotary_frequencies(self.rot_dim, self.base, self.scaling)
+        if self.rot_dim > 1024:
+            raise ValueError(f"rot_dim must be at most 1024, got {rot_dim}")
+        if not math.isfinite(self.gain):
+            raise ValueError(f"gain must be finite, got {self.gain}")
+        self._turns = [f / (2 * math.pi) for f in freq]
+        self._dev = {}
+        self._lock = threading.Lock()
+        capi.load()
+
+    def turns(self, device):
+        """Turns per position of every pair, float64 on ``device`` (kept)."""
+        device = torch.device(device)
+        if device.type == "cuda" and device.index is None:
+            device = torch.device("cuda", torch.cuda.current_device())
+        t = self._dev.get(device)
+        if t is None:
+            with self._lock:
+                t = self._dev.get(device)
+                if t is None:
+                    t = self._dev[device] = torch.tensor(self._turns, dtype=torch.float64, device=device)
+        return t
+
+    def __call__(self, x, positions, out, offset=0):
+        if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _ROTARY_DTYPES:
+            raise ValueError("x must be a float16, bfloat16 or float32 tensor [tokens, heads, head_dim]")
+        n, h, d = x.shape
+        if not 0 <= int(offset) <= d - self.rot_dim:
+            raise ValueError(f"dims [{offset}, {offset} + {self.rot_dim}) must lie inside the head's {d}")
+        _check_rows("x", x, x.shape, x.dtype, None)
+        _check_rows("out", out, x.shape, x.dtype, x.device, written=True)
+        _check_tensor("positions", positions, (n,), torch.int32, x.device)
+        if n == 0:
+            return
+        if out.data_ptr() == x.data_ptr() and out.stride() != x.stride() or \
+                out.data_ptr() != x.data_ptr() and _ranges_meet(x, out):
+            raise ValueError("out must be x itself or must not overlap it")
+        turns = self.turns(x.device)
+        with _on_device(x.device) as stream:
+            capi.rotary(x.data_ptr(), out.data_ptr(), positions.data_ptr(), turns.data_ptr(), self.gain, n, h, d,
+                        self.rot_dim, offset, self.interleaved, x.stride()[:2], out.stride()[:2],
+                        _ROTARY_DTYPES[x.dtype], stream)
+
+
+def _ranges_meet(a, b):
+    def span(t):
+        last = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
+        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+    (a0, a1), (b0, b1) = span(a), span(b)
+    return a0 < b1 and b0 < a1
+
+
+def _check_rows(name, t, shape, dtype, device, written=False, align=1):
+    """A 3-D CUDA tensor with contiguous last dim; its rows start on ``align`` elements, and
+    do not overlap one another when they are written."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be a CUDA tensor (got {t.device})")
+    if device is not None and t.device != device:
+        raise ValueError(f"{name} is on {t.device}, expected {device}")
+    if t.dtype != dtype:
+        raise ValueError(f"{name} has dtype {t.dtype}, expected {dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(shape)}")
+    if t.numel() == 0:
+        return
+    if t.shape[2] > 1 and t.stride(2) != 1:
+        raise ValueError(f"{name}: the last dimension must be contiguous")
+    if align > 1:
+        bad = [s for d, s in enumerate(t.stride()[:2]) if t.shape[d] > 1 and s % align]
+        if bad or t.data_ptr() % (align * t.element_size()):
+            raise ValueError(f"{name}: every row must start on a {align * t.element_size()}-byte boundary")
+    if written:
+        need = t.shape[2]
+        for s, size in sorted((t.stride(d), t.shape[d]) for d in (0, 1) if t.shape[d] > 1):
+            if s < need:
+                raise ValueError(f"{name}: rows overlap (strides {t.stride()})")
+            need = s * (size - 1) + need
+
+
+def _strides(t):
+    """Token and head stride; of a dimension of one entry any stride will do."""
+    return tuple(t.stride(d) if t.shape[d] > 1 else 0 for d in (0, 1))
+
+
+def _check_cache(kv_cache, k_pe_cache, kv_scale, kv_scales, dtype, device):
+    """(form, rows, kv_heads) of a cache [a, b, kv_heads, width] in any of its forms."""
+    if not isinstance(kv_cache, torch.Tensor) or kv_cache.dim() != 4:
+        raise ValueError("kv_cache must be [num_pages, page_size, kv_heads, width] (or [batch, max_seqlen, ...])")
+    lead = tuple(kv_cache.shape[:3])
+    if kv_scales is not None:
+        if kv_scale is not None:
+            raise ValueError("kv_scale belongs to an e4m3 cache, kv_scales to a 4-bit one: pass one of them")
+        form = capi.MLA_CACHE_INT4
+        _check_tensor("kv_cache", kv_cache, (*lead, INT4_BYTES), torch.uint8, device)
+        _check_tensor("kv_scales", kv_scales, (*lead, INT4_GROUPS), torch.float16, device)
+    elif kv_cache.dtype in (torch.uint8, _FP8):
+        if kv_scale is None:
+            raise ValueError("an e4m3 kv_cache needs kv_scale, a 4-bit one kv_scales")
+        form = capi.MLA_CACHE_FP8
+        _check_tensor("kv_cache", kv_cache, (*lead, DIM), kv_cache.dtype, device)
+    else:
+        if kv_scale is not None:
+            raise ValueError("kv_scale belongs to an e4m3 cache")
+        form = capi.MLA_CACHE_MODEL
+        _check_tensor("kv_cache", kv_cache, (*lead, DIM), dtype, device)
+    _check_tensor("k_pe_cache", k_pe_cache, (*lead, PE_DIM), dtype, device)
+    return form, lead[0] * lead[1], lead[2]
+
+
+def _check_dense(kv, k_pe, slots, written):
+    dtype = kv.dtype if isinstance(kv, torch.Tensor) else None
+    if dtype not in _DTYPES or kv.dim() != 3:
+        raise ValueError("kv must be a float16 or bfloat16 tensor [tokens, kv_heads, 512]")
+    n, h = kv.shape[:2]
+    _check_rows("kv", kv, (n, h, DIM), dtype, None, written, align=8)
+    _check_rows("k_pe", k_pe, (n, h, PE_DIM), dtype, kv.device, written, align=8)
+    _check_tensor("slots", slots, (n,), torch.int32, kv.device)
+    return n, h, dtype
+
+
+def cache_append(kv, k_pe, slots, kv_cache, k_pe_cache, kv_scale=None, kv_scales=None, rotary=None, positions=None):
+    """Write rows kv [tokens, kv_heads, 512] and k_pe [tokens, kv_heads, 64] to cache rows
+    ``slots`` (int32 [tokens]; outside the cache, e.g. -1: skipped; slots are distinct).
+
+    The cache ([num_pages, page_size, kv_heads, ...], or [batch, max_seqlen, kv_heads, ...])
+    is 16-bit (kv's type), e4m3 (``kv_scale``: codes of kv / kv_scale) or 4-bit (``kv_cache``
+    uint8 [..., 256] with ``kv_scales`` float16 [..., 16]); k_pe_cache is in kv's type.  With
+    ``rotary`` (a ``Rotary`` of 64 dims) and ``positions`` (int32 [tokens]) k_pe turns on the
+    way.  kv and k_pe may be strided (rows on 16-byte boundaries).
+    """
+    n, h, dtype = _check_dense(kv, k_pe, slots, False)
+    dev = kv.device
+    form, rows, kvh = _check_cache(kv_cache, k_pe_cache, kv_scale, kv_scales, dtype, dev)
+    if kvh != h:
+        raise ValueError(f"kv has {h} KV heads, the cache {kvh}")
+    if (rotary is None) != (positions is None):
+        raise ValueError("rotary and positions go together")
+    turns, gain, inter = None, 1.0, False
+    if rotary is not None:
+        if rotary.rot_dim != PE_DIM:
+            raise ValueError(f"rotary must turn {PE_DIM} dims, not {rotary.rot_dim}")
+        _check_tensor("positions", positions, (n,), torch.int32, dev)
+        turns, gain, inter = rotary.turns(dev), rotary.gain, rotary.interleaved
+    with _on_device(dev) as stream:
+        capi.cache_append(kv.data_ptr(), k_pe.data_ptr(), slots.data_ptr(), kv_cache.data_ptr(),
+                          None if kv_scales is None else kv_scales.data_ptr(), k_pe_cache.data_ptr(),
+                          1.0 if kv_scale is None else kv_scale, None if rotary is None else positions.data_ptr(),
+                          None if rotary is None else turns.data_ptr(), gain, inter, n, h, rows, _strides(kv),
+                          _strides(k_pe), form, _DTYPES[dtype], stream)
+
+
+def cache_gather(slots, kv_cache, k_pe_cache, kv, k_pe, kv_scale=None, kv_scales=None):
+    """Read cache rows ``slots`` back into kv [tokens, kv_heads, 512] and k_pe [tokens,
+    kv_heads, 64]: what the cache stands for, in the model's type (zeros for a slot outside
+    the cache).  The cache and its forms as in ``cache_append``.
+    """
+    n, h, dtype = _check_dense(kv, k_pe, slots, True)
+    dev = kv.device
+    form, rows, kvh = _check_cache(kv_cache, k_pe_cache, kv_scale, kv_scales, dtype, dev)
+    if kvh != h:
+        raise ValueError(f"kv has {h} KV heads, the cache {kvh}")
+    with _on_device(dev) as stream:
+        capi.cache_gather(slots.data_ptr(), kv_cache.data_ptr(), None if kv_scales is None else kv_scales.data_ptr(),
+                          k_pe_cache.data_ptr(), 1.0 if kv_scale is None else kv_scale, kv.data_ptr(),
+                          k_pe.data_ptr(), n, h, rows, _strides(kv), _strides(k_pe), form, _DTYPES[dtype], stream)
