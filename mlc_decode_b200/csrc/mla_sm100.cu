@@ -413,6 +413,7 @@ struct PieceIter {
     }
     v = t < t1 ? m.seq_of(t) : 0;
   }
+  __device__ bool any() const { return t < t1; }   // (a ragged call may give a pair no tiles)
   __device__ bool next(Piece* pc) {
     if (t >= t1) return false;
     while (m.first(v + 1) <= t) ++v;
@@ -437,7 +438,7 @@ __device__ __forceinline__ int max_len(const Params& p) {
   return cover < p.seqlen ? (int)cover : p.seqlen;
 }
 __device__ __forceinline__ int seq_len(const Params& p, int v) {
-  if (p.seqlens == nullptr && p.q_len == 1) return p.seqlen;
+  if (p.seqlens == nullptr && p.q_len == 1) return max_len(p);
   // the plan kernel counts tiles with the same lengths
   return qseq_len(p.seqlens, vseq_seq(p, v), p.q_len, p.kv_heads, max_len(p));
 }
@@ -475,6 +476,7 @@ __device__ __forceinline__ void k_producer(const Params& p, const Ctx& c, uint32
   const uint32_t kempty0 = ptx::smem_u32(&bars->kempty[0]);
   Ring<KS> ring;
   PieceIter it(p, pair);
+  if (!it.any()) return;   // no tiles: no Q loads to wait for either
   // the first Q rows are requested before any K or V traffic
   if (!wait_bar(c, ptx::smem_u32(&bars->q_go), 0u, kErrKLoad)) return;
   // Latent rows are read twice (K now, V one tile later): keep them in L2;
@@ -622,6 +624,7 @@ __device__ __forceinline__ void v_producer(const Params& p, const Ctx& c, uint32
   const uint32_t vempty0 = ptx::smem_u32(&bars->vempty[0]);
   Ring<VS> ring;
   PieceIter it(p, pair);
+  if (!it.any()) return;
   if (!wait_bar(c, ptx::smem_u32(&bars->q_go), 0u, kErrVLoad)) return;
   Piece pc;
   if constexpr (Io<T>::kKv8) {
