@@ -650,7 +650,8 @@ int decode_ext(const char* fn, const void* q, const void* q_pe, const void* kv_c
                const int32_t* block_table, const int32_t* cache_seqlens, void* out, float* lse, void* workspace,
                size_t workspace_bytes, int32_t batch, int32_t q_len, int32_t heads, int32_t kv_heads,
                int32_t max_seqlen_kv, int32_t page_size, int32_t num_pages, int32_t max_pages_per_seq,
-               int32_t dtype, const MlaCfg* cfg, void* stream, bool kv_fp8 = false, float kv_scale = 1.f) {
+               int32_t dtype, const MlaCfg* cfg, void* stream, bool kv_fp8 = false, float kv_scale = 1.f,
+               const void* kv_scales = nullptr) {
   if (kv_fp8 && (!(kv_scale > 0.f) || !isfinite(kv_scale))) {
     set_error("%s: kv_scale must be finite and > 0", fn);
     return MLA_ERR_ARG;
@@ -694,6 +695,7 @@ int decode_ext(const char* fn, const void* q, const void* q_pe, const void* kv_c
   a.kv_heads = kv_heads;
   a.kv_fp8 = kv_fp8 ? 1 : 0;
   a.kv_scale = kv_scale;
+  a.kv_scales = kv_scales;
   a.seqlen_kv = max_seqlen_kv;
   a.dtype = dtype;
   a.softmax_scale = (cfg != nullptr && cfg->softmax_scale != 0.f) ? cfg->softmax_scale : 1.0f / sqrtf((float)kQkDim);
@@ -728,6 +730,24 @@ int decode_ext(const char* fn, const void* q, const void* q_pe, const void* kv_c
 }
 
 }  // namespace
+
+size_t ext_int4_workspace(const char* fn, int batch, int q_len, int heads, int kv_heads, int max_seqlen_kv, int dtype,
+                          const MlaCfg* cfg) {
+  PagedLayout L;
+  if (paged_layout(fn, batch, q_len, heads, kv_heads, max_seqlen_kv, dtype, cfg, &L) != MLA_OK) return 0;
+  return L.total;
+}
+
+int decode_ext_int4(const char* fn, const void* q, const void* q_pe, const void* kv_codes, const void* kv_scales,
+                    const void* k_pe_cache, const int32_t* block_table, const int32_t* cache_seqlens, void* out,
+                    float* lse, void* workspace, size_t workspace_bytes, int batch, int q_len, int heads, int kv_heads,
+                    int max_seqlen_kv, int page_size, int num_pages, int max_pages_per_seq, int dtype,
+                    const MlaCfg* cfg, void* stream) {
+  return decode_ext(fn, q, q_pe, kv_codes, k_pe_cache, block_table, cache_seqlens, out, lse, workspace,
+                    workspace_bytes, batch, q_len, heads, kv_heads, max_seqlen_kv, page_size, num_pages,
+                    max_pages_per_seq, dtype, cfg, stream, false, 1.f, kv_scales);
+}
+
 }  // namespace mla
 
 extern "C" {

@@ -107,6 +107,17 @@ void set_error(const char* fmt, ...);
 int check_decode_call(const char* fn, const void* q, const void* q_pe, const void* kv, const void* k_pe,
                       const void* out, int batch, int heads, int seqlen_kv, int dtype, const MlaCfg* cfg);
 
+// The tensor-core path of a ragged call over a 4-bit cache: workspace layout (0 and an
+// error text when the shape is outside the kernel) and the call, with
+// mla_decode_ext_int4kv's arguments and mla_decode_ext's checks.
+size_t ext_int4_workspace(const char* fn, int batch, int q_len, int heads, int kv_heads, int max_seqlen_kv, int dtype,
+                          const MlaCfg* cfg);
+int decode_ext_int4(const char* fn, const void* q, const void* q_pe, const void* kv_codes, const void* kv_scales,
+                    const void* k_pe_cache, const int32_t* block_table, const int32_t* cache_seqlens, void* out,
+                    float* lse, void* workspace, size_t workspace_bytes, int batch, int q_len, int heads, int kv_heads,
+                    int max_seqlen_kv, int page_size, int num_pages, int max_pages_per_seq, int dtype,
+                    const MlaCfg* cfg, void* stream);
+
 // ---------------------------------------------------------------------------
 // launchers
 // ---------------------------------------------------------------------------
@@ -136,6 +147,9 @@ struct DecodeArgs {
   // (tensor-core kernel only); k_pe stays in `dtype`
   int kv_fp8;
   float kv_scale;
+  // kv holds 4-bit codes and kv_scales [rows][kv_heads][16] float16 their group scales
+  // (tensor-core kernel only); nullptr otherwise
+  const void* kv_scales;
   float softmax_scale;  // multiplies raw scores
   SplitPlan plan;
   cudaStream_t stream;

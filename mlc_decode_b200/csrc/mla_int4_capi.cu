@@ -4,6 +4,7 @@
 #include <math.h>
 
 #include "mla_cache.cuh"
+#include "mla_sm100.cuh"
 
 namespace mla {
 namespace {
@@ -11,6 +12,7 @@ namespace {
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 struct Int4Plan {
+  bool tc;          // tensor-core kernel; else the CUDA-core kernel with `splits` splits
   int splits;
   size_t lse_off, o_off, total;
 };
@@ -38,6 +40,17 @@ int plan_call(const char* fn, int batch, int q_len, int heads, int kv_heads, int
   if (asked < 0 || asked > 8192 || kernel < MLA_KERNEL_AUTO || kernel > MLA_KERNEL_TC) {
     set_error("%s: num_split must be in [0, 8192] and kernel a MlaKernelKind (got %d, %d)", fn, asked, kernel);
     return MLA_ERR_ARG;
+  }
+  const bool covered = sm100_supports_ext(batch, q_len, heads, kv_heads, max_seqlen_kv);
+  if (kernel == MLA_KERNEL_TC && !covered) {
+    set_error("%s: shape outside the tensor-core kernel (batch %d, q_len %d, heads %d, kv_heads %d, max_seqlen_kv %d)",
+              fn, batch, q_len, heads, kv_heads, max_seqlen_kv);
+    return MLA_ERR_UNSUPPORTED;
+  }
+  p->tc = kernel != MLA_KERNEL_SIMT && covered;
+  if (p->tc) {
+    p->total = ext_int4_workspace(fn, batch, q_len, heads, kv_heads, max_seqlen_kv, dtype, cfg);
+    return p->total > 0 ? MLA_OK : MLA_ERR_ARG;
   }
   p->splits = int4_simt_splits((int)qb, heads / kv_heads, max_seqlen_kv, asked);
   const size_t rows = p->splits > 1 ? (size_t)p->splits * batch * q_len * heads : 0;
@@ -76,12 +89,19 @@ int32_t mla_decode_ext_int4kv(const void* q, const void* q_pe, const void* kv_co
   Int4Plan p;
   int rc = plan_call(fn, batch, q_len, heads, kv_heads, max_seqlen_kv, dtype, cfg, &p);
   if (rc != MLA_OK) return rc;
-  if (!q || !q_pe || !kv_codes || !kv_scales || !k_pe_cache || !out) {
+  if (!kv_scales || !aligned16(kv_scales)) {
+    set_error(kv_scales ? "%s: tensor pointers must be 16-byte aligned" : "%s: null pointer", fn);
+    return MLA_ERR_ARG;
+  }
+  if (p.tc)
+    return decode_ext_int4(fn, q, q_pe, kv_codes, kv_scales, k_pe_cache, block_table, cache_seqlens, out, lse,
+                           workspace, workspace_bytes, batch, q_len, heads, kv_heads, max_seqlen_kv, page_size,
+                           num_pages, max_pages_per_seq, dtype, cfg, stream);
+  if (!q || !q_pe || !kv_codes || !k_pe_cache || !out) {
     set_error("%s: null pointer", fn);
     return MLA_ERR_ARG;
   }
-  if (!aligned16(q) || !aligned16(q_pe) || !aligned16(kv_codes) || !aligned16(kv_scales) || !aligned16(k_pe_cache) ||
-      !aligned16(out)) {
+  if (!aligned16(q) || !aligned16(q_pe) || !aligned16(kv_codes) || !aligned16(k_pe_cache) || !aligned16(out)) {
     set_error("%s: tensor pointers must be 16-byte aligned", fn);
     return MLA_ERR_ARG;
   }

@@ -157,22 +157,44 @@ struct Kv8 {};
 // fp16 and P.V runs once instead of as the bf16 hi/lo pair.
 template <typename T, bool kF16>
 struct Cv {};
+// The 4-bit variant: latent rows as codes and group scales (mla_cache.cuh).  Eight
+// converter warps widen each CTA's codes to fp16 ((n - 8) s, one rounding) straight
+// from registers: 16-byte global loads a tile ahead, no staging in shared memory.  A
+// tile is four operand slots of 64 rows x 128 dims: for QK^T slot u of CTA r holds dims
+// [128 u, +128) of the CTA's own 64 rows.  P.V wants from CTA r dims
+// [256 nh + 128 r, +128) of both row halves: for its own half that is slot 2 nh + r as it
+// stands (the same bytes are a K-major operand of QK^T and an MN-major operand of
+// P.V); slot 2 nh + 1 - r is refilled with the peer's half once QK^T has read it.  So a
+// value is widened 1.5 times instead of twice and a tile takes 64 KB, which leaves room
+// for two tiles.  Q's latent dims are fp16, the rope dims run in T.
+template <typename T>
+struct Kv4 {};
 template <typename K>
 struct Io {
   using Out = K;
   static constexpr bool kKv8 = false;
+  static constexpr bool kKv4 = false;
   static constexpr bool kConv = false;   // V through the converter warps
+};
+template <typename T>
+struct Io<Kv4<T>> {
+  using Out = T;
+  static constexpr bool kKv8 = false;
+  static constexpr bool kKv4 = true;
+  static constexpr bool kConv = false;
 };
 template <typename T>
 struct Io<Kv8<T>> {
   using Out = T;
   static constexpr bool kKv8 = true;
+  static constexpr bool kKv4 = false;
   static constexpr bool kConv = false;
 };
 template <typename T, bool kF16>
 struct Io<Cv<T, kF16>> {
   using Out = T;
   static constexpr bool kKv8 = false;
+  static constexpr bool kKv4 = false;
   static constexpr bool kConv = true;
 };
 template <typename T>
@@ -187,6 +209,18 @@ struct Cfg<Kv8<T>> {
   static constexpr int kV8Stages = 3;                // e4m3 V units as loaded (8 KB)
   using PT = __half;
   static_assert(kV8Stages <= 8, "barrier arrays");
+};
+template <typename T>
+struct Cfg<Kv4<T>> {
+  static constexpr uint32_t kFmt = 0;
+  static constexpr uint32_t kPvFmt = 0;
+  static constexpr uint32_t kRopeFmt = Cfg<T>::kFmt;
+  static constexpr int kPParts = 1;
+  static constexpr int kKStages = 8;                 // two tiles of four operand slots
+  static constexpr uint32_t kKStageBytes = kStageBytes;
+  static constexpr int kVStages = 0;                 // (P.V reads the same slots)
+  static constexpr int kV8Stages = 2;                // rope rows of two tiles
+  using PT = __half;
 };
 template <typename T, bool kF16>
 struct Cfg<Cv<T, kF16>> {
@@ -203,7 +237,7 @@ struct Cfg<Cv<T, kF16>> {
   using PT = typename std::conditional<kToF16, __half, typename Cfg<T>::PT>::type;
 };
 template <typename K>
-constexpr int threads_of() { return (Io<K>::kKv8 || Io<K>::kConv) ? 512 : 384; }
+constexpr int threads_of() { return (Io<K>::kKv8 || Io<K>::kKv4 || Io<K>::kConv) ? 512 : 384; }
 
 struct Barriers {
   uint64_t kfull[8], kempty[8];
@@ -248,7 +282,8 @@ struct Params {
   CUtensorMap tm_qpe;   // [qb][h][64]
   CUtensorMap tm_out;   // [qb][h][512] output rows, box 64 x 64 x 1 (stores; rows past h not written)
   CUtensorMap tm_part;  // [slots*128, 512] float32 partial rows, box 32 x 64 (stores)
-  const uint8_t* kv;    // raw latent rows (converter warps)
+  const uint8_t* kv;    // raw latent rows (converter warps): the 4-bit variant's codes
+  const __half* kv_scales;   // 4-bit variant: [rows][kv_heads][16] group scales
   const uint8_t* q;     // raw Q rows, for L2 prefetch
   const uint8_t* qpe;
   void* out;
@@ -279,7 +314,7 @@ struct Params {
   const uint32_t* cu_tiles;
   const int* seqlens;      // [real batch] KV rows per sequence, or nullptr (all seqlen)
   const int* block_table;  // [real batch][max_pages] page ids, or nullptr (contiguous rows)
-  int page_size, max_pages;
+  int page_size, max_pages, num_pages;
   float sl2;            // softmax scale * log2(e)
 };
 
@@ -450,6 +485,15 @@ __device__ __forceinline__ int kv_row(const Params& p, int seq, int row, int len
   return pg * p.page_size + row % p.page_size;
 }
 
+// First cache row of the 64 rows from `row` (a multiple of 64) of sequence `seq`, or -1
+// when the block table names a page the cache does not have (64-row runs never straddle
+// pages).  row < the sequence's length.
+__device__ __forceinline__ long long kv_row64(const Params& p, int seq, int row) {
+  if (p.block_table == nullptr) return (long long)seq * p.seqlen + row;
+  const int pg = __ldg(p.block_table + (size_t)seq * p.max_pages + row / p.page_size);
+  return (unsigned)pg < (unsigned)p.num_pages ? (long long)pg * p.page_size + row % p.page_size : -1;
+}
+
 // Position in a ring of `kStages` shared-memory stages.
 template <int kStages>
 struct Ring {
@@ -476,6 +520,32 @@ __device__ __forceinline__ void k_producer(const Params& p, const Ctx& c, uint32
   const uint32_t kempty0 = ptx::smem_u32(&bars->kempty[0]);
   Ring<KS> ring;
   PieceIter it(p, pair);
+  if constexpr (Io<T>::kKv4) {
+    // 4-bit: the rope rows of each tile (the latent codes go through the converter warps)
+    const uint32_t rfull0 = ptx::smem_u32(&bars->v8full[0]);
+    const uint32_t rfull0_leader = ptx::mapa(rfull0, 0);
+    const uint32_t rempty0 = ptx::smem_u32(&bars->v8empty[0]);
+    const uint64_t once = ptx::l2_policy_evict_first();
+    uint32_t gi = 0;
+    Piece pc;
+    while (it.next(&pc)) {
+      const int kseq = vseq_kvseq(p, pc.bb), kvh = vseq_kvh(p, pc.bb), klen = seq_len(p, pc.bb);
+#pragma unroll 1
+      for (int j = pc.first; j < pc.end; ++j, ++gi) {
+        const uint32_t b = gi & 1u;
+        const int row = j * kTile + 64 * (int)rank;
+        // rows past the length are masked (any row will do); a row on a page outside the
+        // cache reads as zeros: the row past the last is out of the tensor map's range
+        long long y = row < klen ? kv_row64(p, kseq, row) : 0;
+        if (y < 0) y = p.block_table != nullptr ? (long long)p.num_pages * p.page_size : 0;
+        if (gi >= 2 && !wait_bar(c, rempty0 + 8 * b, ((gi - 2) >> 1) & 1u, kErrKLoad)) return;
+        if (leader) ptx::mbar_arrive_expect_tx(rfull0 + 8 * b, 2 * kChunkBytes);
+        ptx::tma_load_3d_pair_hint(sbase + S::kV8Ring + b * kChunkBytes, &p.tm_kpe, rfull0_leader + 8 * b, 0, kvh,
+                                   (int)y, once);
+      }
+    }
+    return;
+  }
   if (!it.any()) return;   // no tiles: no Q loads to wait for either
   // the first Q rows are requested before any K or V traffic
   if (!wait_bar(c, ptx::smem_u32(&bars->q_go), 0u, kErrKLoad)) return;
@@ -563,9 +633,9 @@ __device__ __forceinline__ void q_loader(const Params& p, const Ctx& c, uint32_t
   const uint32_t qtr = ptx::smem_u32(&bars->qtr);
   const uint32_t q_go = ptx::smem_u32(&bars->q_go);
   PieceIter it(p, pair);
-  if constexpr (Io<T>::kKv8) {
-    // FP8: the softmax warps read each piece's Q rows from global memory (they
-    // quantize them); this thread only pulls the rows into L2 ahead of time
+  if constexpr (Io<T>::kKv8 || Io<T>::kKv4) {
+    // FP8 and 4-bit: the softmax warps read each piece's Q rows from global memory
+    // (they convert them); this thread only pulls the rows into L2 ahead of time
     Piece pq;
     bool first = true;
     while (it.next(&pq)) {
@@ -789,6 +859,144 @@ __device__ __forceinline__ void v_converter(const Params& p, const Ctx& c, int p
 }
 
 // ---------------------------------------------------------------------------
+// 4-bit variant: converter warps (warps 8..15).  Thread ct owns row ct / 4 and scale
+// group ct % 4 of every unit (64 rows x 128 dims): one 16-byte load of 32 codes and one
+// scale in, four 16-byte fp16 granules out.  Per tile: fill the four slots for QK^T
+// (each as soon as P.V of two tiles ago has released it; its register then takes the
+// next tile's load), then refill the two slots whose dims this CTA does not own with
+// the peer's rows for P.V of the tile before (once its QK^T has read them).  In this
+// order QK^T of a tile is issued ahead of P.V of the tile before, under which its
+// softmax runs.  Rows past the length and rows of absent pages become zeros.
+// ---------------------------------------------------------------------------
+struct Codes32 {
+  uint4 w;      // 32 codes
+  uint32_t s;   // their scale, in both halves
+};
+
+__device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
+__device__ __forceinline__ __half2 bits_h2(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
+
+// Eight codes of a word as four half pairs times s2: 1024 + n and 64 + n are exact in
+// fp16 (the nibble lands on their last bits, or four above), so are the differences
+// n - 8; the product rounds once.
+__device__ __forceinline__ uint4 widen8(uint32_t w, __half2 s2) {
+  const uint32_t v = w >> 8;
+  const __half2 c0 = bits_h2(0x64086408u), c1 = bits_h2(0x54805480u);   // 1032, 72
+  const __half2 a = __hsub2(bits_h2((w & 0x000f000fu) | 0x64006400u), c0);
+  const __half2 b = __hsub2(bits_h2((w & 0x00f000f0u) | 0x54005400u), c1);
+  const __half2 d = __hsub2(bits_h2((v & 0x000f000fu) | 0x64006400u), c0);
+  const __half2 e = __hsub2(bits_h2((v & 0x00f000f0u) | 0x54005400u), c1);
+  return make_uint4(h2_bits(__hmul2(a, s2)), h2_bits(__hmul2(b, s2)), h2_bits(__hmul2(d, s2)),
+                    h2_bits(__hmul2(e, s2)));
+}
+
+// Row r, group g of a unit at `dst` (two SW128 boxes of 64 dims): granule k of the
+// group at (4 (g & 1) + k) ^ (r & 7) of box g / 2.  The second box's threads take their
+// granules in the order 2 3 0 1: the eight threads of a store phase (two rows, four
+// groups) then hit eight distinct granule columns.
+__device__ __forceinline__ void store_codes(uint8_t* dst, int r, int g, const Codes32& x) {
+  const int flip = (g >> 1) << 1;
+  const uint32_t w[4] = {flip ? x.w.z : x.w.x, flip ? x.w.w : x.w.y, flip ? x.w.x : x.w.z, flip ? x.w.y : x.w.w};
+  uint8_t* row = dst + (g >> 1) * kChunkBytes + r * 128;
+  const __half2 s2 = bits_h2(x.s);
+#pragma unroll
+  for (int k = 0; k < 4; ++k)
+    *reinterpret_cast<uint4*>(row + (((4 * (g & 1) + (k ^ flip)) ^ (r & 7)) << 4)) = widen8(w[k], s2);
+}
+
+template <typename T>
+__device__ __forceinline__ void kv4_converter(const Params& p, const Ctx& c, uint32_t rank, int pair, uint8_t* smem,
+                                              Barriers* bars, int ct, int lane) {
+  using S = Smem<T>;
+  const uint32_t kfull0_leader = ptx::mapa(ptx::smem_u32(&bars->kfull[0]), 0);
+  const uint32_t vfull0_leader = ptx::mapa(ptx::smem_u32(&bars->vfull[0]), 0);
+  const uint32_t read0 = ptx::smem_u32(&bars->kempty[0]);    // QK^T has read a slot
+  const uint32_t free0 = ptx::smem_u32(&bars->vempty[0]);    // P.V has read a slot
+  uint8_t* ring = smem + S::kKRing;
+  const int r = ct >> 2, g = ct & 3;
+  PieceIter it(p, pair);
+  Piece pc;
+  int j = 0, seq = 0, kvh = 0, len = 0;
+  bool more = it.next(&pc);
+  if (!more) return;
+  j = pc.first;
+  // cache positions ((row * kv_heads + kvh), -1: zeros) of this thread's rows of a tile:
+  // its own half's and the peer half's
+  auto locate = [&](long long* own, long long* peer) {
+    seq = vseq_kvseq(p, pc.bb);
+    kvh = vseq_kvh(p, pc.bb);
+    len = seq_len(p, pc.bb);
+    const int ro = j * kTile + 64 * (int)rank, rp = j * kTile + 64 * (1 - (int)rank);
+    const long long bo = ro < len ? kv_row64(p, seq, ro) : -1, bp = rp < len ? kv_row64(p, seq, rp) : -1;
+    *own = (bo >= 0 && ro + r < len) ? (bo + r) * p.kv_heads + kvh : -1;
+    *peer = (bp >= 0 && rp + r < len) ? (bp + r) * p.kv_heads + kvh : -1;
+  };
+  auto advance = [&]() {
+    if (++j < pc.end) return;
+    more = it.next(&pc);
+    if (more) j = pc.first;
+  };
+  // 32 codes of dims [32 q, +32) (q = 0..15) at position `at`
+  auto load = [&](long long at, int q) -> Codes32 {
+    Codes32 x{make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u), 0u};
+    if (at >= 0) {
+      x.w = __ldg(reinterpret_cast<const uint4*>(p.kv + at * (kDim / 2)) + q);
+      const uint32_t h = __ldg(reinterpret_cast<const unsigned short*>(p.kv_scales) + at * 16 + q);
+      x.s = h | (h << 16);
+    }
+    return x;
+  };
+  long long own, peer_prev = -1, peer;
+  locate(&own, &peer);
+  Codes32 k[4];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) k[u] = load(own, 4 * u + g);
+  // refill the two slots of tile i that P.V wants from the peer's rows
+  auto refill = [&](uint32_t i, const Codes32 (&v)[2]) -> bool {
+#pragma unroll
+    for (int nh = 0; nh < 2; ++nh) {
+      const uint32_t slot = 4 * (i & 1u) + 2 * nh + (1 - rank);
+      if (!wait_bar(c, read0 + 8 * slot, (i >> 1) & 1u, kErrVLoad)) return false;
+      store_codes(ring + slot * kStageBytes, r, g, v[nh]);
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(vfull0_leader + 8 * slot);
+    }
+    return true;
+  };
+  uint32_t gi = 0;
+#pragma unroll 1
+  while (more) {
+    advance();
+    long long own_next = -1, peer_next = -1;
+    if (more) locate(&own_next, &peer_next);
+    Codes32 v[2];
+    if (gi > 0) {
+#pragma unroll
+      for (int nh = 0; nh < 2; ++nh) v[nh] = load(peer_prev, 8 * nh + 4 * (int)rank + g);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const uint32_t slot = 4 * (gi & 1u) + u;
+      if (gi >= 2 && !wait_bar(c, free0 + 8 * slot, ((gi - 2) >> 1) & 1u, kErrKLoad)) return;
+      store_codes(ring + slot * kStageBytes, r, g, k[u]);
+      ptx::fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(kfull0_leader + 8 * slot);
+      k[u] = load(own_next, 4 * u + g);
+    }
+    if (gi > 0 && !refill(gi - 1, v)) return;
+    peer_prev = peer;
+    peer = peer_next;
+    ++gi;
+  }
+  Codes32 v[2];
+#pragma unroll
+  for (int nh = 0; nh < 2; ++nh) v[nh] = load(peer_prev, 8 * nh + 4 * (int)rank + g);
+  refill(gi - 1, v);
+}
+
+// ---------------------------------------------------------------------------
 // Tail fixer of the plain variants (warp 9 of each CTA).  A V unit whose 64 token
 // rows run past the sequence's length (the last tile of a sequence) is loaded by
 // the V producer into this CTA's stage on a local barrier instead of the pair
@@ -924,6 +1132,8 @@ __device__ __forceinline__ void qk_issuer(const Params& p, const Ctx& c, int pai
   constexpr uint32_t kIdescRope = ptx::idesc_f16(Cfg<T>::kRopeFmt, 128, 128, 0);
   const uint32_t kfull0 = ptx::smem_u32(&bars->kfull[0]);
   const uint32_t kempty0 = ptx::smem_u32(&bars->kempty[0]);
+  const uint32_t rfull0 = ptx::smem_u32(&bars->v8full[0]);
+  const uint32_t rempty0 = ptx::smem_u32(&bars->v8empty[0]);
   const uint32_t q_full = ptx::smem_u32(&bars->q_full);
   const uint32_t q_empty = ptx::smem_u32(&bars->q_empty);
   const uint32_t qt_full = ptx::smem_u32(&bars->qt_full);
@@ -938,7 +1148,7 @@ __device__ __forceinline__ void qk_issuer(const Params& p, const Ctx& c, int pai
   int piece = 0;
   while (it.next(&pc)) {
     // (FP8: qt_full covers the whole quantized Q, written by the softmax warps)
-    if (!Io<T>::kKv8 && !wait_bar(c, q_full, (uint32_t)piece & 1u, kErrQK)) return;
+    if (!Io<T>::kKv8 && !Io<T>::kKv4 && !wait_bar(c, q_full, (uint32_t)piece & 1u, kErrQK)) return;
     if (!wait_bar(c, qt_full, (uint32_t)piece & 1u, kErrQK)) return;
     ptx::tc_fence_after();
 #pragma unroll 1
@@ -950,10 +1160,14 @@ __device__ __forceinline__ void qk_issuer(const Params& p, const Ctx& c, int pai
       const uint32_t s_tmem = tmem + 64 * b;
 #pragma unroll
       for (int u = 0; u < 5; ++u) {
-        if (!wait_bar(c, kfull0 + 8 * ring.stage, ring.phase, kErrQK)) return;
+        // (4-bit: the rope unit has its own ring of two)
+        const bool own_rope = Io<T>::kKv4 && u == 4;
+        const uint32_t full = own_rope ? rfull0 + 8 * b : kfull0 + 8 * ring.stage;
+        if (!wait_bar(c, full, own_rope ? (gi >> 1) & 1u : ring.phase, kErrQK)) return;
         ptx::tc_fence_after();
         // descriptor low words; +512 = next 8 KB box, +2 = next 32-byte k-step
-        const uint32_t kb = ptx::sw128_desc_lo(sbase + S::kKRing + ring.stage * Cfg<T>::kKStageBytes, 16);
+        const uint32_t kb = ptx::sw128_desc_lo(
+            sbase + (own_rope ? S::kV8Ring + b * kChunkBytes : S::kKRing + ring.stage * Cfg<T>::kKStageBytes), 16);
         if (Io<T>::kKv8 && u < 4) {
           // FP8: latent dims [128 u, +128) in e4m3, 32 per k-step: Q hi from TMEM (4
           // elements per column), Q lo from box u of the Q region
@@ -987,8 +1201,12 @@ __device__ __forceinline__ void qk_issuer(const Params& p, const Ctx& c, int pai
                                 kIdescRope, 1u);
           }
         }
-        ptx::mma_commit_pair_mc(kempty0 + 8 * ring.stage, 0x3);
-        ring.advance();
+        if (own_rope) {
+          ptx::mma_commit_pair_mc(rempty0 + 8 * b, 0x3);
+        } else {
+          ptx::mma_commit_pair_mc(kempty0 + 8 * ring.stage, 0x3);
+          ring.advance();
+        }
       }
       ptx::mma_commit_pair_mc(s_full0 + 8 * b, 0x3);
       if (j == pc.end - 1) ptx::mma_commit_pair_mc(q_empty, 0x3);
@@ -1013,7 +1231,10 @@ __device__ __forceinline__ void pv_issuer(const Params& p, const Ctx& c, int pai
   const uint32_t o_free = ptx::smem_u32(&bars->o_free);
   const uint32_t plo = ptx::sw128_desc_lo(sbase + S::kP, 16);
   constexpr uint32_t kHi = ptx::sw128_desc_hi(1024);
-  Ring<VS> ring;
+  const uint32_t kfull0 = ptx::smem_u32(&bars->kfull[0]);
+  // (4-bit: the K ring's eight slots, in the same order)
+  constexpr uint32_t kRing = Io<T>::kKv4 ? S::kKRing : S::kVRing;
+  Ring<Io<T>::kKv4 ? 8 : VS> ring;
   uint32_t gi = 0;
   PieceIter it(p, pair);
   Piece pc;
@@ -1030,10 +1251,12 @@ __device__ __forceinline__ void pv_issuer(const Params& p, const Ctx& c, int pai
 #pragma unroll 1
       for (int u = 0; u < 4; ++u) {
         const int nh = u >> 1, th = u & 1;
+        // 4-bit: one CTA's slot as QK^T had it, the other's refilled
+        if (Io<T>::kKv4 && !wait_bar(c, kfull0 + 8 * ring.stage, ring.phase, kErrPV)) return;
         if (!wait_bar(c, vfull0 + 8 * ring.stage, ring.phase, kErrPV)) return;
         ptx::tc_fence_after();
         // descriptor low words: V is MN-major (+128 = next 16 rows), P K-major (+2 = next k-step)
-        const uint32_t vb = ptx::sw128_desc_lo(sbase + S::kVRing + ring.stage * kStageBytes, kChunkBytes);
+        const uint32_t vb = ptx::sw128_desc_lo(sbase + kRing + ring.stage * kStageBytes, kChunkBytes);
 #pragma unroll
         for (int part = 0; part < Cfg<T>::kPParts; ++part) {
           const uint32_t pa = plo + b * (S::kPBuf >> 4) + part * (kPBytes >> 4) + th * 512;
@@ -1219,6 +1442,58 @@ __device__ __forceinline__ float quantize_q(const Params& p, int v, uint32_t ran
     *reinterpret_cast<uint4*>(rrow + kChunkBytes + off) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
   }
   return s / a;
+}
+
+// 4-bit variant: this thread's Q row as fp16 operands (rows past the head count zero):
+// latent dims [0, 256) to this lane's TMEM columns [kColQT, +128), this thread's half
+// (hf) of dims [256, 512) to boxes 2 hf, 2 hf + 1 of the Q region and its half of the rope
+// dims, in T, to box 4.
+template <typename Out>
+__device__ __forceinline__ uint32_t pair_to_h2(uint32_t w) {
+  if constexpr (std::is_same<Out, __half>::value) return w;
+  else return bf16x2_to_h2(w);
+}
+template <typename Out>
+__device__ __forceinline__ void load_q_f16(const Params& p, int v, uint32_t rank, int m, int hf, uint8_t* qreg,
+                                           uint32_t tmem, uint32_t lane_off) {
+  const int h = vseq_head0(p, v) + 64 * (int)rank + m;
+  const bool real = h < p.heads;
+  const size_t row = (size_t)vseq_seq(p, v) * p.heads + (real ? h : 0);
+  const uint4* qg = reinterpret_cast<const uint4*>(p.q) + row * (kDim / 8);      // 8 elements a granule
+  const uint4* rg = reinterpret_cast<const uint4*>(p.qpe) + row * (kPeDim / 8);
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  auto conv = [](uint4 x) {
+    return make_uint4(pair_to_h2<Out>(x.x), pair_to_h2<Out>(x.y), pair_to_h2<Out>(x.z), pair_to_h2<Out>(x.w));
+  };
+#pragma unroll 1
+  for (int cb = 0; cb < 4; ++cb) {   // 64 dims: 32 TMEM columns
+    uint4 x[8];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) x[g] = real ? __ldg(qg + 8 * cb + g) : zero;
+    uint32_t w[32];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) {
+      const uint4 y = conv(x[g]);
+      w[4 * g] = y.x;
+      w[4 * g + 1] = y.y;
+      w[4 * g + 2] = y.z;
+      w[4 * g + 3] = y.w;
+    }
+    ptx::tmem_st32(tmem + lane_off + kColQT + 32 * cb, w);
+  }
+#pragma unroll 1
+  for (int bx = 2 * hf; bx < 2 * hf + 2; ++bx) {
+    uint4 x[8];
+#pragma unroll
+    for (int g = 0; g < 8; ++g) x[g] = real ? __ldg(qg + 32 + 8 * bx + g) : zero;
+#pragma unroll
+    for (int g = 0; g < 8; ++g)
+      *reinterpret_cast<uint4*>(qreg + bx * kChunkBytes + m * 128 + ((g ^ (m & 7)) << 4)) = conv(x[g]);
+  }
+#pragma unroll
+  for (int g = 4 * hf; g < 4 * hf + 4; ++g)
+    *reinterpret_cast<uint4*>(qreg + 4 * kChunkBytes + m * 128 + ((g ^ (m & 7)) << 4)) = real ? __ldg(rg + g) : zero;
+  ptx::tmem_wait_st();
 }
 
 // ---------------------------------------------------------------------------
@@ -1425,6 +1700,14 @@ __device__ __forceinline__ void softmax_epilogue(const Params& p, const Ctx& c, 
   auto take_qt = [&](int k, int bb) -> bool {
     if constexpr (kK8) {
       qinv_next = quantize_q<Out>(p, bb, rank, m, hf, smem + S::kQ, tmem, lane_off);
+      ptx::fence_proxy_async_smem();
+      ptx::tc_fence_before();
+      __syncwarp();
+      if (lane == 0) ptx::mbar_arrive_cluster(qt_full_leader);
+      return true;
+    }
+    if constexpr (Io<T>::kKv4) {
+      load_q_f16<Out>(p, bb, rank, m, hf, smem + S::kQ, tmem, lane_off);
       ptx::fence_proxy_async_smem();
       ptx::tc_fence_before();
       __syncwarp();
@@ -1836,7 +2119,9 @@ __device__ __forceinline__ void softmax_epilogue(const Params& p, const Ctx& c, 
 // the kernel: warp 0 K producer, warp 1 TMEM owner + QK^T issuer, warp 2 V
 // producer, warp 3 P.V issuer, warps 4..7 softmax/epilogue, warp 8 Q loader
 // (warps 9..11 complete the third warpgroup).  For an FP8 cache the block has
-// 16 warps: warp 2 also prefetches Q, and warps 8..15 convert V to fp16.  The
+// 16 warps: warp 2 also prefetches Q, and warps 8..15 convert V to fp16.  For a
+// 4-bit cache likewise, with warp 0 loading the rope rows only, no V producer and the
+// converters filling the slots of both GEMMs.  The
 // Cv variant has 16 warps too: warps 12..15 rewrite each landed V stage (tail
 // rows zeroed, bf16 -> fp16 with kF16); warps 9..11 are idle.  In the plain
 // variants warp 9 zeroes the tail rows of a sequence's last V units.
@@ -1858,16 +2143,19 @@ mla_sm100_decode_kernel(const __grid_constant__ Params p) {
 
   if (threadIdx.x == 0) {
     // V operand stages: one expect-tx arrival (TMA), or FP8: kConvWarps converter warps x 2 CTAs
-    const uint32_t n_vfull = Io<T>::kKv8 ? 2u * kConvWarps : (Io<T>::kConv ? 2u * kFixWarps : 1u);
+    // (4-bit: a slot filled for QK^T by both CTAs' converters, refilled for P.V by one's)
+    const uint32_t n_vfull = Io<T>::kKv4   ? (uint32_t)kConvWarps
+                             : Io<T>::kKv8 ? 2u * kConvWarps
+                                           : (Io<T>::kConv ? 2u * kFixWarps : 1u);
     for (int s = 0; s < 8; ++s) {
-      ptx::mbar_init(ptx::smem_u32(&bars->kfull[s]), 1);
+      ptx::mbar_init(ptx::smem_u32(&bars->kfull[s]), Io<T>::kKv4 ? 2u * kConvWarps : 1u);
       ptx::mbar_init(ptx::smem_u32(&bars->kempty[s]), 1);
       ptx::mbar_init(ptx::smem_u32(&bars->vfull[s]), n_vfull);
       ptx::mbar_init(ptx::smem_u32(&bars->vempty[s]), 1);
     }
     for (int s = 0; s < 8; ++s) {
       ptx::mbar_init(ptx::smem_u32(&bars->v8full[s]), 1);
-      ptx::mbar_init(ptx::smem_u32(&bars->v8empty[s]), kConvWarps);
+      ptx::mbar_init(ptx::smem_u32(&bars->v8empty[s]), Io<T>::kKv4 ? 1u : (uint32_t)kConvWarps);
       ptx::mbar_init(ptx::smem_u32(&bars->vfix[s]), 2);
     }
     ptx::mbar_init(ptx::smem_u32(&bars->q_full), 1);
@@ -1897,10 +2185,12 @@ mla_sm100_decode_kernel(const __grid_constant__ Params p) {
     ptx::fence_mbarrier_init();
   }
   if (warp == 0 && lane == 0) {
-    ptx::prefetch_tensormap(&p.tm_kv);
     ptx::prefetch_tensormap(&p.tm_kpe);
-    ptx::prefetch_tensormap(&p.tm_q);
-    ptx::prefetch_tensormap(&p.tm_qpe);
+    if (!Io<T>::kKv4) {
+      ptx::prefetch_tensormap(&p.tm_kv);
+      ptx::prefetch_tensormap(&p.tm_q);
+      ptx::prefetch_tensormap(&p.tm_qpe);
+    }
     ptx::prefetch_tensormap(&p.tm_out);
     if (p.part_o != nullptr) ptx::prefetch_tensormap(&p.tm_part);
   }
@@ -1932,7 +2222,7 @@ mla_sm100_decode_kernel(const __grid_constant__ Params p) {
     ptx::setmaxnreg_dec<kRegsLow>();
   if (warp == 0) {
     if (lane == 0) k_producer<T>(p, c, rank, pair, sbase, bars);
-  } else if (warp == 8 && !Io<T>::kKv8) {
+  } else if (warp == 8 && !Io<T>::kKv8 && !Io<T>::kKv4) {
     if (lane == 0) q_loader<T>(p, c, rank, pair, sbase, bars);
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
@@ -1943,19 +2233,24 @@ mla_sm100_decode_kernel(const __grid_constant__ Params p) {
     }
   } else if (warp == 2) {
     // (FP8: the Q loader only prefetches and never waits; it runs here first)
-    if (Io<T>::kKv8 && lane == 0) q_loader<T>(p, c, rank, pair, sbase, bars);
-    if (lane == 0) v_producer<T>(p, c, rank, pair, sbase, bars);
+    if ((Io<T>::kKv8 || Io<T>::kKv4) && lane == 0) q_loader<T>(p, c, rank, pair, sbase, bars);
+    if constexpr (!Io<T>::kKv4) {
+      if (lane == 0) v_producer<T>(p, c, rank, pair, sbase, bars);
+    }
   } else if (warp == 3) {
     if (rank == 0 && lane == 0) {
       pv_issuer<T>(p, c, pair, sbase, tmem, bars);
       ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->drain_pv), 0x1);
       wait_bar(c, ptx::smem_u32(&bars->drain_pv), 0u, kErrDrain);
     }
+  } else if (Io<T>::kKv4 && warp >= 8) {
+    // 4-bit: warps 8..15 widen the codes
+    if constexpr (Io<T>::kKv4) kv4_converter<T>(p, c, rank, pair, smem, bars, (warp - 8) * 32 + lane, lane);
   } else if (Io<T>::kKv8 && warp >= 8) {
     // FP8: warps 8..15 dequantize the V units
-    v_converter<T>(p, c, pair, smem, bars, (warp - 8) * 32 + lane, lane);
-  } else if (warp == 9 && !Io<T>::kKv8 && !Io<T>::kConv) {
-    v_tailfix<T>(p, c, rank, pair, smem, bars, lane);
+    if constexpr (Io<T>::kKv8) v_converter<T>(p, c, pair, smem, bars, (warp - 8) * 32 + lane, lane);
+  } else if (warp == 9 && !Io<T>::kKv8 && !Io<T>::kKv4 && !Io<T>::kConv) {
+    if constexpr (!Io<T>::kKv4) v_tailfix<T>(p, c, rank, pair, smem, bars, lane);
   } else if (warp >= 12) {
     if constexpr (Io<T>::kConv) v_fix<T>(p, c, pair, smem, bars, (warp - 12) * 32 + lane, lane);
   }
@@ -2494,15 +2789,17 @@ cudaError_t device_info(int dev, DeviceInfo* out) {
   std::lock_guard<std::mutex> lock(g_dev_mutex);
   DeviceInfo& d = g_dev[dev];
   if (!d.ready) {
-    int n[5] = {0, 0, 0, 0, 0};
+    int n[7] = {0, 0, 0, 0, 0, 0, 0};
     cudaError_t err = set_attrs_and_count<__nv_bfloat16>(&n[0]);
     if (err == cudaSuccess) err = set_attrs_and_count<__half>(&n[1]);
     if (err == cudaSuccess) err = set_attrs_and_count<Kv8<__nv_bfloat16>>(&n[2]);
     if (err == cudaSuccess) err = set_attrs_and_count<Kv8<__half>>(&n[3]);
     if (err == cudaSuccess) err = set_attrs_and_count<Cv<__nv_bfloat16, true>>(&n[4]);
+    if (err == cudaSuccess) err = set_attrs_and_count<Kv4<__nv_bfloat16>>(&n[5]);
+    if (err == cudaSuccess) err = set_attrs_and_count<Kv4<__half>>(&n[6]);
     if (err != cudaSuccess) return err;
     d.max_pairs = n[0];
-    for (int i = 1; i < 5; ++i) d.max_pairs = n[i] < d.max_pairs ? n[i] : d.max_pairs;
+    for (int i = 1; i < 7; ++i) d.max_pairs = n[i] < d.max_pairs ? n[i] : d.max_pairs;
     int coop = 0;
     if (cudaDeviceGetAttribute(&coop, cudaDevAttrCooperativeLaunch, dev) != cudaSuccess) {
       cudaGetLastError();
@@ -2642,19 +2939,20 @@ cudaError_t launch_variant(const sm100::Params& p, int pairs, cudaStream_t strea
 
 cudaError_t launch_sm100_combine(const DecodeArgs& a);
 
-cudaError_t launch_sm100_decode_plain_then_combine(const DecodeArgs& a, const sm100::Params& p) {
+// The variant of a call, by its cache's form and the model's type.
+cudaError_t launch_form(const DecodeArgs& a, const sm100::Params& p) {
   using namespace sm100;
   const int pairs = a.plan.bpc;
-  cudaError_t err;
+  const bool bf16 = a.dtype == MLA_DTYPE_BF16;
+  if (a.kv_scales != nullptr)
+    return bf16 ? launch_variant<Kv4<__nv_bfloat16>>(p, pairs, a.stream)
+                : launch_variant<Kv4<__half>>(p, pairs, a.stream);
   if (a.kv_fp8)
-    err = a.dtype == MLA_DTYPE_BF16 ? launch_variant<Kv8<__nv_bfloat16>>(p, pairs, a.stream)
-                                    : launch_variant<Kv8<__half>>(p, pairs, a.stream);
-  else if (a.dtype == MLA_DTYPE_BF16)
-    err = kConvV ? launch_variant<Cv<__nv_bfloat16, true>>(p, pairs, a.stream)
-                 : launch_variant<__nv_bfloat16>(p, pairs, a.stream);
-  else
-    err = launch_variant<__half>(p, pairs, a.stream);
-  return err == cudaSuccess ? launch_sm100_combine(a) : err;
+    return bf16 ? launch_variant<Kv8<__nv_bfloat16>>(p, pairs, a.stream)
+                : launch_variant<Kv8<__half>>(p, pairs, a.stream);
+  if (!bf16) return launch_variant<__half>(p, pairs, a.stream);
+  return kConvV ? launch_variant<Cv<__nv_bfloat16, true>>(p, pairs, a.stream)
+                : launch_variant<__nv_bfloat16>(p, pairs, a.stream);
 }
 
 namespace sm100 {
@@ -2666,7 +2964,7 @@ namespace sm100 {
 struct MapKey {
   const void *q, *q_pe, *kv, *k_pe, *out, *part_o;
   long long part_rows, kv_rows;
-  int g, qb, kv_heads, dtype, out_f32, kv_fp8;
+  int g, qb, kv_heads, dtype, out_f32, form;   // form: 0 model type, 1 e4m3, 2 4-bit
   bool operator==(const MapKey& o) const { return memcmp(this, &o, sizeof(MapKey)) == 0; }
 };
 struct MapEntry {
@@ -2690,7 +2988,7 @@ bool tensor_maps(const DecodeArgs& a, const QShape& qs, Params* p) {
   key.kv_heads = qs.kv_heads;
   key.dtype = a.dtype;
   key.out_f32 = p->out_f32;
-  key.kv_fp8 = a.kv_fp8;
+  key.form = a.kv_scales != nullptr ? 2 : a.kv_fp8;
   constexpr int kSlots = 8;
   thread_local MapEntry cache[kSlots];
   thread_local int filled = 0, next = 0;
@@ -2708,11 +3006,13 @@ bool tensor_maps(const DecodeArgs& a, const QShape& qs, Params* p) {
   const CUtensorMapDataType dt =
       a.dtype == MLA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
   const uint64_t kv_rows = (uint64_t)key.kv_rows;
-  const bool ok_kv = a.kv_fp8 ? make_map_kv(&p->tm_kv, a.kv, kDim, qs.kv_heads, kv_rows,
+  // (4-bit: the latent codes are read without a tensor map, and so is Q)
+  const bool ok_kv = key.form == 2 ? true : a.kv_fp8 ? make_map_kv(&p->tm_kv, a.kv, kDim, qs.kv_heads, kv_rows,
                                             CU_TENSOR_MAP_DATA_TYPE_UINT8, 1)
                                : make_map_kv(&p->tm_kv, a.kv, kDim, qs.kv_heads, kv_rows, dt);
-  if (!ok_kv || !make_map_kv(&p->tm_kpe, a.k_pe, kPeDim, qs.kv_heads, kv_rows, dt) ||
-      !make_map3(&p->tm_q, a.q, kDim, qs.g, qs.qb, dt) || !make_map3(&p->tm_qpe, a.q_pe, kPeDim, qs.g, qs.qb, dt))
+  if (!ok_kv || !make_map_kv(&p->tm_kpe, a.k_pe, kPeDim, qs.kv_heads, kv_rows, dt)) return false;
+  if (key.form != 2 && (!make_map3(&p->tm_q, a.q, kDim, qs.g, qs.qb, dt) ||
+                        !make_map3(&p->tm_qpe, a.q_pe, kPeDim, qs.g, qs.qb, dt)))
     return false;
   if (!(p->out_f32 ? make_map3(&p->tm_out, a.out, kDim, qs.g, qs.qb, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4)
                    : make_map3(&p->tm_out, a.out, kDim, qs.g, qs.qb, dt)))
@@ -2779,23 +3079,17 @@ cudaError_t launch_sm100_decode(const DecodeArgs& a, int variant) {
   p.block_table = a.block_table;
   p.page_size = a.page_size;
   p.max_pages = a.max_pages;
+  p.num_pages = a.num_pages;
+  p.kv_scales = static_cast<const __half*>(a.kv_scales);
   p.kv_scale = a.kv_fp8 ? a.kv_scale : 1.f;
-  cudaError_t lerr;
-  if (a.kv_fp8) {
-    lerr = a.dtype == MLA_DTYPE_BF16 ? launch_variant<Kv8<__nv_bfloat16>>(p, pairs, a.stream)
-                                     : launch_variant<Kv8<__half>>(p, pairs, a.stream);
-  } else if (a.dtype == MLA_DTYPE_BF16) {
-    lerr = kConvV ? launch_variant<Cv<__nv_bfloat16, true>>(p, pairs, a.stream)
-                  : launch_variant<__nv_bfloat16>(p, pairs, a.stream);
-  } else {
-    lerr = launch_variant<__half>(p, pairs, a.stream);
-  }
+  const cudaError_t lerr = launch_form(a, p);
   if (lerr != cudaSuccess && p.coop) {
     // the cooperative launch was refused: the plain launch, and the combine launch
     // merges what the kernel then leaves
     cudaGetLastError();
     p.coop = 0;
-    return launch_sm100_decode_plain_then_combine(a, p);
+    const cudaError_t perr = launch_form(a, p);
+    return perr == cudaSuccess ? launch_sm100_combine(a) : perr;
   }
   return lerr;
 }

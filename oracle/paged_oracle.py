@@ -143,19 +143,47 @@ def rotate_bound(x, freq, gain, offset=0, interleaved=True):
 def decode(q, q_pe, v, k_pe, scale):
     """One query sequence: q [h, 512], q_pe [h, 64], rows v [n, 512], k_pe [n, 64] (float64).
 
-    Returns (out, lse, spread): spread [h, 512] bounds the error of a kernel that rounds
+    Returns (out, lse, spread, ds): spread [h, 512] bounds the error of a kernel that rounds
     each weight and each row value once to fp16 (half a step, 2^-11 relative, each) and the
     row values in the scores too: with ds >= |error of a score|, a weight is off by at most
     exp(2 ds) - 1 relative, so the output by (2 ds + 2 * 2^-11) sum p |v| to first order
-    (a twentieth is added for the rest and for float32 sums).
+    (a twentieth is added for the rest).  A weight below fp16's normal range (2^-14 of the
+    row's largest) is off by up to half the smallest step, 2^-25 of the largest weight,
+    hence 2^-25 sum |v| / z.  ds counts, beside the row values, the float32 sums of 576
+    products: each sum is off by at most 2^-23 (truncated) of the magnitudes' sum, together
+    below 2^-13 of it.  The log-sum-exp is off by at
+    most ds [h, 1], the largest error of a score.
     """
     if len(v) == 0:
-        return np.zeros(q.shape), np.full(len(q), -math.inf), np.zeros(q.shape)
+        return np.zeros(q.shape), np.full(len(q), -math.inf), np.zeros(q.shape), np.zeros((len(q), 1))
     s = (q @ v.T + q_pe @ k_pe.T) * scale
     m = s.max(-1, keepdims=True)
     p = np.exp(s - m)
     z = p.sum(-1, keepdims=True)
     p /= z
     half = 2.0 ** -11
-    ds = (half * scale * (np.abs(q) @ np.abs(v).T)).max(-1, keepdims=True) + 1e-5
-    return p @ v, (np.log(z) + m)[:, 0], 1.05 * (2 * ds + 2 * half) * (p @ np.abs(v))
+    mags = np.abs(q) @ np.abs(v).T
+    sums = mags + np.abs(q_pe) @ np.abs(k_pe).T
+    ds = scale * (half * mags + 2.0 ** -13 * sums).max(-1, keepdims=True) + 1e-5
+    return p @ v, (np.log(z) + m)[:, 0], \
+        1.05 * (2 * ds + 2 * half) * (p @ np.abs(v)) + 2.0 ** -25 * np.abs(v).sum(0) / z, ds
+
+
+def rounding_gate(q, q_pe, v, k_pe, scale, dtype):
+    """What relative L2 distance from the rounded result such a kernel is expected to have, as
+    a square.  A rounding to fp16 is off by a uniform share of half a step, 2^-11 / m relative
+    for a mantissa m in [1, 2), log-uniform: rms r = 2^-11 sqrt(0.541 / 3) = 2.07e-4.  A
+    weight and a row value are rounded once each, and the row values move a score by
+    r scale sqrt(sum q^2 v^2) (rms), that is the weight by as much relative: together
+    d = r sqrt(2 + scale^2 sum q^2 v^2).  The result is then rounded to steps of 2^-7 / m
+    (bf16; fp16 2^-10 / m) of it, 0.72 of that on average: with probability |error| / step it
+    lands on the other neighbour, a whole step away, hence d^2 + step E|error| with
+    E|error| = 0.8 d for a normal error.
+    """
+    s = (q @ v.T + q_pe @ k_pe.T) * scale
+    p = np.exp(s - s.max(-1, keepdims=True))
+    p /= p.sum(-1, keepdims=True)
+    r2 = 2.0 ** -22 * 0.541 / 3
+    d2 = r2 * (2 + scale ** 2 * (p * ((q * q) @ (v * v).T)).sum(-1).mean())
+    step = 0.72 * (2.0 ** -7 if dtype == "bf16" else 2.0 ** -10)
+    return d2 + step * 0.8 * math.sqrt(d2)
