@@ -86,4 +86,15 @@ struct Int4Args {
 int int4_simt_splits(int qb, int g, int max_len, int asked);
 cudaError_t launch_int4_simt(const Int4Args& a, int ns, cudaStream_t stream);
 
+// Warp-level MMA kernel for few query rows (mla_int4_mma.cu): groups of 16 row_tiles
+// query rows (row_tiles 1 or 2) of a KV sequence; workspace [status 256 B][info][partial
+// LSE][partial O], the status word zero before the first call.
+struct Int4MmaPlan {
+  int row_tiles, groups, workers;
+  long long units;      // (sequence, KV head, row group) triples
+  size_t info_off, lse_off, o_off, total;
+};
+Int4MmaPlan int4_mma_plan(int batch, int q_len, int heads, int kv_heads, int max_len, int row_tiles, int asked);
+cudaError_t launch_int4_mma(Int4Args a, const Int4MmaPlan& plan, void* workspace, cudaStream_t stream);
+
 }  // namespace mla

@@ -11,10 +11,16 @@ namespace {
 
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
+enum Int4Kernel { kSimt, kPair, kMma };
+// The warp-level kernel takes calls of up to this many query rows per KV head.
+constexpr int kMmaRows = 64;
+
 struct Int4Plan {
-  bool tc;          // tensor-core kernel; else the CUDA-core kernel with `splits` splits
-  int splits;
-  size_t lse_off, o_off, total;
+  Int4Kernel kernel;
+  int splits;       // CUDA-core kernel
+  Int4MmaPlan mma;
+  size_t lse_off, o_off;
+  size_t total;     // workspace bytes
 };
 
 int plan_call(const char* fn, int batch, int q_len, int heads, int kv_heads, int max_seqlen_kv, int dtype,
@@ -41,17 +47,29 @@ int plan_call(const char* fn, int batch, int q_len, int heads, int kv_heads, int
     set_error("%s: num_split must be in [0, 8192] and kernel a MlaKernelKind (got %d, %d)", fn, asked, kernel);
     return MLA_ERR_ARG;
   }
-  const bool covered = sm100_supports_ext(batch, q_len, heads, kv_heads, max_seqlen_kv);
-  if (kernel == MLA_KERNEL_TC && !covered) {
-    set_error("%s: shape outside the tensor-core kernel (batch %d, q_len %d, heads %d, kv_heads %d, max_seqlen_kv %d)",
-              fn, batch, q_len, heads, kv_heads, max_seqlen_kv);
-    return MLA_ERR_UNSUPPORTED;
-  }
-  p->tc = kernel != MLA_KERNEL_SIMT && covered;
-  if (p->tc) {
+  if (kernel != MLA_KERNEL_SIMT) {
+    const int rows = q_len * (heads / kv_heads);
+    const bool covered = sm100_supports_ext(batch, q_len, heads, kv_heads, max_seqlen_kv);
+    // block_H, query rows per CTA: up to 32 asks for the warp-level kernel, more for the pair kernel
+    const int block_h = cfg != nullptr ? cfg->block_H : 0;
+    const bool mma = block_h > 0 ? block_h <= 32 : (rows <= kMmaRows || !covered);
+    if (mma) {
+      p->kernel = kMma;
+      p->mma = int4_mma_plan(batch, q_len, heads, kv_heads, max_seqlen_kv, (block_h > 0 ? block_h : rows) <= 16 ? 1 : 2,
+                             asked);
+      p->total = p->mma.total;
+      return MLA_OK;
+    }
+    if (!covered) {
+      set_error("%s: shape outside the pair kernel (batch %d, q_len %d, heads %d, kv_heads %d, max_seqlen_kv %d)", fn,
+                batch, q_len, heads, kv_heads, max_seqlen_kv);
+      return MLA_ERR_UNSUPPORTED;
+    }
+    p->kernel = kPair;
     p->total = ext_int4_workspace(fn, batch, q_len, heads, kv_heads, max_seqlen_kv, dtype, cfg);
     return p->total > 0 ? MLA_OK : MLA_ERR_ARG;
   }
+  p->kernel = kSimt;
   p->splits = int4_simt_splits((int)qb, heads / kv_heads, max_seqlen_kv, asked);
   const size_t rows = p->splits > 1 ? (size_t)p->splits * batch * q_len * heads : 0;
   p->lse_off = 0;
@@ -93,7 +111,7 @@ int32_t mla_decode_ext_int4kv(const void* q, const void* q_pe, const void* kv_co
     set_error(kv_scales ? "%s: tensor pointers must be 16-byte aligned" : "%s: null pointer", fn);
     return MLA_ERR_ARG;
   }
-  if (p.tc)
+  if (p.kernel == kPair)
     return decode_ext_int4(fn, q, q_pe, kv_codes, kv_scales, k_pe_cache, block_table, cache_seqlens, out, lse,
                            workspace, workspace_bytes, batch, q_len, heads, kv_heads, max_seqlen_kv, page_size,
                            num_pages, max_pages_per_seq, dtype, cfg, stream);
@@ -128,8 +146,10 @@ int32_t mla_decode_ext_int4kv(const void* q, const void* q_pe, const void* kv_co
   a.seqlens = cache_seqlens;
   a.out = out;
   a.lse = lse;
-  a.part_lse = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.lse_off);
-  a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.o_off);
+  if (p.kernel == kSimt) {
+    a.part_lse = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.lse_off);
+    a.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + p.o_off);
+  }
   a.batch = batch;
   a.q_len = q_len;
   a.heads = heads;
@@ -147,7 +167,8 @@ int32_t mla_decode_ext_int4kv(const void* q, const void* q_pe, const void* kv_co
     set_error("%s: softmax_scale must be finite and > 0", fn);
     return MLA_ERR_ARG;
   }
-  const cudaError_t err = launch_int4_simt(a, p.splits, static_cast<cudaStream_t>(stream));
+  const cudaError_t err = p.kernel == kMma ? launch_int4_mma(a, p.mma, workspace, static_cast<cudaStream_t>(stream))
+                                           : launch_int4_simt(a, p.splits, static_cast<cudaStream_t>(stream));
   if (err != cudaSuccess) {
     set_error("%s: launch failed: %s", fn, cudaGetErrorString(err));
     return MLA_ERR_CUDA;

@@ -252,6 +252,7 @@ struct Barriers {
   uint64_t qts, qtr;     // Q dims [0, 256) staged in shared memory / copied to TMEM
   uint64_t q_go;         // the first piece's Q loads are issued: K and V loads may start
   uint64_t drain_qk, drain_pv;
+  uint64_t mapfull[2], mapempty[2];   // 4-bit variant: batches of tile rows (TileRows)
 };
 static_assert(sizeof(Barriers) <= 1024, "barrier block");
 
@@ -270,7 +271,8 @@ struct Smem {
   static constexpr uint32_t kXmax = kBar + 1024;
   static constexpr uint32_t kXl = kXmax + 2 * 128 * 4;
   static constexpr uint32_t kMisc = kXl + 128 * 4;
-  static constexpr uint32_t kBytes = kMisc + 64 + 1024;   // + alignment slack
+  static constexpr uint32_t kMap = kMisc + 64;   // 4-bit variant: two batches of TileRows
+  static constexpr uint32_t kBytes = kMap + (Io<T>::kKv4 ? 1024 : 0) + 1024;   // + alignment slack
   static_assert(kBytes <= 232448, "shared memory");
   static_assert(kBar >= kMergeTab + 6 * 1024, "cooperative merge staging");
 };
@@ -315,6 +317,7 @@ struct Params {
   const int* seqlens;      // [real batch] KV rows per sequence, or nullptr (all seqlen)
   const int* block_table;  // [real batch][max_pages] page ids, or nullptr (contiguous rows)
   int page_size, max_pages, num_pages;
+  int num_rows;            // rows of the cache
   float sl2;            // softmax scale * log2(e)
 };
 
@@ -350,6 +353,12 @@ __device__ __forceinline__ bool wait_bar_slow(const Ctx& c, uint32_t bar, uint32
 // Bounded wait for the phase of `parity` on a local barrier.
 __device__ __forceinline__ bool wait_bar(const Ctx& c, uint32_t bar, uint32_t parity, uint32_t code) {
   return ptx::mbar_try_wait(bar, parity) || wait_bar_slow(c, bar, parity, code);
+}
+
+// The same by every lane of a warp, with one result for all (so that a warp whose lanes
+// go on to warp-wide instructions gives up as one).
+__device__ __forceinline__ bool wait_warp(const Ctx& c, uint32_t bar, uint32_t parity, uint32_t code) {
+  return __all_sync(0xffffffffu, wait_bar(c, bar, parity, code)) != 0;
 }
 
 __device__ __forceinline__ bool aborted(const Ctx& c) {
@@ -488,10 +497,10 @@ __device__ __forceinline__ int kv_row(const Params& p, int seq, int row, int len
 // First cache row of the 64 rows from `row` (a multiple of 64) of sequence `seq`, or -1
 // when the block table names a page the cache does not have (64-row runs never straddle
 // pages).  row < the sequence's length.
-__device__ __forceinline__ long long kv_row64(const Params& p, int seq, int row) {
-  if (p.block_table == nullptr) return (long long)seq * p.seqlen + row;
+__device__ __forceinline__ int kv_row64(const Params& p, int seq, int row) {
+  if (p.block_table == nullptr) return seq * p.seqlen + row;   // (the host keeps rows below 2^31)
   const int pg = __ldg(p.block_table + (size_t)seq * p.max_pages + row / p.page_size);
-  return (unsigned)pg < (unsigned)p.num_pages ? (long long)pg * p.page_size + row % p.page_size : -1;
+  return (unsigned)pg < (unsigned)p.num_pages ? pg * p.page_size + row % p.page_size : -1;
 }
 
 // Position in a ring of `kStages` shared-memory stages.
@@ -507,11 +516,81 @@ struct Ring {
 };
 
 // ---------------------------------------------------------------------------
+// 4-bit variant: where the rows of each tile of this pair's range are, in shared
+// memory.  Finding a tile's rows is a chain of dependent loads (prefix sums, length,
+// block table: 2,500 cycles a tile when the converter warps walked it themselves); warp
+// 2 does it for 32 tiles at once, one a lane, two batches ahead.
+// ---------------------------------------------------------------------------
+struct TileRows {
+  int own, peer;   // first cache row of this CTA's / the peer's 64 rows, -1: none
+  int valid;       // rows within the length: own | peer << 8; kFirst, kLast tile of a piece
+  int kvh;
+};
+constexpr int kMapBatch = 32;
+constexpr int kFirst = 1 << 16, kLast = 1 << 17;
+constexpr uint32_t kMapReaders = 9;   // eight converter warps and the rope producer; CTA 0: the two issuers too
+
+template <typename T>
+__device__ __forceinline__ void tile_scout(const Params& p, const Ctx& c, uint32_t rank, int pair, uint8_t* smem,
+                                           Barriers* bars, int lane) {
+  TileRows* ring = reinterpret_cast<TileRows*>(smem + Smem<T>::kMap);
+  const uint32_t full0 = ptx::smem_u32(&bars->mapfull[0]), empty0 = ptx::smem_u32(&bars->mapempty[0]);
+  const PieceIter it(p, pair);
+  const uint32_t n = it.t1 - it.t;
+#pragma unroll 1
+  for (uint32_t k = 0; k * kMapBatch < n; ++k) {
+    const uint32_t i = k * kMapBatch + lane;
+    TileRows w{-1, -1, 0, 0};
+    if (i < n) {
+      const int v = it.m.seq_of(it.t + i), len = seq_len(p, v), seq = vseq_kvseq(p, v);
+      const uint32_t x = it.t + i, v0 = it.m.first(v);
+      const int j = (int)(x - v0);
+      w.kvh = vseq_kvh(p, v);
+      if (i == 0 || x == v0) w.valid |= kFirst;
+      if (i == n - 1 || x + 1 == it.m.first(v + 1)) w.valid |= kLast;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = j * kTile + 64 * h;
+        if (row >= len) continue;
+        const int first = kv_row64(p, seq, row), count = len - row < 64 ? len - row : 64;
+        if (first < 0) continue;
+        (h == (int)rank ? w.own : w.peer) = first;
+        w.valid |= count << (h == (int)rank ? 0 : 8);
+      }
+    }
+    if (k >= 2 && !wait_warp(c, empty0 + 8 * (k & 1u), ((k - 2) >> 1) & 1u, kErrKLoad)) return;
+    ring[(k & 1u) * kMapBatch + lane] = w;
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive_local(full0 + 8 * (k & 1u));
+  }
+}
+
+// A reader (a whole warp, or one thread): tile 0, 1, 2, ... in order.
+template <bool kWarp>
+struct TileMapReader {
+  const TileRows* ring;
+  uint32_t full0, empty0;
+  __device__ __forceinline__ TileMapReader(const TileRows* r, Barriers* bars)
+      : ring(r), full0(ptx::smem_u32(&bars->mapfull[0])), empty0(ptx::smem_u32(&bars->mapempty[0])) {}
+  __device__ __forceinline__ bool get(const Ctx& c, uint32_t i, TileRows* w) const {
+    const uint32_t k = i / kMapBatch, full = full0 + 8 * (k & 1u), ph = (k >> 1) & 1u;
+    if (i % kMapBatch == 0 && !(kWarp ? wait_warp(c, full, ph, kErrKLoad) : wait_bar(c, full, ph, kErrKLoad)))
+      return false;
+    *w = ring[i % (2 * kMapBatch)];
+    if (i % kMapBatch == kMapBatch - 1) {
+      if (kWarp) __syncwarp();
+      if (!kWarp || (threadIdx.x & 31) == 0) ptx::mbar_arrive_local(empty0 + 8 * (k & 1u));
+    }
+    return true;
+  }
+};
+
+// ---------------------------------------------------------------------------
 // K producer: Q once per piece, then per tile 4 latent units + 1 rope unit.
 // ---------------------------------------------------------------------------
 template <typename T>
 __device__ __forceinline__ void k_producer(const Params& p, const Ctx& c, uint32_t rank, int pair,
-                                           uint32_t sbase, Barriers* bars) {
+                                           uint8_t* smem, uint32_t sbase, Barriers* bars) {
   using S = Smem<T>;
   constexpr int KS = Cfg<T>::kKStages;
   const bool leader = rank == 0;
@@ -526,23 +605,18 @@ __device__ __forceinline__ void k_producer(const Params& p, const Ctx& c, uint32
     const uint32_t rfull0_leader = ptx::mapa(rfull0, 0);
     const uint32_t rempty0 = ptx::smem_u32(&bars->v8empty[0]);
     const uint64_t once = ptx::l2_policy_evict_first();
-    uint32_t gi = 0;
-    Piece pc;
-    while (it.next(&pc)) {
-      const int kseq = vseq_kvseq(p, pc.bb), kvh = vseq_kvh(p, pc.bb), klen = seq_len(p, pc.bb);
-#pragma unroll 1
-      for (int j = pc.first; j < pc.end; ++j, ++gi) {
-        const uint32_t b = gi & 1u;
-        const int row = j * kTile + 64 * (int)rank;
-        // rows past the length are masked (any row will do); a row on a page outside the
-        // cache reads as zeros: the row past the last is out of the tensor map's range
-        long long y = row < klen ? kv_row64(p, kseq, row) : 0;
-        if (y < 0) y = p.block_table != nullptr ? (long long)p.num_pages * p.page_size : 0;
-        if (gi >= 2 && !wait_bar(c, rempty0 + 8 * b, ((gi - 2) >> 1) & 1u, kErrKLoad)) return;
-        if (leader) ptx::mbar_arrive_expect_tx(rfull0 + 8 * b, 2 * kChunkBytes);
-        ptx::tma_load_3d_pair_hint(sbase + S::kV8Ring + b * kChunkBytes, &p.tm_kpe, rfull0_leader + 8 * b, 0, kvh,
-                                   (int)y, once);
-      }
+    const TileMapReader<false> map(reinterpret_cast<const TileRows*>(smem + S::kMap), bars);
+    for (uint32_t gi = 0; gi < it.t1 - it.t; ++gi) {
+      const uint32_t b = gi & 1u;
+      TileRows w;
+      if (!map.get(c, gi, &w)) return;
+      // no rows here (masked, or on a page outside the cache): zeros, from past the
+      // tensor map's last row
+      const int y = w.own >= 0 ? w.own : p.num_rows;
+      if (gi >= 2 && !wait_bar(c, rempty0 + 8 * b, ((gi - 2) >> 1) & 1u, kErrKLoad)) return;
+      if (leader) ptx::mbar_arrive_expect_tx(rfull0 + 8 * b, 2 * kChunkBytes);
+      ptx::tma_load_3d_pair_hint(sbase + S::kV8Ring + b * kChunkBytes, &p.tm_kpe, rfull0_leader + 8 * b, 0, w.kvh, y,
+                                 once);
     }
     return;
   }
@@ -633,9 +707,9 @@ __device__ __forceinline__ void q_loader(const Params& p, const Ctx& c, uint32_t
   const uint32_t qtr = ptx::smem_u32(&bars->qtr);
   const uint32_t q_go = ptx::smem_u32(&bars->q_go);
   PieceIter it(p, pair);
-  if constexpr (Io<T>::kKv8 || Io<T>::kKv4) {
-    // FP8 and 4-bit: the softmax warps read each piece's Q rows from global memory
-    // (they convert them); this thread only pulls the rows into L2 ahead of time
+  if constexpr (Io<T>::kKv8) {
+    // FP8: the softmax warps read each piece's Q rows from global memory (they
+    // quantize them); this thread only pulls the rows into L2 ahead of time
     Piece pq;
     bool first = true;
     while (it.next(&pq)) {
@@ -859,18 +933,18 @@ __device__ __forceinline__ void v_converter(const Params& p, const Ctx& c, int p
 }
 
 // ---------------------------------------------------------------------------
-// 4-bit variant: converter warps (warps 8..15).  Thread ct owns row ct / 4 and scale
-// group ct % 4 of every unit (64 rows x 128 dims): one 16-byte load of 32 codes and one
-// scale in, four 16-byte fp16 granules out.  Per tile: fill the four slots for QK^T
-// (each as soon as P.V of two tiles ago has released it; its register then takes the
-// next tile's load), then refill the two slots whose dims this CTA does not own with
-// the peer's rows for P.V of the tile before (once its QK^T has read them).  In this
-// order QK^T of a tile is issued ahead of P.V of the tile before, under which its
-// softmax runs.  Rows past the length and rows of absent pages become zeros.
+// 4-bit variant: converter warps (warps 8..15).  A thread's share is a row's scale
+// group (32 codes: one 16-byte load and one scale in, four 16-byte fp16 granules out).
+// Filling a tile's four slots for QK^T, warps 2 u and 2 u + 1 take slot u (32 rows each,
+// four shares a thread); refilling two of them with the peer's rows for P.V, four warps
+// take a slot (16 rows each, two shares a thread): a warp waits, fences and signals
+// twice a tile, not once per slot and share.  A fill's registers take the next
+// tile's loads as soon as they are stored.  Rows past the length and rows of absent
+// pages become zeros.
 // ---------------------------------------------------------------------------
 struct Codes32 {
-  uint4 w;      // 32 codes
-  uint32_t s;   // their scale, in both halves
+  uint4 w;            // 32 codes
+  unsigned short s;   // their scale, as loaded (anything done to it here would wait for the load)
 };
 
 __device__ __forceinline__ uint32_t h2_bits(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
@@ -890,110 +964,206 @@ __device__ __forceinline__ uint4 widen8(uint32_t w, __half2 s2) {
                     h2_bits(__hmul2(e, s2)));
 }
 
-// Row r, group g of a unit at `dst` (two SW128 boxes of 64 dims): granule k of the
-// group at (4 (g & 1) + k) ^ (r & 7) of box g / 2.  The second box's threads take their
-// granules in the order 2 3 0 1: the eight threads of a store phase (two rows, four
-// groups) then hit eight distinct granule columns.
-__device__ __forceinline__ void store_codes(uint8_t* dst, int r, int g, const Codes32& x) {
-  const int flip = (g >> 1) << 1;
-  const uint32_t w[4] = {flip ? x.w.z : x.w.x, flip ? x.w.w : x.w.y, flip ? x.w.x : x.w.z, flip ? x.w.y : x.w.w};
-  uint8_t* row = dst + (g >> 1) * kChunkBytes + r * 128;
-  const __half2 s2 = bits_h2(x.s);
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    *reinterpret_cast<uint4*>(row + (((4 * (g & 1) + (k ^ flip)) ^ (r & 7)) << 4)) = widen8(w[k], s2);
-}
+constexpr uint32_t kFillWarps = 2, kRefillWarps = 4;   // per slot (and CTA)
 
 template <typename T>
 __device__ __forceinline__ void kv4_converter(const Params& p, const Ctx& c, uint32_t rank, int pair, uint8_t* smem,
-                                              Barriers* bars, int ct, int lane) {
+                                              Barriers* bars, int cw, int lane) {
   using S = Smem<T>;
-  const uint32_t kfull0_leader = ptx::mapa(ptx::smem_u32(&bars->kfull[0]), 0);
-  const uint32_t vfull0_leader = ptx::mapa(ptx::smem_u32(&bars->vfull[0]), 0);
-  const uint32_t read0 = ptx::smem_u32(&bars->kempty[0]);    // QK^T has read a slot
-  const uint32_t free0 = ptx::smem_u32(&bars->vempty[0]);    // P.V has read a slot
-  uint8_t* ring = smem + S::kKRing;
-  const int r = ct >> 2, g = ct & 3;
-  PieceIter it(p, pair);
-  Piece pc;
-  int j = 0, seq = 0, kvh = 0, len = 0;
-  bool more = it.next(&pc);
-  if (!more) return;
-  j = pc.first;
-  // cache positions ((row * kv_heads + kvh), -1: zeros) of this thread's rows of a tile:
-  // its own half's and the peer half's
-  auto locate = [&](long long* own, long long* peer) {
-    seq = vseq_kvseq(p, pc.bb);
-    kvh = vseq_kvh(p, pc.bb);
-    len = seq_len(p, pc.bb);
-    const int ro = j * kTile + 64 * (int)rank, rp = j * kTile + 64 * (1 - (int)rank);
-    const long long bo = ro < len ? kv_row64(p, seq, ro) : -1, bp = rp < len ? kv_row64(p, seq, rp) : -1;
-    *own = (bo >= 0 && ro + r < len) ? (bo + r) * p.kv_heads + kvh : -1;
-    *peer = (bp >= 0 && rp + r < len) ? (bp + r) * p.kv_heads + kvh : -1;
-  };
-  auto advance = [&]() {
-    if (++j < pc.end) return;
-    more = it.next(&pc);
-    if (more) j = pc.first;
-  };
-  // 32 codes of dims [32 q, +32) (q = 0..15) at position `at`
-  auto load = [&](long long at, int q) -> Codes32 {
-    Codes32 x{make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u), 0u};
-    if (at >= 0) {
+  const TileMapReader<true> map(reinterpret_cast<const TileRows*>(smem + S::kMap), bars);
+  const PieceIter it(p, pair);
+  const uint32_t n = it.t1 - it.t;
+  if (n == 0) return;
+  // lane: row lane & 7 of every eight, group g of the unit.  The eight lanes of a 16-byte
+  // store phase are eight rows of one group, whose granules the swizzle puts in eight
+  // distinct columns: granule k of group g at (4 (g & 1) + k) ^ (row & 7) of box g / 2
+  const int g = lane >> 3;
+  const int u = cw >> 1, fr = 32 * (cw & 1) + (lane & 7);    // fill: slot u, rows fr + 8 e
+  const int nh = cw >> 2, pr = 16 * (cw & 3) + (lane & 7);   // refill: rows pr + 8 e
+  const uint32_t vs = 2 * nh + (1 - rank);                   // refill: slot (of its tile's four)
+  const uint32_t gx = (uint32_t)((4 * (g & 1)) ^ (lane & 7)) << 4;
+  uint8_t* fill_row = smem + S::kKRing + u * kStageBytes + (g >> 1) * kChunkBytes + fr * 128;
+  uint8_t* refill_row = smem + S::kKRing + vs * kStageBytes + (g >> 1) * kChunkBytes + pr * 128;
+  const uint32_t kfull_leader = ptx::mapa(ptx::smem_u32(&bars->kfull[u]), 0);
+  const uint32_t vfull_leader = ptx::mapa(ptx::smem_u32(&bars->vfull[vs]), 0);
+  const uint32_t freed = ptx::smem_u32(&bars->vempty[u]);    // P.V has read the slot
+  const uint32_t read = ptx::smem_u32(&bars->kempty[vs]);    // QK^T has read the slot
+  const int fq = 4 * u + g, pq = 8 * nh + 4 * (int)rank + g;   // scale groups
+  auto load = [&](Codes32& x, long long at, bool real, int q) {
+    x = Codes32{make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u), 0};
+    if (real) {
       x.w = __ldg(reinterpret_cast<const uint4*>(p.kv + at * (kDim / 2)) + q);
-      const uint32_t h = __ldg(reinterpret_cast<const unsigned short*>(p.kv_scales) + at * 16 + q);
-      x.s = h | (h << 16);
+      x.s = __ldg(reinterpret_cast<const unsigned short*>(p.kv_scales) + at * 16 + q);
     }
-    return x;
   };
-  long long own, peer_prev = -1, peer;
-  locate(&own, &peer);
+  auto store = [&](uint8_t* dst, const Codes32& x) {
+    const __half2 s2 = __half2half2(__ushort_as_half(x.s));
+    *reinterpret_cast<uint4*>(dst + gx) = widen8(x.w.x, s2);
+    *reinterpret_cast<uint4*>(dst + (gx ^ 16u)) = widen8(x.w.y, s2);
+    *reinterpret_cast<uint4*>(dst + (gx ^ 32u)) = widen8(x.w.z, s2);
+    *reinterpret_cast<uint4*>(dst + (gx ^ 48u)) = widen8(x.w.w, s2);
+  };
+  TileRows w;
   Codes32 k[4];
+  auto load_fill = [&]() {
+    const long long at = (long long)(w.own + fr) * p.kv_heads + w.kvh;
 #pragma unroll
-  for (int u = 0; u < 4; ++u) k[u] = load(own, 4 * u + g);
-  // refill the two slots of tile i that P.V wants from the peer's rows
-  auto refill = [&](uint32_t i, const Codes32 (&v)[2]) -> bool {
-#pragma unroll
-    for (int nh = 0; nh < 2; ++nh) {
-      const uint32_t slot = 4 * (i & 1u) + 2 * nh + (1 - rank);
-      if (!wait_bar(c, read0 + 8 * slot, (i >> 1) & 1u, kErrVLoad)) return false;
-      store_codes(ring + slot * kStageBytes, r, g, v[nh]);
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(vfull0_leader + 8 * slot);
-    }
-    return true;
+    for (int e = 0; e < 4; ++e) load(k[e], at + (long long)(8 * e) * p.kv_heads, fr + 8 * e < (w.valid & 255), fq);
   };
-  uint32_t gi = 0;
+  if (!map.get(c, 0, &w)) return;
+  load_fill();
 #pragma unroll 1
-  while (more) {
-    advance();
-    long long own_next = -1, peer_next = -1;
-    if (more) locate(&own_next, &peer_next);
+  for (uint32_t gi = 0; gi < n; ++gi) {
+    const uint32_t b = gi & 1u, ph = (gi >> 1) & 1u;
     Codes32 v[2];
-    if (gi > 0) {
+    {
+      const long long at = (long long)(w.peer + pr) * p.kv_heads + w.kvh;
 #pragma unroll
-      for (int nh = 0; nh < 2; ++nh) v[nh] = load(peer_prev, 8 * nh + 4 * (int)rank + g);
+      for (int e = 0; e < 2; ++e)
+        load(v[e], at + (long long)(8 * e) * p.kv_heads, pr + 8 * e < ((w.valid >> 8) & 255), pq);
     }
+    // ---- fill slot u
+    if (gi >= 2 && !wait_warp(c, freed + 32 * b, ph ^ 1u, kErrKLoad)) return;
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const uint32_t slot = 4 * (gi & 1u) + u;
-      if (gi >= 2 && !wait_bar(c, free0 + 8 * slot, ((gi - 2) >> 1) & 1u, kErrKLoad)) return;
-      store_codes(ring + slot * kStageBytes, r, g, k[u]);
-      ptx::fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) ptx::mbar_arrive_cluster(kfull0_leader + 8 * slot);
-      k[u] = load(own_next, 4 * u + g);
+    for (int e = 0; e < 4; ++e) store(fill_row + b * 4 * kStageBytes + 8 * e * 128, k[e]);
+    // the tensor core reads the slot through the async proxy
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive_cluster(kfull_leader + 32 * b);
+    if (gi + 1 < n) {
+      if (!map.get(c, gi + 1, &w)) return;
+      load_fill();
     }
-    if (gi > 0 && !refill(gi - 1, v)) return;
-    peer_prev = peer;
-    peer = peer_next;
-    ++gi;
+    // ---- refill slot vs once QK^T has read it
+    if (!wait_warp(c, read + 32 * b, ph, kErrVLoad)) return;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) store(refill_row + b * 4 * kStageBytes + 8 * e * 128, v[e]);
+    ptx::fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) ptx::mbar_arrive_cluster(vfull_leader + 32 * b);
   }
-  Codes32 v[2];
+}
+
+// Issuers of the 4-bit variant (whole warps of the even CTA; one elected lane issues).
+// The tile buffer is a template argument and the loop body two tiles, so that every
+// descriptor is the shared-memory base plus a constant: with run-time stage indexes
+// in one divergent lane a unit of four to eight MMAs took 400 ns to issue, whatever it
+// computed.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t pred;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xffffffff;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(pred));
+  return pred != 0;
+}
+
+template <typename T, uint32_t B>
+__device__ __forceinline__ bool kv4_qk_tile(const Ctx& c, uint32_t sbase, uint32_t tmem, Barriers* bars,
+                                            const TileMapReader<true>& map, uint32_t gi, uint32_t* piece) {
+  using S = Smem<T>;
+  constexpr uint32_t kIdesc = ptx::idesc_f16(0, 128, 128, 0);
+  constexpr uint32_t kIdescRope = ptx::idesc_f16(Cfg<T>::kRopeFmt, 128, 128, 0);
+  constexpr uint32_t kHi = ptx::sw128_desc_hi(1024);
+  const uint32_t ph = (gi >> 1) & 1u;
+  TileRows w;
+  if (!map.get(c, gi, &w)) return false;
+  if (w.valid & kFirst) {
+    if (!wait_warp(c, ptx::smem_u32(&bars->qt_full), *piece & 1u, kErrQK)) return false;
+    ++*piece;
+  }
+  // the softmax warps must have read S[B] of tile gi - 2
+  if (gi >= 2 && !wait_warp(c, ptx::smem_u32(&bars->s_free[B]), ph ^ 1u, kErrQK)) return false;
+  const uint32_t s_tmem = tmem + 64 * B;
+  if (!wait_warp(c, ptx::smem_u32(&bars->v8full[B]), ph, kErrQK)) return false;
+  ptx::tc_fence_after();
+  if (elect_one()) {
+    const uint32_t qa = ptx::sw128_desc_lo(sbase + S::kQ + 4 * kChunkBytes, 16);
+    const uint32_t kb = ptx::sw128_desc_lo(sbase + S::kV8Ring + B * kChunkBytes, 16);
 #pragma unroll
-  for (int nh = 0; nh < 2; ++nh) v[nh] = load(peer_prev, 8 * nh + 4 * (int)rank + g);
-  refill(gi - 1, v);
+    for (int kk = 0; kk < 4; ++kk)
+      ptx::mma_pair_f16(s_tmem, ptx::make_desc(qa + kk * 2, kHi), ptx::make_desc(kb + kk * 2, kHi), kIdescRope,
+                        kk == 0 ? 0u : 1u);
+    ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->v8empty[B]), 0x3);
+  }
+  __syncwarp();
+#pragma unroll
+  for (uint32_t u = 0; u < 4; ++u) {
+    if (!wait_warp(c, ptx::smem_u32(&bars->kfull[4 * B + u]), ph, kErrQK)) return false;
+    ptx::tc_fence_after();
+    if (elect_one()) {
+      const uint32_t kb = ptx::sw128_desc_lo(sbase + S::kKRing + (4 * B + u) * kStageBytes, 16);
+      const uint32_t qa = ptx::sw128_desc_lo(sbase + S::kQ + 2 * (u & 1u) * kChunkBytes, 16);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk) {
+        const uint64_t bd = ptx::make_desc(kb + (kk >> 2) * 512 + (kk & 3) * 2, kHi);
+        if (u < 2)   // dims [0, 256): Q from TMEM, 8 columns a k-step
+          ptx::mma_pair_f16_ts(s_tmem, tmem + kColQT + 8 * (8 * u + kk), bd, kIdesc, 1u);
+        else
+          ptx::mma_pair_f16(s_tmem, ptx::make_desc(qa + (kk >> 2) * 512 + (kk & 3) * 2, kHi), bd, kIdesc, 1u);
+      }
+      ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->kempty[4 * B + u]), 0x3);
+      if (u == 3) ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->s_full[B]), 0x3);
+    }
+    __syncwarp();
+  }
+  return true;
+}
+
+template <typename T, uint32_t B>
+__device__ __forceinline__ bool kv4_pv_tile(const Ctx& c, uint32_t sbase, uint32_t tmem, Barriers* bars,
+                                            const TileMapReader<true>& map, uint32_t gi, uint32_t* piece) {
+  using S = Smem<T>;
+  constexpr uint32_t kIdesc = ptx::idesc_f16(0, 128, 256, 1);
+  constexpr uint32_t kHi = ptx::sw128_desc_hi(1024);
+  const uint32_t ph = (gi >> 1) & 1u;
+  TileRows w;
+  if (!map.get(c, gi, &w)) return false;
+  const bool first = (w.valid & kFirst) != 0;
+  if (!wait_warp(c, ptx::smem_u32(&bars->p_full[B]), ph, kErrPV)) return false;
+  if (first) {   // a new piece restarts O: the previous piece's epilogue must have read it
+    if (*piece > 0 && !wait_warp(c, ptx::smem_u32(&bars->o_free), (*piece - 1) & 1u, kErrPV)) return false;
+    ++*piece;
+  }
+#pragma unroll
+  for (uint32_t u = 0; u < 4; ++u) {
+    const uint32_t nh = u >> 1, th = u & 1u;
+    // one CTA's slot as QK^T had it (p_full is behind its fill), the other's refilled
+    if (!wait_warp(c, ptx::smem_u32(&bars->vfull[4 * B + u]), ph, kErrPV)) return false;
+    ptx::tc_fence_after();
+    if (elect_one()) {
+      const uint32_t vb = ptx::sw128_desc_lo(sbase + S::kKRing + (4 * B + u) * kStageBytes, kChunkBytes);
+      const uint32_t pa = ptx::sw128_desc_lo(sbase + S::kP + B * S::kPBuf + th * kChunkBytes, 16);
+#pragma unroll
+      for (int kk = 0; kk < 4; ++kk)
+        ptx::mma_pair_f16(tmem + kColO + 128 * nh, ptx::make_desc(pa + kk * 2, kHi),
+                          ptx::make_desc(vb + kk * 128, kHi), kIdesc, (first && th == 0 && kk == 0) ? 0u : 1u);
+      ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->vempty[4 * B + u]), 0x3);
+      if (u == 3) ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->o_done[B]), 0x3);
+    }
+    __syncwarp();
+  }
+  return true;
+}
+
+template <typename T, bool kQK>
+__device__ __forceinline__ void kv4_issuer(const Params& p, const Ctx& c, int pair, uint8_t* smem, uint32_t sbase,
+                                           uint32_t tmem, Barriers* bars) {
+  const TileMapReader<true> map(reinterpret_cast<const TileRows*>(smem + Smem<T>::kMap), bars);
+  const PieceIter it(p, pair);
+  const uint32_t n = it.t1 - it.t;
+  uint32_t piece = 0;
+#pragma unroll 1
+  for (uint32_t gi = 0; gi < n; gi += 2) {
+    if constexpr (kQK) {
+      if (!kv4_qk_tile<T, 0>(c, sbase, tmem, bars, map, gi, &piece)) return;
+      if (gi + 1 < n && !kv4_qk_tile<T, 1>(c, sbase, tmem, bars, map, gi + 1, &piece)) return;
+    } else {
+      if (!kv4_pv_tile<T, 0>(c, sbase, tmem, bars, map, gi, &piece)) return;
+      if (gi + 1 < n && !kv4_pv_tile<T, 1>(c, sbase, tmem, bars, map, gi + 1, &piece)) return;
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1132,8 +1302,6 @@ __device__ __forceinline__ void qk_issuer(const Params& p, const Ctx& c, int pai
   constexpr uint32_t kIdescRope = ptx::idesc_f16(Cfg<T>::kRopeFmt, 128, 128, 0);
   const uint32_t kfull0 = ptx::smem_u32(&bars->kfull[0]);
   const uint32_t kempty0 = ptx::smem_u32(&bars->kempty[0]);
-  const uint32_t rfull0 = ptx::smem_u32(&bars->v8full[0]);
-  const uint32_t rempty0 = ptx::smem_u32(&bars->v8empty[0]);
   const uint32_t q_full = ptx::smem_u32(&bars->q_full);
   const uint32_t q_empty = ptx::smem_u32(&bars->q_empty);
   const uint32_t qt_full = ptx::smem_u32(&bars->qt_full);
@@ -1148,7 +1316,7 @@ __device__ __forceinline__ void qk_issuer(const Params& p, const Ctx& c, int pai
   int piece = 0;
   while (it.next(&pc)) {
     // (FP8: qt_full covers the whole quantized Q, written by the softmax warps)
-    if (!Io<T>::kKv8 && !Io<T>::kKv4 && !wait_bar(c, q_full, (uint32_t)piece & 1u, kErrQK)) return;
+    if (!Io<T>::kKv8 && !wait_bar(c, q_full, (uint32_t)piece & 1u, kErrQK)) return;
     if (!wait_bar(c, qt_full, (uint32_t)piece & 1u, kErrQK)) return;
     ptx::tc_fence_after();
 #pragma unroll 1
@@ -1160,14 +1328,10 @@ __device__ __forceinline__ void qk_issuer(const Params& p, const Ctx& c, int pai
       const uint32_t s_tmem = tmem + 64 * b;
 #pragma unroll
       for (int u = 0; u < 5; ++u) {
-        // (4-bit: the rope unit has its own ring of two)
-        const bool own_rope = Io<T>::kKv4 && u == 4;
-        const uint32_t full = own_rope ? rfull0 + 8 * b : kfull0 + 8 * ring.stage;
-        if (!wait_bar(c, full, own_rope ? (gi >> 1) & 1u : ring.phase, kErrQK)) return;
+        if (!wait_bar(c, kfull0 + 8 * ring.stage, ring.phase, kErrQK)) return;
         ptx::tc_fence_after();
         // descriptor low words; +512 = next 8 KB box, +2 = next 32-byte k-step
-        const uint32_t kb = ptx::sw128_desc_lo(
-            sbase + (own_rope ? S::kV8Ring + b * kChunkBytes : S::kKRing + ring.stage * Cfg<T>::kKStageBytes), 16);
+        const uint32_t kb = ptx::sw128_desc_lo(sbase + S::kKRing + ring.stage * Cfg<T>::kKStageBytes, 16);
         if (Io<T>::kKv8 && u < 4) {
           // FP8: latent dims [128 u, +128) in e4m3, 32 per k-step: Q hi from TMEM (4
           // elements per column), Q lo from box u of the Q region
@@ -1201,12 +1365,8 @@ __device__ __forceinline__ void qk_issuer(const Params& p, const Ctx& c, int pai
                                 kIdescRope, 1u);
           }
         }
-        if (own_rope) {
-          ptx::mma_commit_pair_mc(rempty0 + 8 * b, 0x3);
-        } else {
-          ptx::mma_commit_pair_mc(kempty0 + 8 * ring.stage, 0x3);
-          ring.advance();
-        }
+        ptx::mma_commit_pair_mc(kempty0 + 8 * ring.stage, 0x3);
+        ring.advance();
       }
       ptx::mma_commit_pair_mc(s_full0 + 8 * b, 0x3);
       if (j == pc.end - 1) ptx::mma_commit_pair_mc(q_empty, 0x3);
@@ -1231,10 +1391,7 @@ __device__ __forceinline__ void pv_issuer(const Params& p, const Ctx& c, int pai
   const uint32_t o_free = ptx::smem_u32(&bars->o_free);
   const uint32_t plo = ptx::sw128_desc_lo(sbase + S::kP, 16);
   constexpr uint32_t kHi = ptx::sw128_desc_hi(1024);
-  const uint32_t kfull0 = ptx::smem_u32(&bars->kfull[0]);
-  // (4-bit: the K ring's eight slots, in the same order)
-  constexpr uint32_t kRing = Io<T>::kKv4 ? S::kKRing : S::kVRing;
-  Ring<Io<T>::kKv4 ? 8 : VS> ring;
+  Ring<VS> ring;
   uint32_t gi = 0;
   PieceIter it(p, pair);
   Piece pc;
@@ -1251,12 +1408,10 @@ __device__ __forceinline__ void pv_issuer(const Params& p, const Ctx& c, int pai
 #pragma unroll 1
       for (int u = 0; u < 4; ++u) {
         const int nh = u >> 1, th = u & 1;
-        // 4-bit: one CTA's slot as QK^T had it, the other's refilled
-        if (Io<T>::kKv4 && !wait_bar(c, kfull0 + 8 * ring.stage, ring.phase, kErrPV)) return;
         if (!wait_bar(c, vfull0 + 8 * ring.stage, ring.phase, kErrPV)) return;
         ptx::tc_fence_after();
         // descriptor low words: V is MN-major (+128 = next 16 rows), P K-major (+2 = next k-step)
-        const uint32_t vb = ptx::sw128_desc_lo(sbase + kRing + ring.stage * kStageBytes, kChunkBytes);
+        const uint32_t vb = ptx::sw128_desc_lo(sbase + S::kVRing + ring.stage * kStageBytes, kChunkBytes);
 #pragma unroll
         for (int part = 0; part < Cfg<T>::kPParts; ++part) {
           const uint32_t pa = plo + b * (S::kPBuf >> 4) + part * (kPBytes >> 4) + th * 512;
@@ -2120,8 +2275,8 @@ __device__ __forceinline__ void softmax_epilogue(const Params& p, const Ctx& c, 
 // producer, warp 3 P.V issuer, warps 4..7 softmax/epilogue, warp 8 Q loader
 // (warps 9..11 complete the third warpgroup).  For an FP8 cache the block has
 // 16 warps: warp 2 also prefetches Q, and warps 8..15 convert V to fp16.  For a
-// 4-bit cache likewise, with warp 0 loading the rope rows only, no V producer and the
-// converters filling the slots of both GEMMs.  The
+// 4-bit cache warp 0 loads the rope rows, warp 2 finds the tiles' rows and warps 8..15
+// fill the slots of both GEMMs.  The
 // Cv variant has 16 warps too: warps 12..15 rewrite each landed V stage (tail
 // rows zeroed, bf16 -> fp16 with kF16); warps 9..11 are idle.  In the plain
 // variants warp 9 zeroes the tail rows of a sequence's last V units.
@@ -2144,11 +2299,11 @@ mla_sm100_decode_kernel(const __grid_constant__ Params p) {
   if (threadIdx.x == 0) {
     // V operand stages: one expect-tx arrival (TMA), or FP8: kConvWarps converter warps x 2 CTAs
     // (4-bit: a slot filled for QK^T by both CTAs' converters, refilled for P.V by one's)
-    const uint32_t n_vfull = Io<T>::kKv4   ? (uint32_t)kConvWarps
+    const uint32_t n_vfull = Io<T>::kKv4   ? kRefillWarps
                              : Io<T>::kKv8 ? 2u * kConvWarps
                                            : (Io<T>::kConv ? 2u * kFixWarps : 1u);
     for (int s = 0; s < 8; ++s) {
-      ptx::mbar_init(ptx::smem_u32(&bars->kfull[s]), Io<T>::kKv4 ? 2u * kConvWarps : 1u);
+      ptx::mbar_init(ptx::smem_u32(&bars->kfull[s]), Io<T>::kKv4 ? 2u * kFillWarps : 1u);
       ptx::mbar_init(ptx::smem_u32(&bars->kempty[s]), 1);
       ptx::mbar_init(ptx::smem_u32(&bars->vfull[s]), n_vfull);
       ptx::mbar_init(ptx::smem_u32(&bars->vempty[s]), 1);
@@ -2181,6 +2336,10 @@ mla_sm100_decode_kernel(const __grid_constant__ Params p) {
     ptx::mbar_init(ptx::smem_u32(&bars->mdone), 4);
     ptx::mbar_init(ptx::smem_u32(&bars->drain_qk), 1);
     ptx::mbar_init(ptx::smem_u32(&bars->drain_pv), 1);
+    for (int b = 0; b < 2; ++b) {
+      ptx::mbar_init(ptx::smem_u32(&bars->mapfull[b]), 1);
+      ptx::mbar_init(ptx::smem_u32(&bars->mapempty[b]), kMapReaders + (rank == 0 ? 2 : 0));
+    }
     *abort_flag = 0u;
     ptx::fence_mbarrier_init();
   }
@@ -2221,31 +2380,47 @@ mla_sm100_decode_kernel(const __grid_constant__ Params p) {
   } else {
     ptx::setmaxnreg_dec<kRegsLow>();
   if (warp == 0) {
-    if (lane == 0) k_producer<T>(p, c, rank, pair, sbase, bars);
+    if (lane == 0) k_producer<T>(p, c, rank, pair, smem, sbase, bars);
   } else if (warp == 8 && !Io<T>::kKv8 && !Io<T>::kKv4) {
     if (lane == 0) q_loader<T>(p, c, rank, pair, sbase, bars);
+  } else if (Io<T>::kKv4 && (warp == 1 || warp == 3)) {
+    if constexpr (Io<T>::kKv4) {
+      if (rank == 0) {
+        if (warp == 1)
+          kv4_issuer<T, true>(p, c, pair, smem, sbase, tmem, bars);
+        else
+          kv4_issuer<T, false>(p, c, pair, smem, sbase, tmem, bars);
+        // every tcgen05 op the elected lane issued has completed once this commit lands
+        const uint32_t drain = ptx::smem_u32(warp == 1 ? &bars->drain_qk : &bars->drain_pv);
+        __syncwarp();
+        if (elect_one()) ptx::mma_commit_pair_mc(drain, 0x1);
+        __syncwarp();
+        wait_bar(c, drain, 0u, kErrDrain);
+      }
+    }
   } else if (warp == 1) {
     if (rank == 0 && lane == 0) {
-      qk_issuer<T>(p, c, pair, sbase, tmem, bars);
+      if constexpr (!Io<T>::kKv4) qk_issuer<T>(p, c, pair, sbase, tmem, bars);
       // every tcgen05 op this thread issued has completed once this commit lands
       ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->drain_qk), 0x1);
       wait_bar(c, ptx::smem_u32(&bars->drain_qk), 0u, kErrDrain);
     }
   } else if (warp == 2) {
     // (FP8: the Q loader only prefetches and never waits; it runs here first)
-    if ((Io<T>::kKv8 || Io<T>::kKv4) && lane == 0) q_loader<T>(p, c, rank, pair, sbase, bars);
-    if constexpr (!Io<T>::kKv4) {
-      if (lane == 0) v_producer<T>(p, c, rank, pair, sbase, bars);
-    }
+    if (Io<T>::kKv8 && lane == 0) q_loader<T>(p, c, rank, pair, sbase, bars);
+    if constexpr (Io<T>::kKv4)
+      tile_scout<T>(p, c, rank, pair, smem, bars, lane);
+    else if (lane == 0)
+      v_producer<T>(p, c, rank, pair, sbase, bars);
   } else if (warp == 3) {
     if (rank == 0 && lane == 0) {
-      pv_issuer<T>(p, c, pair, sbase, tmem, bars);
+      if constexpr (!Io<T>::kKv4) pv_issuer<T>(p, c, pair, sbase, tmem, bars);
       ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->drain_pv), 0x1);
       wait_bar(c, ptx::smem_u32(&bars->drain_pv), 0u, kErrDrain);
     }
   } else if (Io<T>::kKv4 && warp >= 8) {
     // 4-bit: warps 8..15 widen the codes
-    if constexpr (Io<T>::kKv4) kv4_converter<T>(p, c, rank, pair, smem, bars, (warp - 8) * 32 + lane, lane);
+    if constexpr (Io<T>::kKv4) kv4_converter<T>(p, c, rank, pair, smem, bars, warp - 8, lane);
   } else if (Io<T>::kKv8 && warp >= 8) {
     // FP8: warps 8..15 dequantize the V units
     if constexpr (Io<T>::kKv8) v_converter<T>(p, c, pair, smem, bars, (warp - 8) * 32 + lane, lane);
@@ -3080,6 +3255,7 @@ cudaError_t launch_sm100_decode(const DecodeArgs& a, int variant) {
   p.page_size = a.page_size;
   p.max_pages = a.max_pages;
   p.num_pages = a.num_pages;
+  p.num_rows = a.block_table != nullptr ? a.num_pages * a.page_size : a.batch * a.seqlen_kv;
   p.kv_scales = static_cast<const __half*>(a.kv_scales);
   p.kv_scale = a.kv_fp8 ? a.kv_scale : 1.f;
   const cudaError_t lerr = launch_form(a, p);

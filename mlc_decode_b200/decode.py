@@ -402,11 +402,13 @@ class MlaPagedDecodeKernel:
         return _clock_probe(self._ws, device, dtype)
 
     def device_status(self, device, dtype) -> int:
-        """Status word the kernel leaves in the workspace (0 = no timeout)."""
-        ws = self._ws.get((torch.device(device).index, dtype))
-        if ws is None or ws.numel() < 4:
-            return 0
-        return int(ws[:4].view(torch.int32).item())
+        """Status word the kernels leave in the workspaces (0 = no timeout)."""
+        index = torch.device(device).index
+        for key in ((index, dtype), (index, dtype, "int4")):
+            ws = self._ws.get(key)
+            if ws is not None and ws.numel() >= 4 and int(ws[:4].view(torch.int32).item()) != 0:
+                return int(ws[:4].view(torch.int32).item())
+        return 0
 
     def __call__(self, q, q_pe, kv_cache, k_pe_cache, cache_seqlens, out, lse=None, block_table=None,
                  kv_scale=None):
