@@ -139,12 +139,12 @@ struct Walk {
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
   if constexpr (std::is_same<T, __half>::value)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -182,7 +182,8 @@ __global__ void __launch_bounds__(kThreads, Lay<MT>::kCtasPerSm)
 mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
   using L = Lay<MT>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  // (aligned by an offset: a pointer rounded as an integer would make every access generic)
+  uint8_t* smem = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t sbase = ptx::smem_u32(smem);
   const Int4Args& a = p.a;
   volatile uint32_t* abort = reinterpret_cast<volatile uint32_t*>(smem + L::kMisc);
@@ -567,14 +568,15 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
   }
 }
 
-// Merge of the units that a range's end cut: one 128-thread CTA per query row at a time
-// (four dims a thread), eight partial rows in flight.  The LSE algebra of mla_combine.cu.
-template <typename T>
-__global__ void __launch_bounds__(128) mla_int4_mma_combine_kernel(Int4Args a, const int2* __restrict__ info, int g,
-                                                                   int groups, int rows, long long items) {
+// Merge of the units that a range's end cut: one CTA per query row at a time, G groups of
+// 128 threads (four dims a thread) taking every G-th piece, eight pieces in flight each;
+// their sums meet in shared memory.  The LSE algebra of mla_combine.cu.
+template <typename T, int kMergeGroups>
+__global__ void __launch_bounds__(128 * kMergeGroups)
+mla_int4_mma_combine_kernel(Int4Args a, const int2* __restrict__ info, int g, int groups, int rows, long long items) {
   __shared__ float s_w[kMaxWorkers];
-  __shared__ float s_red[4];
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  __shared__ float4 s_acc[kMergeGroups][128];
+  const int grp = threadIdx.x >> 7, tid = threadIdx.x & 127, lane = tid & 31;
   const int units_per_seq = a.kv_heads * groups, rows_all = a.q_len * g;
   ptx::grid_dep_wait();
   for (long long i = blockIdx.x; i < items; i += gridDim.x) {
@@ -583,51 +585,66 @@ __global__ void __launch_bounds__(128) mla_int4_mma_combine_kernel(Int4Args a, c
     const int2 w = __ldcg(info + unit);
     const int s = (int)(unit / units_per_seq), sub = (int)(unit - (long long)s * units_per_seq);
     const int r = (sub % groups) * rows + row;
-    if (w.x < 0 || r >= rows_all) continue;   // (the same for every thread)
+    if (w.x < 0 || r >= rows_all) continue;      // (the same for every thread)
     const int w0 = w.x >> 1, n = w.y - w0 + 1;   // (at most kMaxWorkers)
     // after the unit's first piece each worker's first
     auto slot = [&](int k) -> long long { return k == 0 ? (long long)w.x : 2ll * (w0 + k); };
+    auto piece = [&](int k) -> float4 {
+      return k < n ? __ldcg(reinterpret_cast<const float4*>(a.part_o + (slot(k) * rows + row) * kDim) + tid)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+    };
+    float4 v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = piece(grp + kMergeGroups * u);
+    for (int k = threadIdx.x; k < n; k += 128 * kMergeGroups) s_w[k] = __ldcg(a.part_lse + slot(k) * rows + row);
+    __syncthreads();
+    // every warp reduces the pieces' LSEs itself
     float mx = -INFINITY;
-    for (int k = tid; k < n; k += 128) {
-      const float x = __ldcg(a.part_lse + slot(k) * rows + row);
-      s_w[k] = x;
-      mx = fmaxf(mx, x);
-    }
+    for (int k = lane; k < n; k += 32) mx = fmaxf(mx, s_w[k]);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    if (lane == 0) s_red[warp] = mx;
-    __syncthreads();
-    mx = fmaxf(fmaxf(s_red[0], s_red[1]), fmaxf(s_red[2], s_red[3]));
-    const bool any = mx > -INFINITY;
+    const bool any = mx > -INFINITY || mx != mx;
     float sum = 0.f;
     if (any)
-      for (int k = lane; k < n; k += 32) sum += exp2f((s_w[k] - mx) * kLog2e);   // (every warp the whole sum)
+      for (int k = lane; k < n; k += 32) sum += exp2f((s_w[k] - mx) * kLog2e);
 #pragma unroll
     for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
     const float lse = any ? mx + logf(sum) : -INFINITY;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int k0 = 0; any && k0 < n; k0 += 8) {
-      float4 v[8];
-#pragma unroll
-      for (int u = 0; u < 8; ++u)
-        v[u] = k0 + u < n ? __ldcg(reinterpret_cast<const float4*>(a.part_o + (slot(k0 + u) * rows + row) * kDim) + tid)
-                          : make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int k0 = grp; any && k0 < n; k0 += 8 * kMergeGroups) {
 #pragma unroll
       for (int u = 0; u < 8; ++u) {
-        if (k0 + u >= n) break;
-        const float e = exp2f((s_w[k0 + u] - lse) * kLog2e);
+        const int k = k0 + kMergeGroups * u;
+        if (k >= n) break;
+        const float e = exp2f((s_w[k] - lse) * kLog2e);
         acc.x = fmaf(e, v[u].x, acc.x);
         acc.y = fmaf(e, v[u].y, acc.y);
         acc.z = fmaf(e, v[u].z, acc.z);
         acc.w = fmaf(e, v[u].w, acc.w);
       }
+      if (k0 + 8 * kMergeGroups < n) {
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = piece(k0 + kMergeGroups * (8 + u));
+      }
     }
-    const int pos_t = r / g;
-    const long long qi = ((long long)s * a.q_len + pos_t) * a.heads + (sub / groups) * g + (r - pos_t * g);
-    *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + qi * kDim + 4 * tid) =
-        make_uint2(Elt<T>::pack2(acc.x, acc.y), Elt<T>::pack2(acc.z, acc.w));
-    if (a.lse != nullptr && tid == 0) a.lse[qi] = lse;
-    __syncthreads();   // s_w and s_red are free for the next row
+    if (grp > 0) s_acc[grp][tid] = acc;
+    __syncthreads();
+    if (grp == 0) {
+#pragma unroll
+      for (int o = 1; o < kMergeGroups; ++o) {
+        const float4 x = s_acc[o][tid];
+        acc.x += x.x;
+        acc.y += x.y;
+        acc.z += x.z;
+        acc.w += x.w;
+      }
+      const int pos_t = r / g;
+      const long long qi = ((long long)s * a.q_len + pos_t) * a.heads + (sub / groups) * g + (r - pos_t * g);
+      *reinterpret_cast<uint2*>(static_cast<T*>(a.out) + qi * kDim + 4 * tid) =
+          make_uint2(Elt<T>::pack2(acc.x, acc.y), Elt<T>::pack2(acc.z, acc.w));
+      if (a.lse != nullptr && tid == 0) a.lse[qi] = lse;
+    }
+    __syncthreads();   // the shared arrays are free for the next row
   }
 }
 
@@ -728,16 +745,21 @@ cudaError_t launch_typed(const MmaParams& p, int workers, cudaStream_t stream) {
   if (err != cudaSuccess) return err;
   const long long items = (long long)p.a.batch * p.a.kv_heads * p.groups * L::kRows;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(items < 148 * 16 ? items : 148 * 16), 1, 1);
-  cfg.blockDim = dim3(128, 1, 1);
+  // few rows are cut into many pieces each, many rows into few (b128 h16 s4096, three
+  // pieces a row: 16 us more with four groups; b1 h16 s131072, 296 pieces: 18 us less)
+  const bool few = items < 148 * 4;
+  const long long ctas = few ? items : (items < 148 * 16 ? items : 148 * 16);
+  cfg.gridDim = dim3((unsigned)ctas, 1, 1);
+  cfg.blockDim = dim3(few ? 512 : 128, 1, 1);
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, mla_int4_mma_combine_kernel<T>, p.a, (const int2*)p.info, p.g, p.groups, L::kRows,
-                            items);
+  const int2* info = p.info;
+  return few ? cudaLaunchKernelEx(&cfg, mla_int4_mma_combine_kernel<T, 4>, p.a, info, p.g, p.groups, L::kRows, items)
+             : cudaLaunchKernelEx(&cfg, mla_int4_mma_combine_kernel<T, 1>, p.a, info, p.g, p.groups, L::kRows, items);
 }
 
 }  // namespace
