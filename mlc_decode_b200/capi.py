@@ -6,6 +6,7 @@ if it is missing or fails to load, every entry point raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -70,6 +71,8 @@ def lib_path() -> str:
 def load(build_if_missing: bool = True):
     """Load (building first if allowed and needed) and return the CDLL."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -410,54 +413,52 @@ def int4kv_workspace_bytes(batch, q_len, heads, kv_heads, max_seqlen_kv, dtype, 
     return int(n)
 
 
+# The wrappers below pass their arguments on as they are (Python ints and addresses): they
+# are called once or more per decode step, where every conversion shows.
 def decode_ext_int4kv(q, q_pe, kv_codes, kv_scales, k_pe_cache, block_table, cache_seqlens, out, lse, ws, ws_bytes,
                       batch, q_len, heads, kv_heads, max_seqlen_kv, page_size, num_pages, max_pages, dtype,
                       cfg: MlaCfg, stream) -> None:
     """mla_decode_ext_int4kv: mla_decode_ext over a latent cache held in 4 bits."""
-    check(load().mla_decode_ext_int4kv(q, q_pe, kv_codes, kv_scales, k_pe_cache, block_table, cache_seqlens, out, lse,
-                                       ws, ws_bytes, int(batch), int(q_len), int(heads), int(kv_heads),
-                                       int(max_seqlen_kv), int(page_size), int(num_pages), int(max_pages),
-                                       int(dtype), ctypes.byref(cfg), stream))
+    rc = load().mla_decode_ext_int4kv(q, q_pe, kv_codes, kv_scales, k_pe_cache, block_table, cache_seqlens, out, lse,
+                                      ws, ws_bytes, batch, q_len, heads, kv_heads, max_seqlen_kv, page_size,
+                                      num_pages, max_pages, dtype, ctypes.byref(cfg), stream)
+    if rc:
+        check(rc)
 
 
+@functools.lru_cache(maxsize=256)
 def block_tables_workspace_bytes(batch, num_tokens) -> int:
-    n = load().mla_block_tables_workspace_bytes(int(batch), int(num_tokens))
+    n = load().mla_block_tables_workspace_bytes(batch, num_tokens)
     if n == 0:
         msg = last_error()
         if msg:
             raise MlaError(1, msg)
-    return int(n)
+    return n
 
 
-def extend_block_tables(block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens, new_free_pos, slots,
-                        positions, cu_new, ws, ws_bytes, batch, max_pages, page_size, num_pages, num_free, num_tokens,
-                        q_len, stream) -> None:
-    """mla_extend_block_tables (pointers are device addresses)."""
-    check(load().mla_extend_block_tables(block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens,
-                                         new_free_pos, slots, positions, cu_new, ws, ws_bytes, int(batch),
-                                         int(max_pages), int(page_size), int(num_pages), int(num_free),
-                                         int(num_tokens), int(q_len), stream))
+def extend_block_tables(*args) -> None:
+    """mla_extend_block_tables, its arguments in order (pointers are device addresses)."""
+    rc = load().mla_extend_block_tables(*args)
+    if rc:
+        check(rc)
 
 
-def rotary(x, out, positions, turns, gain, tokens, heads, head_dim, rot_dim, offset, interleaved, x_strides,
-           out_strides, dtype, stream) -> None:
-    """mla_rotary; strides are (token, head) in elements."""
-    check(load().mla_rotary(x, out, positions, turns, float(gain), int(tokens), int(heads), int(head_dim),
-                            int(rot_dim), int(offset), int(bool(interleaved)), *map(int, x_strides),
-                            *map(int, out_strides), int(dtype), stream))
+def rotary(*args) -> None:
+    """mla_rotary, its arguments in order."""
+    rc = load().mla_rotary(*args)
+    if rc:
+        check(rc)
 
 
-def cache_append(kv, k_pe, slots, kv_cache, kv_scales, k_pe_cache, kv_scale, positions, turns, gain, interleaved,
-                 tokens, kv_heads, cache_rows, kv_strides, pe_strides, form, dtype, stream) -> None:
-    """mla_cache_append; strides are (token, head) in elements."""
-    check(load().mla_cache_append(kv, k_pe, slots, kv_cache, kv_scales, k_pe_cache, float(kv_scale), positions, turns,
-                                  float(gain), int(bool(interleaved)), int(tokens), int(kv_heads), int(cache_rows),
-                                  *map(int, kv_strides), *map(int, pe_strides), int(form), int(dtype), stream))
+def cache_append(*args) -> None:
+    """mla_cache_append, its arguments in order."""
+    rc = load().mla_cache_append(*args)
+    if rc:
+        check(rc)
 
 
-def cache_gather(slots, kv_cache, kv_scales, k_pe_cache, kv_scale, kv, k_pe, tokens, kv_heads, cache_rows, kv_strides,
-                 pe_strides, form, dtype, stream) -> None:
-    """mla_cache_gather; strides are (token, head) in elements."""
-    check(load().mla_cache_gather(slots, kv_cache, kv_scales, k_pe_cache, float(kv_scale), kv, k_pe, int(tokens),
-                                  int(kv_heads), int(cache_rows), *map(int, kv_strides), *map(int, pe_strides),
-                                  int(form), int(dtype), stream))
+def cache_gather(*args) -> None:
+    """mla_cache_gather, its arguments in order."""
+    rc = load().mla_cache_gather(*args)
+    if rc:
+        check(rc)

@@ -7,7 +7,8 @@
 // lane l holds dims [8 l, 8 l + 8) and [256 + 8 l, 256 + 8 l + 8) in two 16-byte loads,
 // so the four lanes of a 32-dim group find its largest value in two shuffles, each
 // lane's eight codes are one 32-bit word and a warp stores whole 128-byte lines; lane l
-// also turns rope pair l.
+// also turns rope pair l.  In calls long enough to fill the GPU a warp has the loads of
+// kLong rows in flight before it stores the first.
 #include <cuda_fp8.h>
 
 #include "mla_cache.cuh"
@@ -15,7 +16,9 @@
 namespace mla {
 namespace {
 
-constexpr int kWarps = 8;   // rows per CTA
+constexpr int kWarps = 8;
+constexpr int kLong = 2;            // rows in flight per warp of a long call
+constexpr long long kLongRows = 148ll * 64 * kLong;   // a long call: every warp slot of the GPU gets that many
 
 struct CacheArgs {
   const void* kv;          // append: rows in; gather: unused
@@ -52,120 +55,180 @@ __device__ __forceinline__ uint4 pack8(const float (&f)[8]) {
                     Elt<T>::pack2(f[6], f[7]));
 }
 
+// rint(f / s) clamped to a code's range, + 8; NaN is 0's code.
+__device__ __forceinline__ uint32_t code_of(float f, float s) {
+  const float r = rintf(__fdiv_rn(f, s));
+  return f == f ? (uint32_t)((int)fminf(fmaxf(r, -8.f), 7.f) + 8) : 8u;
+}
+
 // This lane's eight dims as codes (low nibble first: dims 0 2 4 6 1 3 5 7) and its
 // group's scale.  s = half(max / 7) may round below max / 7, hence the clamp; a group of
 // zeros (or one whose scale rounds to zero) has code 8, the value 0; NaN stores as 0 and
 // infinities as the largest code.
+// f / s is f times the reciprocal, off by two units of its last place (below 1.3e-6 up
+// to 8): it rounds to the same integer unless it lies within 1e-5 of a half, where (and
+// for values that are not finite) the lane divides.  One reciprocal, no conversion
+// instruction: the sum with 1.5 x 2^23 leaves the rounded integer in its last bits.
 __device__ __forceinline__ uint32_t quantise8(const float (&f)[8], __half* scale) {
-  float m = 0.f;
+  float m = 0.f, sum = 0.f;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(f[k]));
+  for (int k = 0; k < 8; ++k) {
+    m = fmaxf(m, fabsf(f[k]));
+    sum += fabsf(f[k]);
+  }
+  const bool finite = sum < INFINITY;
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
   m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
   const __half s = __float2half_rn(fminf(__fdiv_rn(m, 7.f), 65504.f));
   const float sf = __half2float(s);
   *scale = s;
-  uint32_t w = 0x88888888u;
-  if (sf > 0.f) {
+  if (!(sf > 0.f)) return 0x88888888u;
+  const float inv = __fdiv_rn(1.f, sf);
+  const float magic = 12582912.f;   // 1.5 x 2^23: a sum's last bit counts ones
+  uint32_t w = 0;
+  bool sure = finite;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) {
+    const float q = fminf(fmaxf(f[k] * inv, -8.f), 7.f);
+    const float t = q + magic;
+    sure = sure && fabsf(fabsf(q - (t - magic)) - 0.5f) > 1e-5f;
+    w |= ((__float_as_uint(t) + 8u) & 15u) << (4 * ((k >> 1) + 4 * (k & 1)));
+  }
+  if (!sure) {
     w = 0;
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      // clamped before the conversion: infinities become the largest codes; NaN fails
-      // the comparison and becomes 0
-      const float r = rintf(__fdiv_rn(f[k], sf));
-      const int n = f[k] == f[k] ? (int)fminf(fmaxf(r, -8.f), 7.f) + 8 : 8;
-      w |= (uint32_t)n << (4 * ((k >> 1) + 4 * (k & 1)));
-    }
+    for (int k = 0; k < 8; ++k) w |= code_of(f[k], sf) << (4 * ((k >> 1) + 4 * (k & 1)));
   }
   return w;
 }
 
 enum Form { kModel = MLA_CACHE_MODEL, kFp8 = MLA_CACHE_FP8, kInt4 = MLA_CACHE_INT4 };
 
-template <typename T, int F>
+template <typename T, int F, int R>
 __global__ void __launch_bounds__(32 * kWarps) mla_cache_append_kernel(CacheArgs a) {
   const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (item >= a.tokens * a.kv_heads) return;
-  const long long t = item / a.kv_heads;
-  const int kvh = (int)(item - t * a.kv_heads);
-  const int slot = __ldg(a.slots + t);
-  if (slot < 0 || slot >= a.rows) return;
-  const long long row = (long long)slot * a.kv_heads + kvh;
-  const uint4* kv = reinterpret_cast<const uint4*>(static_cast<const T*>(a.kv) + t * a.kv_token + kvh * a.kv_head);
-  const uint4 x0 = __ldg(kv + lane), x1 = __ldg(kv + 32 + lane);
-  const T* pe = static_cast<const T*>(a.k_pe) + t * a.pe_token + kvh * a.pe_head;
+  const long long items = a.tokens * a.kv_heads;
+  const long long first = ((long long)blockIdx.x * kWarps + (threadIdx.x >> 5)) * R;
   const int d0 = a.interleaved ? 2 * lane : lane, d1 = a.interleaved ? 2 * lane + 1 : lane + 32;
-  const T p0 = pe[d0], p1 = pe[d1];
-  if constexpr (F == kModel) {
-    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.kv_cache) + row * kDim);
-    dst[lane] = x0;
-    dst[32 + lane] = x1;
-  } else {
-    float f0[8], f1[8];
-    unpack8<T>(x0, f0);
-    unpack8<T>(x1, f1);
-    if constexpr (F == kFp8) {
-      uint32_t w[4];
+  uint4 x0[R], x1[R];
+  T p0[R], p1[R];
+  int slot[R], kvh[R], pos[R];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float* f = k < 2 ? f0 + 4 * k : f1 + 4 * (k - 2);
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(f[0], a.kv_scale), __fdiv_rn(f[1], a.kv_scale)),
-                                                     __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(__fdiv_rn(f[2], a.kv_scale), __fdiv_rn(f[3], a.kv_scale)),
-                                                     __NV_SATFINITE, __NV_E4M3);
-        w[k] = lo | (hi << 16);
-      }
-      uint2* dst = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.kv_cache) + row * kDim);
-      dst[lane] = make_uint2(w[0], w[1]);
-      dst[32 + lane] = make_uint2(w[2], w[3]);
+  for (int i = 0; i < R; ++i) {
+    slot[i] = -1;
+    if (first + i >= items) continue;
+    const long long t = a.kv_heads == 1 ? first + i : (first + i) / a.kv_heads;
+    kvh[i] = (int)(first + i - t * a.kv_heads);
+    slot[i] = __ldg(a.slots + t);
+    const uint4* kv =
+        reinterpret_cast<const uint4*>(static_cast<const T*>(a.kv) + t * a.kv_token + kvh[i] * a.kv_head);
+    x0[i] = __ldg(kv + lane);
+    x1[i] = __ldg(kv + 32 + lane);
+    const T* pe = static_cast<const T*>(a.k_pe) + t * a.pe_token + kvh[i] * a.pe_head;
+    p0[i] = pe[d0];
+    p1[i] = pe[d1];
+    pos[i] = a.positions != nullptr ? __ldg(a.positions + t) : 0;
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (slot[i] < 0 || slot[i] >= a.rows) continue;   // (the same for the whole warp)
+    const long long row = (long long)slot[i] * a.kv_heads + kvh[i];
+    if constexpr (F == kModel) {
+      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.kv_cache) + row * kDim);
+      dst[lane] = x0[i];
+      dst[32 + lane] = x1[i];
     } else {
-      __half s0, s1;
-      const uint32_t w0 = quantise8(f0, &s0), w1 = quantise8(f1, &s1);
-      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.kv_cache) + row * kI4Bytes);
-      dst[lane] = w0;
-      dst[32 + lane] = w1;
-      if ((lane & 3) == 0) {
-        __half* sc = static_cast<__half*>(a.scales) + row * kI4Groups;
-        sc[lane >> 2] = s0;
-        sc[8 + (lane >> 2)] = s1;
+      float f0[8], f1[8];
+      unpack8<T>(x0[i], f0);
+      unpack8<T>(x1[i], f1);
+      if constexpr (F == kFp8) {
+        uint32_t w[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float* f = k < 2 ? f0 + 4 * k : f1 + 4 * (k - 2);
+          const uint32_t lo = __nv_cvt_float2_to_fp8x2(
+              make_float2(__fdiv_rn(f[0], a.kv_scale), __fdiv_rn(f[1], a.kv_scale)), __NV_SATFINITE, __NV_E4M3);
+          const uint32_t hi = __nv_cvt_float2_to_fp8x2(
+              make_float2(__fdiv_rn(f[2], a.kv_scale), __fdiv_rn(f[3], a.kv_scale)), __NV_SATFINITE, __NV_E4M3);
+          w[k] = lo | (hi << 16);
+        }
+        uint2* dst = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.kv_cache) + row * kDim);
+        dst[lane] = make_uint2(w[0], w[1]);
+        dst[32 + lane] = make_uint2(w[2], w[3]);
+      } else {
+        __half s0, s1;
+        const uint32_t w0 = quantise8(f0, &s0), w1 = quantise8(f1, &s1);
+        uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.kv_cache) + row * kI4Bytes);
+        dst[lane] = w0;
+        dst[32 + lane] = w1;
+        if ((lane & 3) == 0) {
+          __half* sc = static_cast<__half*>(a.scales) + row * kI4Groups;
+          sc[lane >> 2] = s0;
+          sc[8 + (lane >> 2)] = s1;
+        }
       }
     }
-  }
-  T* pc = static_cast<T*>(a.k_pe_cache) + row * kPeDim;
-  if (a.positions != nullptr) {
-    const float2 c = rotary_cos_sin(__ldg(a.positions + t), __ldg(a.turns + lane), a.gain);
-    const float u = Elt<T>::to1(p0), v = Elt<T>::to1(p1);
-    pc[d0] = Elt<T>::from(u * c.x - v * c.y);
-    pc[d1] = Elt<T>::from(u * c.y + v * c.x);
-  } else {
-    pc[d0] = p0;
-    pc[d1] = p1;
+    T* pc = static_cast<T*>(a.k_pe_cache) + row * kPeDim;
+    if (a.positions != nullptr) {
+      const float2 c = rotary_cos_sin(pos[i], __ldg(a.turns + lane), a.gain);
+      const float u = Elt<T>::to1(p0[i]), v = Elt<T>::to1(p1[i]);
+      pc[d0] = Elt<T>::from(u * c.x - v * c.y);
+      pc[d1] = Elt<T>::from(u * c.y + v * c.x);
+    } else {
+      pc[d0] = p0[i];
+      pc[d1] = p1[i];
+    }
   }
 }
 
-template <typename T, int F>
+template <typename T, int F, int R>
 __global__ void __launch_bounds__(32 * kWarps) mla_cache_gather_kernel(CacheArgs a) {
   const int lane = threadIdx.x & 31;
-  const long long item = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (item >= a.tokens * a.kv_heads) return;
-  const long long t = item / a.kv_heads;
-  const int kvh = (int)(item - t * a.kv_heads);
-  const int slot = __ldg(a.slots + t);
-  const bool real = slot >= 0 && slot < a.rows;
-  const long long row = real ? (long long)slot * a.kv_heads + kvh : 0;
-  uint4 y0 = make_uint4(0u, 0u, 0u, 0u), y1 = y0;
-  uint32_t pe = 0;
-  if (real) {
-    pe = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.k_pe_cache) + row * kPeDim) + lane);
+  const long long items = a.tokens * a.kv_heads;
+  const long long first = ((long long)blockIdx.x * kWarps + (threadIdx.x >> 5)) * R;
+  // what the row's cache form has for this lane: two 16-byte (model), 8-byte (e4m3) or
+  // 4-byte (codes) pieces, the pieces' scales and a rope pair
+  uint4 y0[R], y1[R];
+  uint32_t pe[R];
+  __half s0[R], s1[R];
+  int slot[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    slot[i] = -1;
+    y0[i] = y1[i] = make_uint4(0u, 0u, 0u, 0u);
+    pe[i] = 0;
+    if (first + i < items) slot[i] = __ldg(a.slots + (a.kv_heads == 1 ? first + i : (first + i) / a.kv_heads));
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (slot[i] < 0 || slot[i] >= a.rows) continue;
+    const int kvh = a.kv_heads == 1 ? 0 : (int)((first + i) % a.kv_heads);
+    const long long row = (long long)slot[i] * a.kv_heads + kvh;
+    pe[i] = __ldg(reinterpret_cast<const uint32_t*>(static_cast<const T*>(a.k_pe_cache) + row * kPeDim) + lane);
+    const uint8_t* src = static_cast<const uint8_t*>(a.kv_cache);
     if constexpr (F == kModel) {
-      const uint4* src = reinterpret_cast<const uint4*>(static_cast<const T*>(a.kv_cache) + row * kDim);
-      y0 = __ldg(src + lane);
-      y1 = __ldg(src + 32 + lane);
+      y0[i] = __ldg(reinterpret_cast<const uint4*>(src + row * kDim * 2) + lane);
+      y1[i] = __ldg(reinterpret_cast<const uint4*>(src + row * kDim * 2) + 32 + lane);
     } else if constexpr (F == kFp8) {
-      const uint2* src = reinterpret_cast<const uint2*>(static_cast<const uint8_t*>(a.kv_cache) + row * kDim);
-      const uint2 w0 = __ldg(src + lane), w1 = __ldg(src + 32 + lane);
-      const uint32_t w[4] = {w0.x, w0.y, w1.x, w1.y};
+      const uint2 w0 = __ldg(reinterpret_cast<const uint2*>(src + row * kDim) + lane);
+      const uint2 w1 = __ldg(reinterpret_cast<const uint2*>(src + row * kDim) + 32 + lane);
+      y0[i] = make_uint4(w0.x, w0.y, 0u, 0u);
+      y1[i] = make_uint4(w1.x, w1.y, 0u, 0u);
+    } else {
+      y0[i].x = __ldg(reinterpret_cast<const uint32_t*>(src + row * kI4Bytes) + lane);
+      y1[i].x = __ldg(reinterpret_cast<const uint32_t*>(src + row * kI4Bytes) + 32 + lane);
+      const __half* sc = static_cast<const __half*>(a.scales) + row * kI4Groups;
+      s0[i] = __ldg(sc + (lane >> 2));
+      s1[i] = __ldg(sc + 8 + (lane >> 2));
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    if (first + i >= items) continue;
+    const bool real = slot[i] >= 0 && slot[i] < a.rows;
+    uint4 o0 = y0[i], o1 = y1[i];
+    if constexpr (F == kFp8) {
+      const uint32_t w[4] = {y0[i].x, y0[i].y, y1[i].x, y1[i].y};
       float f[2][8];
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
@@ -173,40 +236,49 @@ __global__ void __launch_bounds__(32 * kWarps) mla_cache_gather_kernel(CacheArgs
         f[k >> 2][2 * (k & 3)] = __half2float(__ushort_as_half(h.x)) * a.kv_scale;
         f[k >> 2][2 * (k & 3) + 1] = __half2float(__ushort_as_half(h.y)) * a.kv_scale;
       }
-      y0 = pack8<T>(f[0]);
-      y1 = pack8<T>(f[1]);
-    } else {
-      const uint32_t* src = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.kv_cache) + row * kI4Bytes);
-      const __half* sc = static_cast<const __half*>(a.scales) + row * kI4Groups;
-      const uint32_t w[2] = {__ldg(src + lane), __ldg(src + 32 + lane)};
-      const float s[2] = {__half2float(__ldg(sc + (lane >> 2))), __half2float(__ldg(sc + 8 + (lane >> 2)))};
-      float f[2][8];
+      o0 = pack8<T>(f[0]);
+      o1 = pack8<T>(f[1]);
+    } else if constexpr (F == kInt4) {
+      if (real) {
+        const uint32_t w[2] = {y0[i].x, y1[i].x};
+        const float s[2] = {__half2float(s0[i]), __half2float(s1[i])};
+        float f[2][8];
 #pragma unroll
-      for (int v = 0; v < 2; ++v)
+        for (int v = 0; v < 2; ++v)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float2 n = __half22float2(i4_pair(w[v], j));
-          f[v][2 * j] = n.x * s[v];
-          f[v][2 * j + 1] = n.y * s[v];
-        }
-      y0 = pack8<T>(f[0]);
-      y1 = pack8<T>(f[1]);
+          for (int j = 0; j < 4; ++j) {
+            const float2 n = __half22float2(i4_pair(w[v], j));
+            f[v][2 * j] = n.x * s[v];
+            f[v][2 * j + 1] = n.y * s[v];
+          }
+        o0 = pack8<T>(f[0]);
+        o1 = pack8<T>(f[1]);
+      }
     }
+    const long long t = a.kv_heads == 1 ? first + i : (first + i) / a.kv_heads;
+    const int kvh = (int)(first + i - t * a.kv_heads);
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.kv_out) + t * a.kv_token + kvh * a.kv_head);
+    dst[lane] = o0;
+    dst[32 + lane] = o1;
+    reinterpret_cast<uint32_t*>(static_cast<T*>(a.k_pe_out) + t * a.pe_token + kvh * a.pe_head)[lane] = pe[i];
   }
-  uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.kv_out) + t * a.kv_token + kvh * a.kv_head);
-  dst[lane] = y0;
-  dst[32 + lane] = y1;
-  reinterpret_cast<uint32_t*>(static_cast<T*>(a.k_pe_out) + t * a.pe_token + kvh * a.pe_head)[lane] = pe;
 }
 
+template <typename T, int F, int R>
+void launch_rows(const CacheArgs& a, bool append, cudaStream_t s) {
+  const long long items = a.tokens * a.kv_heads;
+  const unsigned grid = (unsigned)((items + kWarps * R - 1) / (kWarps * R));
+  if (append)
+    mla_cache_append_kernel<T, F, R><<<grid, 32 * kWarps, 0, s>>>(a);
+  else
+    mla_cache_gather_kernel<T, F, R><<<grid, 32 * kWarps, 0, s>>>(a);
+}
 template <typename T, int F>
 void launch_one(const CacheArgs& a, bool append, cudaStream_t s) {
-  const long long items = a.tokens * a.kv_heads;
-  const unsigned grid = (unsigned)((items + kWarps - 1) / kWarps);
-  if (append)
-    mla_cache_append_kernel<T, F><<<grid, 32 * kWarps, 0, s>>>(a);
+  if (a.tokens * a.kv_heads >= kLongRows)
+    launch_rows<T, F, kLong>(a, append, s);
   else
-    mla_cache_gather_kernel<T, F><<<grid, 32 * kWarps, 0, s>>>(a);
+    launch_rows<T, F, 1>(a, append, s);
 }
 
 int run(const char* fn, const CacheArgs& a, bool append, int form, int dtype, void* stream) {

@@ -317,6 +317,14 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
     int row_len[MT];
     long long pos = x0;                              // flattened tile
     int tile = 0;
+    // offsets within a stage: granule c of row r of a swizzled box is at c ^ (r & 7), so a
+    // thread's other granules are its first one's address with bits 4..6 exclusive-ored
+    const uint32_t k_off = (dq >> 1) * (kCodeBytes / 2) + (32 * tq + qr) * 128 + ((((dq & 1) * 4) ^ qr) << 4) + 4 * t;
+    const uint32_t r_off = kCodeBytes + (32 * tq + qr) * 128 + (((2 * dq) ^ qr) << 4) + 4 * t;
+    // word 8 warp + qr of a row: chunk 2 (warp % 4) + qr / 4 of box warp / 4, scale group 2 warp + qr / 4
+    const uint32_t v_off = (warp >> 2) * (kCodeBytes / 2) + 2 * t * 128 +
+                           (((2 * (warp & 3) + (qr >> 2)) ^ (2 * t)) << 4) + 4 * (qr & 3);
+    const uint32_t vs_off = kCodeBytes + kRopeBytes + 2 * t * 32 + (2 * warp + (qr >> 2)) * 2;
     while (it.left > 0) {
       // ---- a piece: tiles [j0, j1) of unit (s, sub)
       const int s = it.s, sub = it.sub, kvh = sub / p.groups, r_base = (sub % p.groups) * L::kRows;
@@ -361,8 +369,7 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
         const int st = tile % L::kStages;
         if ((tile & 31) == 0 && warp == 7) look_ahead(tile / 32 + 1);
         wait_full(full0 + 8 * st, (uint32_t)(tile / L::kStages) & 1u, abort, p.status, kErrLoad);
-        const uint8_t* codes = smem + st * kStage;
-        const uint8_t* rope = codes + kCodeBytes;
+        const uint32_t stage = st * kStage;
         uint8_t* scales = smem + st * kStage + kCodeBytes + kRopeBytes;
         const int valid = len - j * kTileR;
         if (valid < kTileR) {
@@ -375,20 +382,17 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
         // ---- S, this warp's rows [32 tq, +32) and dims [128 dq, +128) (and 16 rope dims)
 #pragma unroll
         for (int nb = 0; nb < 4; ++nb) {
-          const int row = 32 * tq + 8 * nb + qr;
-          const uint8_t* crow = codes + (dq >> 1) * (kCodeBytes / 2) + row * 128 + 4 * t;
-          const uint8_t* prow = rope + row * 128 + 4 * t;
-          const uint2 sc = *reinterpret_cast<const uint2*>(scales + row * 32 + dq * 8);
+          const uint2 sc = *reinterpret_cast<const uint2*>(scales + (32 * tq + 8 * nb + qr) * 32 + dq * 8);
           float c[MT][4];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) c[mt][0] = c[mt][1] = c[mt][2] = c[mt][3] = 0.f;
-          const uint32_t r0 = *reinterpret_cast<const uint32_t*>(prow + (((2 * dq) ^ qr) << 4));
-          const uint32_t r1 = *reinterpret_cast<const uint32_t*>(prow + (((2 * dq + 1) ^ qr) << 4));
+          const uint32_t r0 = *reinterpret_cast<const uint32_t*>(smem + (stage + r_off) + 1024 * nb);
+          const uint32_t r1 = *reinterpret_cast<const uint32_t*>(smem + ((stage + r_off) ^ 16u) + 1024 * nb);
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) mma16816<T>(c[mt], qpf[mt], r0, r1);
 #pragma unroll
           for (int jj = 0; jj < 4; ++jj) {
-            const uint32_t w = *reinterpret_cast<const uint32_t*>(crow + ((((dq & 1) * 4 + jj) ^ qr) << 4));
+            const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + ((stage + k_off) ^ (16u * jj)) + 1024 * nb);
             const uint32_t s16 = jj < 2 ? sc.x : sc.y;
             uint32_t f[4];
             widen4(w, u2h(__byte_perm(s16, 0, (jj & 1) ? 0x3232 : 0x1010)), f);
@@ -464,10 +468,6 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
             }
           }
         }
-        // word 8 warp + qr of a row: chunk 2 (warp % 4) + qr / 4 of box warp / 4, scale group 2 warp + qr / 4
-        const uint8_t* vbase = codes + (warp >> 2) * (kCodeBytes / 2) + 4 * (qr & 3);
-        const int chunk = 2 * (warp & 3) + (qr >> 2);
-        const uint8_t* sbase_v = scales + (2 * warp + (qr >> 2)) * 2;
 #pragma unroll
         for (int ks = 0; ks < 4; ++ks) {
           uint32_t pf[MT][4];
@@ -482,11 +482,12 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
           uint32_t f[2][2][4];   // [rows 2 t and 2 t + 8][even, odd dims][pair]
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const int ra = 16 * ks + 8 * h + 2 * t;
-            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(vbase + ra * 128 + ((chunk ^ (2 * t)) << 4));
-            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(vbase + ra * 128 + 128 + ((chunk ^ (2 * t + 1)) << 4));
-            const uint32_t sa = *reinterpret_cast<const unsigned short*>(sbase_v + ra * 32);
-            const uint32_t sb = *reinterpret_cast<const unsigned short*>(sbase_v + ra * 32 + 32);
+            // rows 16 ks + 8 h + 2 t and the next
+            const int up = 16 * ks + 8 * h;
+            const uint32_t w0 = *reinterpret_cast<const uint32_t*>(smem + (stage + v_off) + up * 128);
+            const uint32_t w1 = *reinterpret_cast<const uint32_t*>(smem + ((stage + v_off) ^ 16u) + 128 + up * 128);
+            const uint32_t sa = *reinterpret_cast<const unsigned short*>(smem + (stage + vs_off) + up * 32);
+            const uint32_t sb = *reinterpret_cast<const unsigned short*>(smem + (stage + vs_off) + up * 32 + 32);
             const __half2 s2 = u2h(sa | (sb << 16));
             widen4(__byte_perm(w0, w1, 0x5410), s2, f[h][0]);
             widen4(__byte_perm(w0, w1, 0x7632), s2, f[h][1]);

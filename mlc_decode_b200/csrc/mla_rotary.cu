@@ -13,6 +13,22 @@ namespace mla {
 namespace {
 
 constexpr int kThreads = 256;
+constexpr int kUnroll = 4;
+
+// Division of n < 2^31 by a run-time constant d >= 1: a 32-bit multiplication and shifts
+// (m = floor(2^32 (2^s - d) / d) + 1, s = ceil(log2 d); Granlund and Montgomery).
+struct FastDiv {
+  uint32_t m, s;
+  explicit FastDiv(uint32_t d) {
+    s = 0;
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int div(int n) const {
+    const uint32_t t = __umulhi(m, (uint32_t)n);
+    return (int)(((uint64_t)t + (uint32_t)n) >> s);
+  }
+};
 
 template <typename T>
 struct Io {
@@ -34,6 +50,7 @@ struct RotaryArgs {
   int tokens, heads, head_dim, rot, offset, interleaved;
   long long xs_token, xs_head, os_token, os_head;   // strides in elements
   int tokens_per_cta;
+  FastDiv by_items, by_heads;
 };
 
 template <typename T, int V>
@@ -55,71 +72,68 @@ __global__ void __launch_bounds__(kThreads) mla_rotary_kernel(RotaryArgs a) {
   }
   __syncthreads();
   using W = Vec<T, V>;
-  constexpr int VI = V == 1 ? 2 : V;            // interleaved: elements per item (whole pairs)
-  const int rot_items = a.interleaved ? a.rot / VI : pairs / V;
-  // the copied dims (only when the result goes elsewhere): [0, offset) and [offset + rot, head_dim)
-  const bool copy = a.out != a.x;
-  const int copy_items = copy ? (a.head_dim - a.rot) / V : 0;
-  const int items = rot_items + copy_items;
+  // an item: V rotated elements of a head (interleaved: whole pairs; halves: V pairs, a
+  // vector of either half) or V copied ones (only when the result goes elsewhere)
+  const int inter = a.interleaved;
+  const int rot_items = inter ? (V == 1 ? pairs : a.rot / V) : pairs / V;
+  const int items = rot_items + (a.out != a.x ? (a.head_dim - a.rot) / V : 0);
   const int total = nt * a.heads * items;
-  for (int i = threadIdx.x; i < total; i += kThreads) {
-    const int row = i / items, it = i - row * items;
-    const int t = row / a.heads, h = row - t * a.heads;
-    const T* x = static_cast<const T*>(a.x) + (t0 + t) * a.xs_token + h * a.xs_head;
-    T* o = static_cast<T*>(a.out) + (t0 + t) * a.os_token + h * a.os_head;
-    if (it >= rot_items) {
-      int d = (it - rot_items) * V;
-      if (d >= a.offset) d += a.rot;
-      *reinterpret_cast<W*>(o + d) = *reinterpret_cast<const W*>(x + d);
-      continue;
+  constexpr int kInterPairs = V == 1 ? 1 : V / 2;   // pairs of an interleaved item
+  for (int i0 = threadIdx.x; i0 < total; i0 += kThreads * kUnroll) {
+    W u[kUnroll], v[kUnroll];
+    T* dst[kUnroll];
+    int at[kUnroll];   // index of the first pair's angle in s_cs, -1: copied, -2: none
+#pragma unroll
+    for (int k = 0; k < kUnroll; ++k) {
+      const int i = i0 + k * kThreads;
+      at[k] = -2;
+      if (i >= total) continue;
+      const int row = a.by_items.div(i), it = i - row * items;
+      const int t = a.by_heads.div(row), h = row - t * a.heads;
+      const bool rot = it < rot_items;
+      int d;
+      if (rot) {
+        d = a.offset + (inter ? it * 2 * kInterPairs : it * V);
+        at[k] = t * pairs + (inter ? it * kInterPairs : it * V);
+      } else {
+        d = (it - rot_items) * V;
+        if (d >= a.offset) d += a.rot;
+        at[k] = -1;
+      }
+      const T* x = static_cast<const T*>(a.x) + (t0 + t) * a.xs_token + h * a.xs_head + d;
+      dst[k] = static_cast<T*>(a.out) + (t0 + t) * a.os_token + h * a.os_head + d;
+      u[k] = *reinterpret_cast<const W*>(x);
+      if (rot && (V == 1 || !inter)) v[k] = *reinterpret_cast<const W*>(x + (inter ? 1 : pairs));
     }
-    const float2* cs = s_cs + t * pairs;
-    if (a.interleaved) {
-      const int d = a.offset + it * VI;
-      using WI = Vec<T, V == 1 ? 1 : V>;
-      T e[VI];
-      if constexpr (V == 1) {
-        e[0] = x[d];
-        e[1] = x[d + 1];
-      } else {
-        const WI w = *reinterpret_cast<const WI*>(x + d);
 #pragma unroll
-        for (int k = 0; k < VI; ++k) e[k] = w.e[k];
-      }
+    for (int k = 0; k < kUnroll; ++k) {
+      if (at[k] == -2) continue;
+      if (at[k] >= 0) {
+        const float2* cs = s_cs + at[k];
+        if (V == 1 || !inter) {   // the two elements of a pair in u and v
 #pragma unroll
-      for (int k = 0; k < VI / 2; ++k) {
-        const float2 c = cs[it * (VI / 2) + k];
-        const float u = Io<T>::to(e[2 * k]), v = Io<T>::to(e[2 * k + 1]);
-        e[2 * k] = Io<T>::from(u * c.x - v * c.y);
-        e[2 * k + 1] = Io<T>::from(u * c.y + v * c.x);
-      }
-      if constexpr (V == 1) {
-        o[d] = e[0];
-        o[d + 1] = e[1];
-      } else {
-        WI w;
+          for (int e = 0; e < V; ++e) {
+            const float p = Io<T>::to(u[k].e[e]), q = Io<T>::to(v[k].e[e]);
+            u[k].e[e] = Io<T>::from(p * cs[e].x - q * cs[e].y);
+            v[k].e[e] = Io<T>::from(p * cs[e].y + q * cs[e].x);
+          }
+          *reinterpret_cast<W*>(dst[k] + (inter ? 1 : pairs)) = v[k];
+        } else {
 #pragma unroll
-        for (int k = 0; k < VI; ++k) w.e[k] = e[k];
-        *reinterpret_cast<WI*>(o + d) = w;
+          for (int e = 0; e < V / 2; ++e) {
+            const float p = Io<T>::to(u[k].e[2 * e]), q = Io<T>::to(u[k].e[2 * e + 1]);
+            u[k].e[2 * e] = Io<T>::from(p * cs[e].x - q * cs[e].y);
+            u[k].e[2 * e + 1] = Io<T>::from(p * cs[e].y + q * cs[e].x);
+          }
+        }
       }
-    } else {
-      const int d = a.offset + it * V;
-      W u = *reinterpret_cast<const W*>(x + d), v = *reinterpret_cast<const W*>(x + d + pairs);
-#pragma unroll
-      for (int k = 0; k < V; ++k) {
-        const float2 c = cs[it * V + k];
-        const float p = Io<T>::to(u.e[k]), q = Io<T>::to(v.e[k]);
-        u.e[k] = Io<T>::from(p * c.x - q * c.y);
-        v.e[k] = Io<T>::from(p * c.y + q * c.x);
-      }
-      *reinterpret_cast<W*>(o + d) = u;
-      *reinterpret_cast<W*>(o + d + pairs) = v;
+      *reinterpret_cast<W*>(dst[k]) = u[k];
     }
   }
 }
 
 template <typename T>
-cudaError_t launch(const RotaryArgs& a, cudaStream_t stream) {
+cudaError_t launch(RotaryArgs a, cudaStream_t stream) {
   constexpr int V = 16 / sizeof(T);
   // 16-byte accesses need every start (base, token, head, the rotated dims and, for
   // halves, their second half) on a vector boundary and whole vectors throughout
@@ -128,6 +142,9 @@ cudaError_t launch(const RotaryArgs& a, cudaStream_t stream) {
   const bool wide = ((reinterpret_cast<uintptr_t>(a.x) | reinterpret_cast<uintptr_t>(a.out)) & 15) == 0 &&
                     step % V == 0;
   const unsigned grid = (unsigned)((a.tokens + a.tokens_per_cta - 1) / a.tokens_per_cta);
+  const int v = wide ? V : 1;
+  const int items = (a.interleaved && v > 1 ? a.rot / v : a.rot / 2 / v) + (a.out != a.x ? (a.head_dim - a.rot) / v : 0);
+  a.by_items = FastDiv((uint32_t)items);
   const size_t smem = (size_t)a.tokens_per_cta * (a.rot / 2) * sizeof(float2);
   if (wide)
     mla_rotary_kernel<T, V><<<grid, kThreads, smem, stream>>>(a);
@@ -179,7 +196,8 @@ extern "C" int32_t mla_rotary(const void* x, void* out, const int32_t* positions
   int per = 2048 / (heads * head_dim / 8 + 1);
   per = per < 1 ? 1 : (per > 8 ? 8 : per);
   const RotaryArgs a{x, out, positions, turns, gain, tokens, heads, head_dim, rot_dim, offset, interleaved != 0,
-                     x_token_stride, x_head_stride, out_token_stride, out_head_stride, per};
+                     x_token_stride, x_head_stride, out_token_stride, out_head_stride, per, FastDiv(1),
+                     FastDiv((uint32_t)heads)};
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   const cudaError_t err = dtype == MLA_DTYPE_F16    ? launch<__half>(a, s)
                           : dtype == MLA_DTYPE_BF16 ? launch<__nv_bfloat16>(a, s)

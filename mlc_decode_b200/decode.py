@@ -10,7 +10,6 @@ allocated on first use and reused, and passes it through the C ABI.
 """
 from __future__ import annotations
 
-import contextlib
 import math
 import os
 import threading
@@ -40,14 +39,21 @@ def _check_tensor(name, t, shape, dtype, device):
         raise ValueError(f"{name} must be contiguous")
 
 
-@contextlib.contextmanager
-def _on_device(device):
-    """The current stream of ``device`` (its handle), with that device current."""
+def _fits(t, shape, dtype, index):
+    """The quick form of ``_check_tensor`` (which explains a failure): no more than a
+    microsecond a tensor."""
+    return (type(t) is torch.Tensor and t.dtype is dtype and t.get_device() == index and t.shape == shape
+            and t.is_contiguous())
+
+
+def _on_device(device, call, *args):
+    """``call(*args, stream)`` with ``device`` current, on its current stream (the raw handle:
+    a Stream object costs a microsecond)."""
     if torch.cuda.current_device() == device.index:
-        yield torch.cuda.current_stream(device).cuda_stream
+        call(*args, torch._C._cuda_getCurrentRawStream(device.index))
     else:
         with torch.cuda.device(device):
-            yield torch.cuda.current_stream(device).cuda_stream
+            call(*args, torch._C._cuda_getCurrentRawStream(device.index))
 
 
 class MlaDecodeKernel:
@@ -475,38 +481,41 @@ class MlaPagedDecodeKernel:
         """
         b, h, smax, ql, kvh = self.batch, self.heads, self.max_seqlen_kv, self.q_len, self.kv_heads
         dtype = q.dtype if isinstance(q, torch.Tensor) else None
-        if dtype not in _DTYPES:
+        code = _DTYPES.get(dtype)
+        if code is None:
             raise ValueError(f"q must be float16 or bfloat16, got {dtype}")
         dev = q.device
         qshape = (b, h) if ql == 1 else (b, ql, h)
-        _check_tensor("q", q, (*qshape, DIM), dtype, None)
-        _check_tensor("q_pe", q_pe, (*qshape, PE_DIM), dtype, dev)
-        _check_tensor("out", out, (*qshape, DIM), dtype, dev)
-        if lse is not None:
-            _check_tensor("lse", lse, qshape, torch.float32, dev)
-        if cache_seqlens is not None:
-            _check_tensor("cache_seqlens", cache_seqlens, (b,), torch.int32, dev)
-        if block_table is None:
-            lead, page_size, num_pages, max_pages = (b, smax, kvh), 0, 0, 0
-        else:
+        table_ptr, page_size, num_pages, max_pages = None, 0, 0, 0
+        lead = (b, smax, kvh)
+        if block_table is not None:
             if not isinstance(kv_codes, torch.Tensor) or kv_codes.dim() != 4:
                 raise ValueError(f"kv_codes must be [num_pages, page_size, {kvh}, 256]")
-            num_pages, page_size = int(kv_codes.shape[0]), int(kv_codes.shape[1])
-            if block_table.dim() != 2 or block_table.shape[0] != b:
-                raise ValueError(f"block_table must be [batch, max_pages], got {tuple(block_table.shape)}")
-            max_pages = int(block_table.shape[1])
-            _check_tensor("block_table", block_table, (b, max_pages), torch.int32, dev)
+            if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
+                raise ValueError("block_table must be an int32 tensor [batch, max_pages]")
+            num_pages, page_size = kv_codes.shape[:2]
+            max_pages = block_table.shape[1]
+            table_ptr = block_table.data_ptr()
             lead = (num_pages, page_size, kvh)
-        _check_tensor("kv_codes", kv_codes, (*lead, DIM // 2), torch.uint8, dev)
-        _check_tensor("kv_scales", kv_scales, (*lead, DIM // 32), torch.float16, dev)
-        _check_tensor("k_pe_cache", k_pe_cache, (*lead, PE_DIM), dtype, dev)
-        with _on_device(dev) as stream:
+        index = dev.index
+        for name, t, shape, want in (("q", q, (*qshape, DIM), dtype), ("q_pe", q_pe, (*qshape, PE_DIM), dtype),
+                                     ("out", out, (*qshape, DIM), dtype),
+                                     ("kv_codes", kv_codes, (*lead, DIM // 2), torch.uint8),
+                                     ("kv_scales", kv_scales, (*lead, DIM // 32), torch.float16),
+                                     ("k_pe_cache", k_pe_cache, (*lead, PE_DIM), dtype),
+                                     ("lse", lse, qshape, torch.float32),
+                                     ("cache_seqlens", cache_seqlens, (b,), torch.int32),
+                                     ("block_table", block_table, (b, max_pages), torch.int32)):
+            if not _fits(t, shape, want, index) and not (t is None and name in ("lse", "cache_seqlens", "block_table")):
+                _check_tensor(name, t, shape, want, dev)
+        ws = self._ws.get((index, dtype, "int4"))
+        if ws is None:
             ws = self._int4_workspace(dev, dtype)
-            capi.decode_ext_int4kv(q.data_ptr(), q_pe.data_ptr(), kv_codes.data_ptr(), kv_scales.data_ptr(),
-                                   k_pe_cache.data_ptr(), None if block_table is None else block_table.data_ptr(),
-                                   None if cache_seqlens is None else cache_seqlens.data_ptr(), out.data_ptr(),
-                                   None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), b, ql, h, kvh,
-                                   smax, page_size, num_pages, max_pages, _DTYPES[dtype], self._ccfg, stream)
+        _on_device(dev, capi.decode_ext_int4kv, q.data_ptr(), q_pe.data_ptr(), kv_codes.data_ptr(),
+                   kv_scales.data_ptr(), k_pe_cache.data_ptr(), table_ptr,
+                   None if cache_seqlens is None else cache_seqlens.data_ptr(), out.data_ptr(),
+                   None if lse is None else lse.data_ptr(), ws.data_ptr(), ws.numel(), b, ql, h, kvh, smax, page_size,
+                   num_pages, max_pages, code, self._ccfg)
 
     def _int4_workspace(self, device, dtype):
         key = (device.index, dtype, "int4")
@@ -515,8 +524,9 @@ class MlaPagedDecodeKernel:
             with self._lock:
                 ws = self._ws.get(key)
                 if ws is None:
-                    n = capi.int4kv_workspace_bytes(self.batch, self.q_len, self.heads, self.kv_heads,
-                                                    self.max_seqlen_kv, _DTYPES[dtype], self._ccfg)
+                    with torch.cuda.device(device):   # (the plan counts the device's SMs)
+                        n = capi.int4kv_workspace_bytes(self.batch, self.q_len, self.heads, self.kv_heads,
+                                                        self.max_seqlen_kv, _DTYPES[dtype], self._ccfg)
                     ws = self._ws[key] = torch.zeros(max(n, 1), dtype=torch.uint8, device=device)
         return ws
 

@@ -15,7 +15,7 @@ import threading
 import torch
 
 from . import capi
-from .decode import _DTYPES, _FP8, DIM, PE_DIM, _check_tensor, _on_device
+from .decode import _DTYPES, _FP8, DIM, PE_DIM, _check_tensor, _fits, _on_device
 
 INT4_GROUP = 32                      # dims per scale of the 4-bit form
 INT4_GROUPS = DIM // INT4_GROUP      # scales per row
@@ -45,24 +45,20 @@ def extend_block_tables(block_table, cache_seqlens, new_lens, free_pages, free_p
     i32 = torch.int32
     _check_tensor("block_table", block_table, (b, max_pages), i32, None)
     n, nf = (t.numel() if isinstance(t, torch.Tensor) else -1 for t in (slots, free_pages))
-    for name, t, shape in (("cache_seqlens", cache_seqlens, (b,)), ("new_lens", new_lens, (b,)),
-                           ("free_pages", free_pages, (nf,)), ("free_pos", free_pos, (1,)),
-                           ("new_seqlens", new_seqlens, (b,)), ("new_free_pos", new_free_pos, (1,)),
-                           ("slots", slots, (n,)), ("positions", positions, (n,))):
-        if not (type(t) is torch.Tensor and t.dtype == i32 and t.device == dev and t.shape == shape
-                and t.is_contiguous()):
-            _check_tensor(name, t, shape, i32, dev)
-    if cu_new is not None:
-        _check_tensor("cu_new", cu_new, (b + 1,), i32, dev)
-    with _on_device(dev) as stream:
-        nbytes = capi.block_tables_workspace_bytes(b, n)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-        capi.extend_block_tables(block_table.data_ptr(), cache_seqlens.data_ptr(), new_lens.data_ptr(),
-                                 free_pages.data_ptr(), free_pos.data_ptr(), new_seqlens.data_ptr(),
-                                 new_free_pos.data_ptr(), slots.data_ptr(), positions.data_ptr(),
-                                 None if cu_new is None else cu_new.data_ptr(),
-                                 None if ws is None else ws.data_ptr(), nbytes, b, max_pages, page_size, num_pages,
-                                 nf, n, q_len, stream)
+    index = dev.index
+    for name, t, k in (("cache_seqlens", cache_seqlens, b), ("new_lens", new_lens, b), ("free_pages", free_pages, nf),
+                       ("free_pos", free_pos, 1), ("new_seqlens", new_seqlens, b), ("new_free_pos", new_free_pos, 1),
+                       ("slots", slots, n), ("positions", positions, n), ("cu_new", cu_new, b + 1)):
+        if not (type(t) is torch.Tensor and t.dtype is i32 and t.get_device() == index and t.numel() == k
+                and t.dim() == 1 and t.is_contiguous()) and not (t is None and name == "cu_new"):
+            _check_tensor(name, t, (k,), i32, dev)
+    nbytes = capi.block_tables_workspace_bytes(b, n)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _on_device(dev, capi.extend_block_tables, block_table.data_ptr(), cache_seqlens.data_ptr(), new_lens.data_ptr(),
+               free_pages.data_ptr(), free_pos.data_ptr(), new_seqlens.data_ptr(), new_free_pos.data_ptr(),
+               slots.data_ptr(), positions.data_ptr(), None if cu_new is None else cu_new.data_ptr(),
+               None if ws is None else ws.data_ptr(), nbytes, b, max_pages, int(page_size), int(num_pages), nf, n,
+               int(q_len))
 
 
 def rotary_frequencies(rot_dim, base=10000.0, scaling=None):
@@ -141,6 +137,9 @@ class Rotary:
 
     def turns(self, device):
         """Turns per position of every pair, float64 on ``device`` (kept)."""
+        t = self._dev.get(device)
+        if t is not None:
+            return t
         device = torch.device(device)
         if device.type == "cuda" and device.index is None:
             device = torch.device("cuda", torch.cuda.current_device())
@@ -155,31 +154,30 @@ class Rotary:
     def __call__(self, x, positions, out, offset=0):
         if not isinstance(x, torch.Tensor) or x.dim() != 3 or x.dtype not in _ROTARY_DTYPES:
             raise ValueError("x must be a float16, bfloat16 or float32 tensor [tokens, heads, head_dim]")
-        n, h, d = x.shape
+        n, h, d = shape = x.shape
         if not 0 <= int(offset) <= d - self.rot_dim:
             raise ValueError(f"dims [{offset}, {offset} + {self.rot_dim}) must lie inside the head's {d}")
-        _check_rows("x", x, x.shape, x.dtype, None)
-        _check_rows("out", out, x.shape, x.dtype, x.device, written=True)
-        _check_tensor("positions", positions, (n,), torch.int32, x.device)
+        dev = x.device
+        if not _fits(x, shape, x.dtype, dev.index) or dev.type != "cuda":
+            _check_rows("x", x, shape, x.dtype, None)
+        if not _fits(out, shape, x.dtype, dev.index):
+            _check_rows("out", out, shape, x.dtype, dev, written=True)
+        if not _fits(positions, (n,), torch.int32, dev.index):
+            _check_tensor("positions", positions, (n,), torch.int32, dev)
         if n == 0:
             return
-        if out.data_ptr() == x.data_ptr() and out.stride() != x.stride() or \
-                out.data_ptr() != x.data_ptr() and _ranges_meet(x, out):
+        xp, op, xs, os_ = x.data_ptr(), out.data_ptr(), x.stride(), out.stride()
+        if xs != os_ if xp == op else _ranges_meet(x, out):
             raise ValueError("out must be x itself or must not overlap it")
-        turns = self.turns(x.device)
-        with _on_device(x.device) as stream:
-            capi.rotary(x.data_ptr(), out.data_ptr(), positions.data_ptr(), turns.data_ptr(), self.gain, n, h, d,
-                        self.rot_dim, offset, self.interleaved, x.stride()[:2], out.stride()[:2],
-                        _ROTARY_DTYPES[x.dtype], stream)
+        _on_device(dev, capi.rotary, xp, op, positions.data_ptr(), self.turns(dev).data_ptr(), self.gain, n, h, d,
+                   self.rot_dim, int(offset), self.interleaved, xs[0], xs[1], os_[0], os_[1], _ROTARY_DTYPES[x.dtype])
 
 
 def _ranges_meet(a, b):
-    def span(t):
-        last = sum((s - 1) * st for s, st in zip(t.shape, t.stride()))
-        return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
-
-    (a0, a1), (b0, b1) = span(a), span(b)
-    return a0 < b1 and b0 < a1
+    a0, b0 = a.data_ptr(), b.data_ptr()
+    first, low, high = (a, a0, b0) if a0 < b0 else (b, b0, a0)
+    last = sum((s - 1) * st for s, st in zip(first.shape, first.stride()))
+    return high < low + (last + 1) * first.element_size()
 
 
 def _check_rows(name, t, shape, dtype, device, written=False, align=1):
@@ -213,31 +211,36 @@ def _check_rows(name, t, shape, dtype, device, written=False, align=1):
 
 def _strides(t):
     """Token and head stride; of a dimension of one entry any stride will do."""
-    return tuple(t.stride(d) if t.shape[d] > 1 else 0 for d in (0, 1))
+    (n, h, _), (sn, sh, _) = t.shape, t.stride()
+    return sn if n > 1 else 0, sh if h > 1 else 0
 
 
 def _check_cache(kv_cache, k_pe_cache, kv_scale, kv_scales, dtype, device):
     """(form, rows, kv_heads) of a cache [a, b, kv_heads, width] in any of its forms."""
+    def need(name, t, shape, want):
+        if not _fits(t, shape, want, device.index):
+            _check_tensor(name, t, shape, want, device)
+
     if not isinstance(kv_cache, torch.Tensor) or kv_cache.dim() != 4:
         raise ValueError("kv_cache must be [num_pages, page_size, kv_heads, width] (or [batch, max_seqlen, ...])")
-    lead = tuple(kv_cache.shape[:3])
+    lead = kv_cache.shape[:3]
     if kv_scales is not None:
         if kv_scale is not None:
             raise ValueError("kv_scale belongs to an e4m3 cache, kv_scales to a 4-bit one: pass one of them")
         form = capi.MLA_CACHE_INT4
-        _check_tensor("kv_cache", kv_cache, (*lead, INT4_BYTES), torch.uint8, device)
-        _check_tensor("kv_scales", kv_scales, (*lead, INT4_GROUPS), torch.float16, device)
+        need("kv_cache", kv_cache, (*lead, INT4_BYTES), torch.uint8)
+        need("kv_scales", kv_scales, (*lead, INT4_GROUPS), torch.float16)
     elif kv_cache.dtype in (torch.uint8, _FP8):
         if kv_scale is None:
             raise ValueError("an e4m3 kv_cache needs kv_scale, a 4-bit one kv_scales")
         form = capi.MLA_CACHE_FP8
-        _check_tensor("kv_cache", kv_cache, (*lead, DIM), kv_cache.dtype, device)
+        need("kv_cache", kv_cache, (*lead, DIM), kv_cache.dtype)
     else:
         if kv_scale is not None:
             raise ValueError("kv_scale belongs to an e4m3 cache")
         form = capi.MLA_CACHE_MODEL
-        _check_tensor("kv_cache", kv_cache, (*lead, DIM), dtype, device)
-    _check_tensor("k_pe_cache", k_pe_cache, (*lead, PE_DIM), dtype, device)
+        need("kv_cache", kv_cache, (*lead, DIM), dtype)
+    need("k_pe_cache", k_pe_cache, (*lead, PE_DIM), dtype)
     return form, lead[0] * lead[1], lead[2]
 
 
@@ -246,9 +249,12 @@ def _check_dense(kv, k_pe, slots, written):
     if dtype not in _DTYPES or kv.dim() != 3:
         raise ValueError("kv must be a float16 or bfloat16 tensor [tokens, kv_heads, 512]")
     n, h = kv.shape[:2]
-    _check_rows("kv", kv, (n, h, DIM), dtype, None, written, align=8)
-    _check_rows("k_pe", k_pe, (n, h, PE_DIM), dtype, kv.device, written, align=8)
-    _check_tensor("slots", slots, (n,), torch.int32, kv.device)
+    dev = kv.device
+    for name, t, shape in (("kv", kv, (n, h, DIM)), ("k_pe", k_pe, (n, h, PE_DIM))):
+        if not (_fits(t, shape, dtype, dev.index) and dev.type == "cuda" and t.data_ptr() % 16 == 0):
+            _check_rows(name, t, shape, dtype, None if name == "kv" else dev, written, align=8)
+    if not _fits(slots, (n,), torch.int32, dev.index):
+        _check_tensor("slots", slots, (n,), torch.int32, dev)
     return n, h, dtype
 
 
@@ -273,14 +279,13 @@ def cache_append(kv, k_pe, slots, kv_cache, k_pe_cache, kv_scale=None, kv_scales
     if rotary is not None:
         if rotary.rot_dim != PE_DIM:
             raise ValueError(f"rotary must turn {PE_DIM} dims, not {rotary.rot_dim}")
-        _check_tensor("positions", positions, (n,), torch.int32, dev)
-        turns, gain, inter = rotary.turns(dev), rotary.gain, rotary.interleaved
-    with _on_device(dev) as stream:
-        capi.cache_append(kv.data_ptr(), k_pe.data_ptr(), slots.data_ptr(), kv_cache.data_ptr(),
-                          None if kv_scales is None else kv_scales.data_ptr(), k_pe_cache.data_ptr(),
-                          1.0 if kv_scale is None else kv_scale, None if rotary is None else positions.data_ptr(),
-                          None if rotary is None else turns.data_ptr(), gain, inter, n, h, rows, _strides(kv),
-                          _strides(k_pe), form, _DTYPES[dtype], stream)
+        if not _fits(positions, (n,), torch.int32, dev.index):
+            _check_tensor("positions", positions, (n,), torch.int32, dev)
+        turns, gain, inter = rotary.turns(dev).data_ptr(), rotary.gain, rotary.interleaved
+    _on_device(dev, capi.cache_append, kv.data_ptr(), k_pe.data_ptr(), slots.data_ptr(), kv_cache.data_ptr(),
+               None if kv_scales is None else kv_scales.data_ptr(), k_pe_cache.data_ptr(),
+               1.0 if kv_scale is None else float(kv_scale), None if rotary is None else positions.data_ptr(), turns, gain,
+               inter, n, h, rows, *_strides(kv), *_strides(k_pe), form, _DTYPES[dtype])
 
 
 def cache_gather(slots, kv_cache, k_pe_cache, kv, k_pe, kv_scale=None, kv_scales=None):
@@ -293,7 +298,7 @@ def cache_gather(slots, kv_cache, k_pe_cache, kv, k_pe, kv_scale=None, kv_scales
     form, rows, kvh = _check_cache(kv_cache, k_pe_cache, kv_scale, kv_scales, dtype, dev)
     if kvh != h:
         raise ValueError(f"kv has {h} KV heads, the cache {kvh}")
-    with _on_device(dev) as stream:
-        capi.cache_gather(slots.data_ptr(), kv_cache.data_ptr(), None if kv_scales is None else kv_scales.data_ptr(),
-                          k_pe_cache.data_ptr(), 1.0 if kv_scale is None else kv_scale, kv.data_ptr(),
-                          k_pe.data_ptr(), n, h, rows, _strides(kv), _strides(k_pe), form, _DTYPES[dtype], stream)
+    _on_device(dev, capi.cache_gather, slots.data_ptr(), kv_cache.data_ptr(),
+               None if kv_scales is None else kv_scales.data_ptr(), k_pe_cache.data_ptr(),
+               1.0 if kv_scale is None else float(kv_scale), kv.data_ptr(), k_pe.data_ptr(), n, h, rows, *_strides(kv),
+               *_strides(k_pe), form, _DTYPES[dtype])
