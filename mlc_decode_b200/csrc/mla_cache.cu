@@ -10,6 +10,9 @@
 // also turns rope pair l.  In calls long enough to fill the GPU a warp has the loads of
 // kLong rows in flight before it stores the first.
 #include <cuda_fp8.h>
+#include <string.h>
+
+#include <type_traits>
 
 #include "mla_cache.cuh"
 
@@ -29,7 +32,7 @@ struct CacheArgs {
   void* kv_cache;          // [rows][kv_heads][512] (model type or e4m3) or [rows][kv_heads][256] (codes)
   void* scales;            // [rows][kv_heads][16] float16 (4-bit form)
   void* k_pe_cache;        // [rows][kv_heads][64]
-  float kv_scale;
+  float kv_scale, kv_recip;   // e4m3: the scale, and its reciprocal or 0 (quotient)
   const int* positions;    // rotary: [tokens], else nullptr
   const double* turns;     // [32]
   float gain;
@@ -61,45 +64,91 @@ __device__ __forceinline__ uint32_t code_of(float f, float s) {
   return f == f ? (uint32_t)((int)fminf(fmaxf(r, -8.f), 7.f) + 8) : 8u;
 }
 
+// The larger of two pairs' magnitudes, element by element; NaN wins.
+template <typename T>
+__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
+  a &= 0x7fff7fffu;
+  b &= 0x7fff7fffu;
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  } else {
+    const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&m);
+  }
+}
+
 // This lane's eight dims as codes (low nibble first: dims 0 2 4 6 1 3 5 7) and its
 // group's scale.  s = half(max / 7) may round below max / 7, hence the clamp; a group of
 // zeros (or one whose scale rounds to zero) has code 8, the value 0; NaN stores as 0 and
 // infinities as the largest code.
-// f / s is f times the reciprocal, off by two units of its last place (below 1.3e-6 up
-// to 8): it rounds to the same integer unless it lies within 1e-5 of a half, where (and
-// for values that are not finite) the lane divides.  One reciprocal, no conversion
-// instruction: the sum with 1.5 x 2^23 leaves the rounded integer in its last bits.
-__device__ __forceinline__ uint32_t quantise8(const float (&f)[8], __half* scale) {
-  float m = 0.f, sum = 0.f;
+// max / 7 as a product with 1 / 7, off by 2^-23, rounds to the same half: the maximum has
+// at most 11 bits, so max / 7 is no closer than 2^-12 / 7 of itself to the middle of two
+// normal halves.  f / s is f times an approximate reciprocal, off by less than 2e-6: it
+// rounds to the same integer unless it lies within 1e-5 of a half.  There, in groups that
+// are not finite and where the scale is below fp16's normal range (the only groups whose
+// quotients may pass 7.5) the lane divides.  A fused product and sum with 1.5 x 2^23 + 8 leaves the code in the last
+// bits of its result, which a multiply-add moves to its nibble: five instructions a dim.
+template <typename T>
+__device__ __forceinline__ uint32_t quantise8(uint4 x, __half* scale) {
+  const uint32_t m2 = max_abs2<T>(max_abs2<T>(x.x, x.y), max_abs2<T>(x.z, x.w));
+  const float2 mm = Elt<T>::to2(m2);
+  float m = mm.x > mm.y || mm.x != mm.x ? mm.x : mm.y;   // (NaN wins)
+  float o = __shfl_xor_sync(0xffffffffu, m, 1);
+  m = o > m || o != o ? o : m;
+  o = __shfl_xor_sync(0xffffffffu, m, 2);
+  m = o > m || o != o ? o : m;
+  float f[8];
+  unpack8<T>(x, f);
+  __half s = __float2half_rn(m * (1.f / 7.f));
+  float sf = __half2float(s);
+  float inv;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf));
+  constexpr float kMagic = 12582920.f;               // 1.5 x 2^23 + 8
+  constexpr uint32_t kBits = 0x4b400000u;            // the bits of 1.5 x 2^23
+  uint32_t w = 0u - kBits * 0x11111111u;
+  float far = 0.f;                                   // largest distance from an integer
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    m = fmaxf(m, fabsf(f[k]));
-    sum += fabsf(f[k]);
+    const float t = fmaf(f[k], inv, kMagic);
+    far = fmaxf(far, fabsf(fmaf(f[k], inv, kMagic - t)));
+    w += __float_as_uint(t) << (4 * ((k >> 1) + 4 * (k & 1)));
   }
-  const bool finite = sum < INFINITY;
-  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-  m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-  const __half s = __float2half_rn(fminf(__fdiv_rn(m, 7.f), 65504.f));
-  const float sf = __half2float(s);
+  if (far > 0.49999f || !(sf >= 6.103515625e-5f && sf < INFINITY)) {
+    // (the four lanes of a group agree on the scale: all of them or none pass the second test)
+    if (!(sf >= 6.103515625e-5f && sf < INFINITY)) {
+      m = 0.f;                                       // the largest of the numbers' magnitudes
+#pragma unroll
+      for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(f[k]));
+      const unsigned group = 0xfu << (threadIdx.x & 28);
+      m = fmaxf(m, __shfl_xor_sync(group, m, 1));
+      m = fmaxf(m, __shfl_xor_sync(group, m, 2));
+      s = __float2half_rn(fminf(__fdiv_rn(m, 7.f), 65504.f));
+      sf = __half2float(s);
+    }
+    w = 0x88888888u;
+    if (sf > 0.f) {
+      w = 0;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) w |= code_of(f[k], sf) << (4 * ((k >> 1) + 4 * (k & 1)));
+    }
+  }
   *scale = s;
-  if (!(sf > 0.f)) return 0x88888888u;
-  const float inv = __fdiv_rn(1.f, sf);
-  const float magic = 12582912.f;   // 1.5 x 2^23: a sum's last bit counts ones
-  uint32_t w = 0;
-  bool sure = finite;
-#pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float q = fminf(fmaxf(f[k] * inv, -8.f), 7.f);
-    const float t = q + magic;
-    sure = sure && fabsf(fabsf(q - (t - magic)) - 0.5f) > 1e-5f;
-    w |= ((__float_as_uint(t) + 8u) & 15u) << (4 * ((k >> 1) + 4 * (k & 1)));
-  }
-  if (!sure) {
-    w = 0;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) w |= code_of(f[k], sf) << (4 * ((k >> 1) + 4 * (k & 1)));
-  }
   return w;
+}
+
+// e4m3 code pair of (a / s, b / s), each quotient rounded to float32 first: with the
+// correctly rounded reciprocal r of s, q = a r and one residual step give the correctly
+// rounded quotient (Markstein), unless s's significand is all ones or the numbers leave
+// float32's normal range; the host then sets r to zero and the lane divides.  A
+// quotient past e4m3's range saturates whatever its last bit.
+__device__ __forceinline__ float quotient(float a, float s, float r) {
+  if (r == 0.f) return __fdiv_rn(a, s);
+  const float q = a * r;
+  return fabsf(q) < 1e6f ? fmaf(fmaf(-q, s, a), r, q) : q;
+}
+__device__ __forceinline__ uint32_t e4m3x2_of(float a, float b, float s, float r) {
+  return __nv_cvt_float2_to_fp8x2(make_float2(quotient(a, s, r), quotient(b, s, r)), __NV_SATFINITE, __NV_E4M3);
 }
 
 enum Form { kModel = MLA_CACHE_MODEL, kFp8 = MLA_CACHE_FP8, kInt4 = MLA_CACHE_INT4 };
@@ -109,9 +158,10 @@ __global__ void __launch_bounds__(32 * kWarps) mla_cache_append_kernel(CacheArgs
   const int lane = threadIdx.x & 31;
   const long long items = a.tokens * a.kv_heads;
   const long long first = ((long long)blockIdx.x * kWarps + (threadIdx.x >> 5)) * R;
-  const int d0 = a.interleaved ? 2 * lane : lane, d1 = a.interleaved ? 2 * lane + 1 : lane + 32;
   uint4 x0[R], x1[R];
-  T p0[R], p1[R];
+  // rope pair `lane`: two neighbours in one word, or elements lane and lane + 32 (halves)
+  const bool words = a.interleaved || a.positions == nullptr;
+  uint32_t pe2[R];
   int slot[R], kvh[R], pos[R];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -125,8 +175,11 @@ __global__ void __launch_bounds__(32 * kWarps) mla_cache_append_kernel(CacheArgs
     x0[i] = __ldg(kv + lane);
     x1[i] = __ldg(kv + 32 + lane);
     const T* pe = static_cast<const T*>(a.k_pe) + t * a.pe_token + kvh[i] * a.pe_head;
-    p0[i] = pe[d0];
-    p1[i] = pe[d1];
+    if (words)
+      pe2[i] = __ldg(reinterpret_cast<const uint32_t*>(pe) + lane);
+    else
+      pe2[i] = __ldg(reinterpret_cast<const unsigned short*>(pe) + lane) |
+               ((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(pe) + 32 + lane) << 16);
     pos[i] = a.positions != nullptr ? __ldg(a.positions + t) : 0;
   }
 #pragma unroll
@@ -138,26 +191,22 @@ __global__ void __launch_bounds__(32 * kWarps) mla_cache_append_kernel(CacheArgs
       dst[lane] = x0[i];
       dst[32 + lane] = x1[i];
     } else {
-      float f0[8], f1[8];
-      unpack8<T>(x0[i], f0);
-      unpack8<T>(x1[i], f1);
       if constexpr (F == kFp8) {
+        float f0[8], f1[8];
+        unpack8<T>(x0[i], f0);
+        unpack8<T>(x1[i], f1);
         uint32_t w[4];
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           const float* f = k < 2 ? f0 + 4 * k : f1 + 4 * (k - 2);
-          const uint32_t lo = __nv_cvt_float2_to_fp8x2(
-              make_float2(__fdiv_rn(f[0], a.kv_scale), __fdiv_rn(f[1], a.kv_scale)), __NV_SATFINITE, __NV_E4M3);
-          const uint32_t hi = __nv_cvt_float2_to_fp8x2(
-              make_float2(__fdiv_rn(f[2], a.kv_scale), __fdiv_rn(f[3], a.kv_scale)), __NV_SATFINITE, __NV_E4M3);
-          w[k] = lo | (hi << 16);
+          w[k] = e4m3x2_of(f[0], f[1], a.kv_scale, a.kv_recip) | (e4m3x2_of(f[2], f[3], a.kv_scale, a.kv_recip) << 16);
         }
         uint2* dst = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.kv_cache) + row * kDim);
         dst[lane] = make_uint2(w[0], w[1]);
         dst[32 + lane] = make_uint2(w[2], w[3]);
       } else {
         __half s0, s1;
-        const uint32_t w0 = quantise8(f0, &s0), w1 = quantise8(f1, &s1);
+        const uint32_t w0 = quantise8<T>(x0[i], &s0), w1 = quantise8<T>(x1[i], &s1);
         uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.kv_cache) + row * kI4Bytes);
         dst[lane] = w0;
         dst[32 + lane] = w1;
@@ -168,15 +217,18 @@ __global__ void __launch_bounds__(32 * kWarps) mla_cache_append_kernel(CacheArgs
         }
       }
     }
-    T* pc = static_cast<T*>(a.k_pe_cache) + row * kPeDim;
+    uint32_t pair = pe2[i];
     if (a.positions != nullptr) {
       const float2 c = rotary_cos_sin(pos[i], __ldg(a.turns + lane), a.gain);
-      const float u = Elt<T>::to1(p0[i]), v = Elt<T>::to1(p1[i]);
-      pc[d0] = Elt<T>::from(u * c.x - v * c.y);
-      pc[d1] = Elt<T>::from(u * c.y + v * c.x);
+      const float2 u = Elt<T>::to2(pair);
+      pair = Elt<T>::pack2(u.x * c.x - u.y * c.y, u.x * c.y + u.y * c.x);
+    }
+    T* pc = static_cast<T*>(a.k_pe_cache) + row * kPeDim;
+    if (words) {
+      reinterpret_cast<uint32_t*>(pc)[lane] = pair;
     } else {
-      pc[d0] = p0[i];
-      pc[d1] = p1[i];
+      reinterpret_cast<unsigned short*>(pc)[lane] = (unsigned short)pair;
+      reinterpret_cast<unsigned short*>(pc)[32 + lane] = (unsigned short)(pair >> 16);
     }
   }
 }
@@ -356,6 +408,9 @@ int32_t mla_cache_append(const void* kv, const void* k_pe, const int32_t* slots,
   a.scales = kv_scales;
   a.k_pe_cache = k_pe_cache;
   a.kv_scale = kv_scale;
+  uint32_t bits;
+  memcpy(&bits, &kv_scale, sizeof(bits));
+  a.kv_recip = kv_scale > 1e-30f && kv_scale < 1e30f && (bits & 0x7fffffu) != 0x7fffffu ? 1.f / kv_scale : 0.f;
   a.positions = positions;
   a.turns = turns;
   a.gain = gain;

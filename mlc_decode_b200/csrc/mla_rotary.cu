@@ -3,17 +3,18 @@
 // frequency times a gain.  Pairs are neighbours (interleaved) or half the rotated width
 // apart (halves); the head's other dims are copied.
 //
-// Bound: bytes, x once in and once out.  A CTA takes kTokens tokens: its threads first
+// Bound: bytes, x once in and once out.  A CTA takes a few tokens: its threads first
 // fill a shared table of the tokens' cosines and sines (one angle per pair and token
 // instead of one per pair, token and head: the angle is a double product and a
-// sincospif), then walk the tokens' heads in vectors of 16 bytes.
+// sincospif), then walk the tokens' heads in vectors of 16 bytes, one in flight per
+// thread and many threads per SM (two and four per thread, with their registers, were
+// slower: 142 us against 170 and 189 at 8192 x 128 x 192, interleaved).
 #include "mla_cache.cuh"
 
 namespace mla {
 namespace {
 
 constexpr int kThreads = 256;
-constexpr int kUnroll = 4;
 
 // Division of n < 2^31 by a run-time constant d >= 1: a 32-bit multiplication and shifts
 // (m = floor(2^32 (2^s - d) / d) + 1, s = ceil(log2 d); Granlund and Montgomery).
@@ -79,56 +80,39 @@ __global__ void __launch_bounds__(kThreads) mla_rotary_kernel(RotaryArgs a) {
   const int items = rot_items + (a.out != a.x ? (a.head_dim - a.rot) / V : 0);
   const int total = nt * a.heads * items;
   constexpr int kInterPairs = V == 1 ? 1 : V / 2;   // pairs of an interleaved item
-  for (int i0 = threadIdx.x; i0 < total; i0 += kThreads * kUnroll) {
-    W u[kUnroll], v[kUnroll];
-    T* dst[kUnroll];
-    int at[kUnroll];   // index of the first pair's angle in s_cs, -1: copied, -2: none
-#pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      const int i = i0 + k * kThreads;
-      at[k] = -2;
-      if (i >= total) continue;
-      const int row = a.by_items.div(i), it = i - row * items;
-      const int t = a.by_heads.div(row), h = row - t * a.heads;
-      const bool rot = it < rot_items;
-      int d;
-      if (rot) {
-        d = a.offset + (inter ? it * 2 * kInterPairs : it * V);
-        at[k] = t * pairs + (inter ? it * kInterPairs : it * V);
-      } else {
-        d = (it - rot_items) * V;
-        if (d >= a.offset) d += a.rot;
-        at[k] = -1;
-      }
-      const T* x = static_cast<const T*>(a.x) + (t0 + t) * a.xs_token + h * a.xs_head + d;
-      dst[k] = static_cast<T*>(a.out) + (t0 + t) * a.os_token + h * a.os_head + d;
-      u[k] = *reinterpret_cast<const W*>(x);
-      if (rot && (V == 1 || !inter)) v[k] = *reinterpret_cast<const W*>(x + (inter ? 1 : pairs));
+  for (int i = threadIdx.x; i < total; i += kThreads) {
+    const int row = a.by_items.div(i), it = i - row * items;
+    const int t = a.by_heads.div(row), h = row - t * a.heads;
+    const T* x = static_cast<const T*>(a.x) + (t0 + t) * a.xs_token + h * a.xs_head;
+    T* o = static_cast<T*>(a.out) + (t0 + t) * a.os_token + h * a.os_head;
+    if (it >= rot_items) {
+      int d = (it - rot_items) * V;
+      if (d >= a.offset) d += a.rot;
+      *reinterpret_cast<W*>(o + d) = *reinterpret_cast<const W*>(x + d);
+      continue;
     }
+    const int d = a.offset + (inter ? it * 2 * kInterPairs : it * V);
+    const float2* cs = s_cs + t * pairs + (inter ? it * kInterPairs : it * V);
+    W u = *reinterpret_cast<const W*>(x + d);
+    if (V == 1 || !inter) {   // the two elements of a pair in u and v
+      const int gap = inter ? 1 : pairs;
+      W v = *reinterpret_cast<const W*>(x + d + gap);
 #pragma unroll
-    for (int k = 0; k < kUnroll; ++k) {
-      if (at[k] == -2) continue;
-      if (at[k] >= 0) {
-        const float2* cs = s_cs + at[k];
-        if (V == 1 || !inter) {   // the two elements of a pair in u and v
-#pragma unroll
-          for (int e = 0; e < V; ++e) {
-            const float p = Io<T>::to(u[k].e[e]), q = Io<T>::to(v[k].e[e]);
-            u[k].e[e] = Io<T>::from(p * cs[e].x - q * cs[e].y);
-            v[k].e[e] = Io<T>::from(p * cs[e].y + q * cs[e].x);
-          }
-          *reinterpret_cast<W*>(dst[k] + (inter ? 1 : pairs)) = v[k];
-        } else {
-#pragma unroll
-          for (int e = 0; e < V / 2; ++e) {
-            const float p = Io<T>::to(u[k].e[2 * e]), q = Io<T>::to(u[k].e[2 * e + 1]);
-            u[k].e[2 * e] = Io<T>::from(p * cs[e].x - q * cs[e].y);
-            u[k].e[2 * e + 1] = Io<T>::from(p * cs[e].y + q * cs[e].x);
-          }
-        }
+      for (int e = 0; e < V; ++e) {
+        const float p = Io<T>::to(u.e[e]), q = Io<T>::to(v.e[e]);
+        u.e[e] = Io<T>::from(p * cs[e].x - q * cs[e].y);
+        v.e[e] = Io<T>::from(p * cs[e].y + q * cs[e].x);
       }
-      *reinterpret_cast<W*>(dst[k]) = u[k];
+      *reinterpret_cast<W*>(o + d + gap) = v;
+    } else {
+#pragma unroll
+      for (int e = 0; e < V / 2; ++e) {
+        const float p = Io<T>::to(u.e[2 * e]), q = Io<T>::to(u.e[2 * e + 1]);
+        u.e[2 * e] = Io<T>::from(p * cs[e].x - q * cs[e].y);
+        u.e[2 * e + 1] = Io<T>::from(p * cs[e].y + q * cs[e].x);
+      }
     }
+    *reinterpret_cast<W*>(o + d) = u;
   }
 }
 
