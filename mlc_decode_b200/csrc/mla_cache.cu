@@ -7,8 +7,10 @@
 // lane l holds dims [8 l, 8 l + 8) and [256 + 8 l, 256 + 8 l + 8) in two 16-byte loads,
 // so the four lanes of a 32-dim group find its largest value in two shuffles, each
 // lane's eight codes are one 32-bit word and a warp stores whole 128-byte lines; lane l
-// also turns rope pair l.  In calls long enough to fill the GPU a warp has the loads of
-// kLong rows in flight before it stores the first.
+// also turns rope pair l.  A gather long enough to fill the GPU has the loads of two rows
+// in flight per warp (131072 4-bit rows 39 us, 41 with one); an append, which computes
+// more, does better with one row and more warps (58 us against 62 and 94 with two and
+// four).
 #include <cuda_fp8.h>
 #include <string.h>
 
@@ -20,8 +22,7 @@ namespace mla {
 namespace {
 
 constexpr int kWarps = 8;
-constexpr int kLong = 2;            // rows in flight per warp of a long call
-constexpr long long kLongRows = 148ll * 64 * kLong;   // a long call: every warp slot of the GPU gets that many
+constexpr long long kLongRows = 148ll * 64 * 2;   // a long gather: two rows for every warp slot of the GPU
 
 struct CacheArgs {
   const void* kv;          // append: rows in; gather: unused
@@ -87,8 +88,10 @@ __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
 // normal halves.  f / s is f times an approximate reciprocal, off by less than 2e-6: it
 // rounds to the same integer unless it lies within 1e-5 of a half.  There, in groups that
 // are not finite and where the scale is below fp16's normal range (the only groups whose
-// quotients may pass 7.5) the lane divides.  A fused product and sum with 1.5 x 2^23 + 8 leaves the code in the last
-// bits of its result, which a multiply-add moves to its nibble: five instructions a dim.
+// quotients may pass 7.5) the lane divides.  A fused product and sum with 1.5 x 2^23 rounds to
+// the integer; the codes of the even and of the odd dims are summed with their nibbles'
+// weights as floats (below 2^16, exact): the float pipe has twice the rate of the
+// integer one, which bounded this kernel.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(uint4 x, __half* scale) {
   const uint32_t m2 = max_abs2<T>(max_abs2<T>(x.x, x.y), max_abs2<T>(x.z, x.w));
@@ -104,16 +107,21 @@ __device__ __forceinline__ uint32_t quantise8(uint4 x, __half* scale) {
   float sf = __half2float(s);
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf));
-  constexpr float kMagic = 12582920.f;               // 1.5 x 2^23 + 8
-  constexpr uint32_t kBits = 0x4b400000u;            // the bits of 1.5 x 2^23
-  uint32_t w = 0u - kBits * 0x11111111u;
+  constexpr float kMagic = 12582912.f;               // 1.5 x 2^23: a sum's last bit counts ones
+  float even = 34952.f, odd = 34952.f;               // 0x8888: n + 8 is the code
   float far = 0.f;                                   // largest distance from an integer
 #pragma unroll
   for (int k = 0; k < 8; ++k) {
-    const float t = fmaf(f[k], inv, kMagic);
-    far = fmaxf(far, fabsf(fmaf(f[k], inv, kMagic - t)));
-    w += __float_as_uint(t) << (4 * ((k >> 1) + 4 * (k & 1)));
+    const float minus_n = kMagic - fmaf(f[k], inv, kMagic);
+    far = fmaxf(far, fabsf(fmaf(f[k], inv, minus_n)));
+    const float weight = -(float)(1 << (4 * (k >> 1)));
+    if (k & 1)
+      odd = fmaf(minus_n, weight, odd);
+    else
+      even = fmaf(minus_n, weight, even);
   }
+  // 2^23 + a 16-bit integer has it in its last bits
+  uint32_t w = __byte_perm(__float_as_uint(even + 8388608.f), __float_as_uint(odd + 8388608.f), 0x5410);
   if (far > 0.49999f || !(sf >= 6.103515625e-5f && sf < INFINITY)) {
     // (the four lanes of a group agree on the scale: all of them or none pass the second test)
     if (!(sf >= 6.103515625e-5f && sf < INFINITY)) {
@@ -153,83 +161,66 @@ __device__ __forceinline__ uint32_t e4m3x2_of(float a, float b, float s, float r
 
 enum Form { kModel = MLA_CACHE_MODEL, kFp8 = MLA_CACHE_FP8, kInt4 = MLA_CACHE_INT4 };
 
-template <typename T, int F, int R>
-__global__ void __launch_bounds__(32 * kWarps) mla_cache_append_kernel(CacheArgs a) {
+template <typename T, int F>
+__global__ void __launch_bounds__(32 * kWarps, 8) mla_cache_append_kernel(CacheArgs a) {
   const int lane = threadIdx.x & 31;
-  const long long items = a.tokens * a.kv_heads;
-  const long long first = ((long long)blockIdx.x * kWarps + (threadIdx.x >> 5)) * R;
-  uint4 x0[R], x1[R];
+  const long long item = (long long)blockIdx.x * kWarps + (threadIdx.x >> 5);
+  if (item >= a.tokens * a.kv_heads) return;
+  const long long t = a.kv_heads == 1 ? item : item / a.kv_heads;
+  const int kvh = (int)(item - t * a.kv_heads);
+  const int slot = __ldg(a.slots + t);
+  const uint4* kv = reinterpret_cast<const uint4*>(static_cast<const T*>(a.kv) + t * a.kv_token + kvh * a.kv_head);
+  const uint4 x0 = __ldg(kv + lane), x1 = __ldg(kv + 32 + lane);
+  const T* pe = static_cast<const T*>(a.k_pe) + t * a.pe_token + kvh * a.pe_head;
   // rope pair `lane`: two neighbours in one word, or elements lane and lane + 32 (halves)
   const bool words = a.interleaved || a.positions == nullptr;
-  uint32_t pe2[R];
-  int slot[R], kvh[R], pos[R];
-#pragma unroll
-  for (int i = 0; i < R; ++i) {
-    slot[i] = -1;
-    if (first + i >= items) continue;
-    const long long t = a.kv_heads == 1 ? first + i : (first + i) / a.kv_heads;
-    kvh[i] = (int)(first + i - t * a.kv_heads);
-    slot[i] = __ldg(a.slots + t);
-    const uint4* kv =
-        reinterpret_cast<const uint4*>(static_cast<const T*>(a.kv) + t * a.kv_token + kvh[i] * a.kv_head);
-    x0[i] = __ldg(kv + lane);
-    x1[i] = __ldg(kv + 32 + lane);
-    const T* pe = static_cast<const T*>(a.k_pe) + t * a.pe_token + kvh[i] * a.pe_head;
-    if (words)
-      pe2[i] = __ldg(reinterpret_cast<const uint32_t*>(pe) + lane);
-    else
-      pe2[i] = __ldg(reinterpret_cast<const unsigned short*>(pe) + lane) |
-               ((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(pe) + 32 + lane) << 16);
-    pos[i] = a.positions != nullptr ? __ldg(a.positions + t) : 0;
+  uint32_t pair = words ? __ldg(reinterpret_cast<const uint32_t*>(pe) + lane)
+                        : __ldg(reinterpret_cast<const unsigned short*>(pe) + lane) |
+                              ((uint32_t)__ldg(reinterpret_cast<const unsigned short*>(pe) + 32 + lane) << 16);
+  if (a.positions != nullptr) {
+    const float2 c = rotary_cos_sin(__ldg(a.positions + t), __ldg(a.turns + lane), a.gain);
+    const float2 u = Elt<T>::to2(pair);
+    pair = Elt<T>::pack2(u.x * c.x - u.y * c.y, u.x * c.y + u.y * c.x);
   }
+  if (slot < 0 || slot >= a.rows) return;
+  const long long row = (long long)slot * a.kv_heads + kvh;
+  if constexpr (F == kModel) {
+    uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.kv_cache) + row * kDim);
+    dst[lane] = x0;
+    dst[32 + lane] = x1;
+  } else {
+    if constexpr (F == kFp8) {
+      float f0[8], f1[8];
+      unpack8<T>(x0, f0);
+      unpack8<T>(x1, f1);
+      uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < R; ++i) {
-    if (slot[i] < 0 || slot[i] >= a.rows) continue;   // (the same for the whole warp)
-    const long long row = (long long)slot[i] * a.kv_heads + kvh[i];
-    if constexpr (F == kModel) {
-      uint4* dst = reinterpret_cast<uint4*>(static_cast<T*>(a.kv_cache) + row * kDim);
-      dst[lane] = x0[i];
-      dst[32 + lane] = x1[i];
+      for (int k = 0; k < 4; ++k) {
+        const float* f = k < 2 ? f0 + 4 * k : f1 + 4 * (k - 2);
+        w[k] = e4m3x2_of(f[0], f[1], a.kv_scale, a.kv_recip) | (e4m3x2_of(f[2], f[3], a.kv_scale, a.kv_recip) << 16);
+      }
+      uint2* dst = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.kv_cache) + row * kDim);
+      dst[lane] = make_uint2(w[0], w[1]);
+      dst[32 + lane] = make_uint2(w[2], w[3]);
     } else {
-      if constexpr (F == kFp8) {
-        float f0[8], f1[8];
-        unpack8<T>(x0[i], f0);
-        unpack8<T>(x1[i], f1);
-        uint32_t w[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float* f = k < 2 ? f0 + 4 * k : f1 + 4 * (k - 2);
-          w[k] = e4m3x2_of(f[0], f[1], a.kv_scale, a.kv_recip) | (e4m3x2_of(f[2], f[3], a.kv_scale, a.kv_recip) << 16);
-        }
-        uint2* dst = reinterpret_cast<uint2*>(static_cast<uint8_t*>(a.kv_cache) + row * kDim);
-        dst[lane] = make_uint2(w[0], w[1]);
-        dst[32 + lane] = make_uint2(w[2], w[3]);
-      } else {
-        __half s0, s1;
-        const uint32_t w0 = quantise8<T>(x0[i], &s0), w1 = quantise8<T>(x1[i], &s1);
-        uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.kv_cache) + row * kI4Bytes);
-        dst[lane] = w0;
-        dst[32 + lane] = w1;
-        if ((lane & 3) == 0) {
-          __half* sc = static_cast<__half*>(a.scales) + row * kI4Groups;
-          sc[lane >> 2] = s0;
-          sc[8 + (lane >> 2)] = s1;
-        }
+      __half s0, s1;
+      const uint32_t w0 = quantise8<T>(x0, &s0), w1 = quantise8<T>(x1, &s1);
+      uint32_t* dst = reinterpret_cast<uint32_t*>(static_cast<uint8_t*>(a.kv_cache) + row * kI4Bytes);
+      dst[lane] = w0;
+      dst[32 + lane] = w1;
+      if ((lane & 3) == 0) {
+        __half* sc = static_cast<__half*>(a.scales) + row * kI4Groups;
+        sc[lane >> 2] = s0;
+        sc[8 + (lane >> 2)] = s1;
       }
     }
-    uint32_t pair = pe2[i];
-    if (a.positions != nullptr) {
-      const float2 c = rotary_cos_sin(pos[i], __ldg(a.turns + lane), a.gain);
-      const float2 u = Elt<T>::to2(pair);
-      pair = Elt<T>::pack2(u.x * c.x - u.y * c.y, u.x * c.y + u.y * c.x);
-    }
-    T* pc = static_cast<T*>(a.k_pe_cache) + row * kPeDim;
-    if (words) {
-      reinterpret_cast<uint32_t*>(pc)[lane] = pair;
-    } else {
-      reinterpret_cast<unsigned short*>(pc)[lane] = (unsigned short)pair;
-      reinterpret_cast<unsigned short*>(pc)[32 + lane] = (unsigned short)(pair >> 16);
-    }
+  }
+  T* pc = static_cast<T*>(a.k_pe_cache) + row * kPeDim;
+  if (words) {
+    reinterpret_cast<uint32_t*>(pc)[lane] = pair;
+  } else {
+    reinterpret_cast<unsigned short*>(pc)[lane] = (unsigned short)pair;
+    reinterpret_cast<unsigned short*>(pc)[32 + lane] = (unsigned short)(pair >> 16);
   }
 }
 
@@ -316,21 +307,16 @@ __global__ void __launch_bounds__(32 * kWarps) mla_cache_gather_kernel(CacheArgs
   }
 }
 
-template <typename T, int F, int R>
-void launch_rows(const CacheArgs& a, bool append, cudaStream_t s) {
-  const long long items = a.tokens * a.kv_heads;
-  const unsigned grid = (unsigned)((items + kWarps * R - 1) / (kWarps * R));
-  if (append)
-    mla_cache_append_kernel<T, F, R><<<grid, 32 * kWarps, 0, s>>>(a);
-  else
-    mla_cache_gather_kernel<T, F, R><<<grid, 32 * kWarps, 0, s>>>(a);
-}
 template <typename T, int F>
 void launch_one(const CacheArgs& a, bool append, cudaStream_t s) {
-  if (a.tokens * a.kv_heads >= kLongRows)
-    launch_rows<T, F, kLong>(a, append, s);
+  const long long items = a.tokens * a.kv_heads;
+  const unsigned grid = (unsigned)((items + kWarps - 1) / kWarps);
+  if (append)
+    mla_cache_append_kernel<T, F><<<grid, 32 * kWarps, 0, s>>>(a);
+  else if (items >= kLongRows)
+    mla_cache_gather_kernel<T, F, 2><<<(grid + 1) / 2, 32 * kWarps, 0, s>>>(a);
   else
-    launch_rows<T, F, 1>(a, append, s);
+    mla_cache_gather_kernel<T, F, 1><<<grid, 32 * kWarps, 0, s>>>(a);
 }
 
 int run(const char* fn, const CacheArgs& a, bool append, int form, int dtype, void* stream) {

@@ -83,36 +83,40 @@ __global__ void __launch_bounds__(kThreads) mla_rotary_kernel(RotaryArgs a) {
   for (int i = threadIdx.x; i < total; i += kThreads) {
     const int row = a.by_items.div(i), it = i - row * items;
     const int t = a.by_heads.div(row), h = row - t * a.heads;
-    const T* x = static_cast<const T*>(a.x) + (t0 + t) * a.xs_token + h * a.xs_head;
-    T* o = static_cast<T*>(a.out) + (t0 + t) * a.os_token + h * a.os_head;
-    if (it >= rot_items) {
-      int d = (it - rot_items) * V;
-      if (d >= a.offset) d += a.rot;
-      *reinterpret_cast<W*>(o + d) = *reinterpret_cast<const W*>(x + d);
-      continue;
-    }
-    const int d = a.offset + (inter ? it * 2 * kInterPairs : it * V);
-    const float2* cs = s_cs + t * pairs + (inter ? it * kInterPairs : it * V);
-    W u = *reinterpret_cast<const W*>(x + d);
-    if (V == 1 || !inter) {   // the two elements of a pair in u and v
-      const int gap = inter ? 1 : pairs;
-      W v = *reinterpret_cast<const W*>(x + d + gap);
+    // rotated and copied items load and store at the same places in the code (apart, they
+    // would take turns: 174 us against 142)
+    const bool rot = it < rot_items;
+    int d = (it - rot_items) * V;
+    if (rot)
+      d = a.offset + (inter ? it * 2 * kInterPairs : it * V);
+    else if (d >= a.offset)
+      d += a.rot;
+    const T* x = static_cast<const T*>(a.x) + (t0 + t) * a.xs_token + h * a.xs_head + d;
+    T* o = static_cast<T*>(a.out) + (t0 + t) * a.os_token + h * a.os_head + d;
+    const int gap = inter ? 1 : pairs;
+    const bool two = rot && (V == 1 || !inter);   // the two elements of a pair in u and v
+    W u = *reinterpret_cast<const W*>(x), v = u;
+    if (two) v = *reinterpret_cast<const W*>(x + gap);
+    if (rot) {
+      const float2* cs = s_cs + t * pairs + (inter ? it * kInterPairs : it * V);
+      if (V == 1 || !inter) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float p = Io<T>::to(u.e[e]), q = Io<T>::to(v.e[e]);
-        u.e[e] = Io<T>::from(p * cs[e].x - q * cs[e].y);
-        v.e[e] = Io<T>::from(p * cs[e].y + q * cs[e].x);
-      }
-      *reinterpret_cast<W*>(o + d + gap) = v;
-    } else {
+        for (int e = 0; e < V; ++e) {
+          const float p = Io<T>::to(u.e[e]), q = Io<T>::to(v.e[e]);
+          u.e[e] = Io<T>::from(p * cs[e].x - q * cs[e].y);
+          v.e[e] = Io<T>::from(p * cs[e].y + q * cs[e].x);
+        }
+      } else {
 #pragma unroll
-      for (int e = 0; e < V / 2; ++e) {
-        const float p = Io<T>::to(u.e[2 * e]), q = Io<T>::to(u.e[2 * e + 1]);
-        u.e[2 * e] = Io<T>::from(p * cs[e].x - q * cs[e].y);
-        u.e[2 * e + 1] = Io<T>::from(p * cs[e].y + q * cs[e].x);
+        for (int e = 0; e < V / 2; ++e) {
+          const float p = Io<T>::to(u.e[2 * e]), q = Io<T>::to(u.e[2 * e + 1]);
+          u.e[2 * e] = Io<T>::from(p * cs[e].x - q * cs[e].y);
+          u.e[2 * e + 1] = Io<T>::from(p * cs[e].y + q * cs[e].x);
+        }
       }
     }
-    *reinterpret_cast<W*>(o + d) = u;
+    if (two) *reinterpret_cast<W*>(o + gap) = v;
+    *reinterpret_cast<W*>(o) = u;
   }
 }
 

@@ -157,16 +157,14 @@ struct Kv8 {};
 // fp16 and P.V runs once instead of as the bf16 hi/lo pair.
 template <typename T, bool kF16>
 struct Cv {};
-// The 4-bit variant: latent rows as codes and group scales (mla_cache.cuh).  Eight
-// converter warps widen each CTA's codes to fp16 ((n - 8) s, one rounding) straight
-// from registers: 16-byte global loads a tile ahead, no staging in shared memory.  A
-// tile is four operand slots of 64 rows x 128 dims: for QK^T slot u of CTA r holds dims
-// [128 u, +128) of the CTA's own 64 rows.  P.V wants from CTA r dims
-// [256 nh + 128 r, +128) of both row halves: for its own half that is slot 2 nh + r as it
-// stands (the same bytes are a K-major operand of QK^T and an MN-major operand of
-// P.V); slot 2 nh + 1 - r is refilled with the peer's half once QK^T has read it.  So a
-// value is widened 1.5 times instead of twice and a tile takes 64 KB, which leaves room
-// for two tiles.  Q's latent dims are fp16, the rope dims run in T.
+// The 4-bit variant: latent rows as codes and group scales (mla_cache.cuh).  Sixteen
+// converter warps widen codes to fp16 ((n - 8) s, one rounding) straight from
+// registers: 16-byte global loads a tile ahead, no staging in shared memory.  Two
+// warps own one operand slot of 16 KB: four K units (this CTA's 64 rows x 128 dims) and four
+// V units (128 of this CTA's dims of 64 rows), and refill it as soon as its GEMM has
+// read it.  (Slots shared by both GEMMs, a value widened 1.5 times instead of twice, were
+// held from QK^T's fill to P.V's end: 5.1 us a tile pass with room for two, 279 us at
+// b64 h128 s8192.)  Q's latent dims are fp16, the rope dims run in T.
 template <typename T>
 struct Kv4 {};
 template <typename K>
@@ -216,9 +214,9 @@ struct Cfg<Kv4<T>> {
   static constexpr uint32_t kPvFmt = 0;
   static constexpr uint32_t kRopeFmt = Cfg<T>::kFmt;
   static constexpr int kPParts = 1;
-  static constexpr int kKStages = 8;                 // two tiles of four operand slots
+  static constexpr int kKStages = 8;                 // four K and four V slots, one tile
   static constexpr uint32_t kKStageBytes = kStageBytes;
-  static constexpr int kVStages = 0;                 // (P.V reads the same slots)
+  static constexpr int kVStages = 0;                 // (counted above)
   static constexpr int kV8Stages = 2;                // rope rows of two tiles
   using PT = __half;
 };
@@ -237,7 +235,14 @@ struct Cfg<Cv<T, kF16>> {
   using PT = typename std::conditional<kToF16, __half, typename Cfg<T>::PT>::type;
 };
 template <typename K>
-constexpr int threads_of() { return (Io<K>::kKv8 || Io<K>::kKv4 || Io<K>::kConv) ? 512 : 384; }
+constexpr int threads_of() { return Io<K>::kKv4 ? 768 : (Io<K>::kKv8 || Io<K>::kConv) ? 512 : 384; }
+// 4-bit variant: 24 warps, launched with 80 registers a thread
+constexpr uint32_t kRegsLow4 = 64, kRegsSoftmax4 = 160;
+static_assert(5 * 128 * kRegsLow4 + 128 * kRegsSoftmax4 <= 768 * 80, "register split (4-bit variant)");
+template <typename K>
+constexpr uint32_t regs_low() { return Io<K>::kKv4 ? kRegsLow4 : kRegsLow; }
+template <typename K>
+constexpr uint32_t regs_softmax() { return Io<K>::kKv4 ? kRegsSoftmax4 : kRegsSoftmax; }
 
 struct Barriers {
   uint64_t kfull[8], kempty[8];
@@ -527,8 +532,10 @@ struct TileRows {
   int kvh;
 };
 constexpr int kMapBatch = 32;
+constexpr int kPrefetch = 3;          // tiles ahead whose codes are pulled into L2
 constexpr int kFirst = 1 << 16, kLast = 1 << 17;
-constexpr uint32_t kMapReaders = 9;   // eight converter warps and the rope producer; CTA 0: the two issuers too
+constexpr int kWidenWarps = 16;
+constexpr uint32_t kMapReaders = kWidenWarps + 1;   // with the rope producer; CTA 0: the two issuers too
 
 template <typename T>
 __device__ __forceinline__ void tile_scout(const Params& p, const Ctx& c, uint32_t rank, int pair, uint8_t* smem,
@@ -606,10 +613,23 @@ __device__ __forceinline__ void k_producer(const Params& p, const Ctx& c, uint32
     const uint32_t rempty0 = ptx::smem_u32(&bars->v8empty[0]);
     const uint64_t once = ptx::l2_policy_evict_first();
     const TileMapReader<false> map(reinterpret_cast<const TileRows*>(smem + S::kMap), bars);
-    for (uint32_t gi = 0; gi < it.t1 - it.t; ++gi) {
-      const uint32_t b = gi & 1u;
-      TileRows w;
-      if (!map.get(c, gi, &w)) return;
+    const uint32_t n = it.t1 - it.t;
+    TileRows ahead[kPrefetch + 1] = {};   // tiles i .. i - kPrefetch
+    for (uint32_t i = 0; i < n + kPrefetch; ++i) {
+#pragma unroll
+      for (int k = kPrefetch; k > 0; --k) ahead[k] = ahead[k - 1];
+      if (i < n) {
+        if (!map.get(c, i, &ahead[0])) return;
+        // this CTA's rows into L2, for its K units and the peer's V units
+        const int rows = ahead[0].valid & 255;
+        if (p.kv_heads == 1 && rows > 0) {
+          ptx::prefetch_l2(p.kv + (size_t)ahead[0].own * (kDim / 2), rows * (kDim / 2));
+          ptx::prefetch_l2(p.kv_scales + (size_t)ahead[0].own * 16, rows * 32);
+        }
+      }
+      if (i < kPrefetch) continue;
+      const uint32_t gi = i - kPrefetch, b = gi & 1u;
+      const TileRows w = ahead[kPrefetch];
       // no rows here (masked, or on a page outside the cache): zeros, from past the
       // tensor map's last row
       const int y = w.own >= 0 ? w.own : p.num_rows;
@@ -933,14 +953,11 @@ __device__ __forceinline__ void v_converter(const Params& p, const Ctx& c, int p
 }
 
 // ---------------------------------------------------------------------------
-// 4-bit variant: converter warps (warps 8..15).  A thread's share is a row's scale
-// group (32 codes: one 16-byte load and one scale in, four 16-byte fp16 granules out).
-// Filling a tile's four slots for QK^T, warps 2 u and 2 u + 1 take slot u (32 rows each,
-// four shares a thread); refilling two of them with the peer's rows for P.V, four warps
-// take a slot (16 rows each, two shares a thread): a warp waits, fences and signals
-// twice a tile, not once per slot and share.  A fill's registers take the next
-// tile's loads as soon as they are stored.  Rows past the length and rows of absent
-// pages become zeros.
+// 4-bit variant: converter warps (warps 8..23), two for each operand slot of 64 rows x
+// 128 dims.  A thread's share is a row's scale group (32 codes: one 16-byte load and one
+// scale in, four 16-byte fp16 granules out), four shares a tile, whose registers take
+// the next tile's loads as soon as they are stored.  Rows past the length and rows of
+// absent pages become zeros.
 // ---------------------------------------------------------------------------
 struct Codes32 {
   uint4 w;            // 32 codes
@@ -964,8 +981,6 @@ __device__ __forceinline__ uint4 widen8(uint32_t w, __half2 s2) {
                     h2_bits(__hmul2(e, s2)));
 }
 
-constexpr uint32_t kFillWarps = 2, kRefillWarps = 4;   // per slot (and CTA)
-
 template <typename T>
 __device__ __forceinline__ void kv4_converter(const Params& p, const Ctx& c, uint32_t rank, int pair, uint8_t* smem,
                                               Barriers* bars, int cw, int lane) {
@@ -974,73 +989,59 @@ __device__ __forceinline__ void kv4_converter(const Params& p, const Ctx& c, uin
   const PieceIter it(p, pair);
   const uint32_t n = it.t1 - it.t;
   if (n == 0) return;
-  // lane: row lane & 7 of every eight, group g of the unit.  The eight lanes of a 16-byte
-  // store phase are eight rows of one group, whose granules the swizzle puts in eight
-  // distinct columns: granule k of group g at (4 (g & 1) + k) ^ (row & 7) of box g / 2
-  const int g = lane >> 3;
-  const int u = cw >> 1, fr = 32 * (cw & 1) + (lane & 7);    // fill: slot u, rows fr + 8 e
-  const int nh = cw >> 2, pr = 16 * (cw & 3) + (lane & 7);   // refill: rows pr + 8 e
-  const uint32_t vs = 2 * nh + (1 - rank);                   // refill: slot (of its tile's four)
-  const uint32_t gx = (uint32_t)((4 * (g & 1)) ^ (lane & 7)) << 4;
-  uint8_t* fill_row = smem + S::kKRing + u * kStageBytes + (g >> 1) * kChunkBytes + fr * 128;
-  uint8_t* refill_row = smem + S::kKRing + vs * kStageBytes + (g >> 1) * kChunkBytes + pr * 128;
-  const uint32_t kfull_leader = ptx::mapa(ptx::smem_u32(&bars->kfull[u]), 0);
-  const uint32_t vfull_leader = ptx::mapa(ptx::smem_u32(&bars->vfull[vs]), 0);
-  const uint32_t freed = ptx::smem_u32(&bars->vempty[u]);    // P.V has read the slot
-  const uint32_t read = ptx::smem_u32(&bars->kempty[vs]);    // QK^T has read the slot
-  const int fq = 4 * u + g, pq = 8 * nh + 4 * (int)rank + g;   // scale groups
-  auto load = [&](Codes32& x, long long at, bool real, int q) {
-    x = Codes32{make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u), 0};
-    if (real) {
-      x.w = __ldg(reinterpret_cast<const uint4*>(p.kv + at * (kDim / 2)) + q);
-      x.s = __ldg(reinterpret_cast<const unsigned short*>(p.kv_scales) + at * 16 + q);
-    }
-  };
-  auto store = [&](uint8_t* dst, const Codes32& x) {
-    const __half2 s2 = __half2half2(__ushort_as_half(x.s));
-    *reinterpret_cast<uint4*>(dst + gx) = widen8(x.w.x, s2);
-    *reinterpret_cast<uint4*>(dst + (gx ^ 16u)) = widen8(x.w.y, s2);
-    *reinterpret_cast<uint4*>(dst + (gx ^ 32u)) = widen8(x.w.z, s2);
-    *reinterpret_cast<uint4*>(dst + (gx ^ 48u)) = widen8(x.w.w, s2);
-  };
-  TileRows w;
+  // warps 0..7: K unit u, dims [128 u, +128) of this CTA's rows; warps 8..15: V unit
+  // (nh, th), dims [256 nh + 128 rank, +128) of row half th; two warps a unit, 32 rows each
+  const int un = cw >> 1, u = un & 3, nh = u >> 1, th = u & 1;
+  const bool is_k = un < 4, own = is_k || th == (int)rank;
+  // lane: row r0 + 8 e, group g of the unit: eight lanes load two rows' 64 bytes.  Stores:
+  // granule k of the group at (4 (g & 1) + k) ^ (r & 7) of box g / 2; the second box's
+  // lanes take their granules in the order 2 3 0 1, so the eight lanes of a store phase
+  // (two rows, four groups) hit eight distinct granule columns
+  const int g = lane & 3, r0 = 32 * (cw & 1) + (lane >> 2);
+  const int q = is_k ? 4 * u + g : 8 * nh + 4 * (int)rank + g;
+  const uint32_t full_leader = ptx::mapa(ptx::smem_u32(is_k ? &bars->kfull[u] : &bars->vfull[u]), 0);
+  const uint32_t read = ptx::smem_u32(is_k ? &bars->kempty[u] : &bars->vempty[u]);
+  uint8_t* row = smem + S::kKRing + un * kStageBytes + (g >> 1) * kChunkBytes + r0 * 128;
+  const bool flip = g >= 2;
+  const uint32_t gx = (uint32_t)((4 * (g & 1) + (flip ? 2 : 0)) ^ (r0 & 7)) << 4;
+  const uint8_t* codes = p.kv + 16 * q;
+  const __half* scales = p.kv_scales + q;
   Codes32 k[4];
-  auto load_fill = [&]() {
-    const long long at = (long long)(w.own + fr) * p.kv_heads + w.kvh;
+  auto load = [&](uint32_t i) -> bool {
+    TileRows w;
+    if (!map.get(c, i, &w)) return false;
+    const int base = own ? w.own : w.peer, valid = (own ? w.valid : w.valid >> 8) & 255;
+    const long long at = (long long)(base + r0) * p.kv_heads + w.kvh;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) load(k[e], at + (long long)(8 * e) * p.kv_heads, fr + 8 * e < (w.valid & 255), fq);
+    for (int e = 0; e < 4; ++e) {
+      k[e] = Codes32{make_uint4(0x88888888u, 0x88888888u, 0x88888888u, 0x88888888u), 0};
+      if (r0 + 8 * e < valid) {
+        const long long ae = at + (long long)(8 * e) * p.kv_heads;
+        k[e].w = __ldg(reinterpret_cast<const uint4*>(codes + ae * (kDim / 2)));
+        k[e].s = __ldg(reinterpret_cast<const unsigned short*>(scales + ae * 16));
+      }
+    }
+    return true;
   };
-  if (!map.get(c, 0, &w)) return;
-  load_fill();
+  if (!load(0)) return;
 #pragma unroll 1
   for (uint32_t gi = 0; gi < n; ++gi) {
-    const uint32_t b = gi & 1u, ph = (gi >> 1) & 1u;
-    Codes32 v[2];
-    {
-      const long long at = (long long)(w.peer + pr) * p.kv_heads + w.kvh;
+    if (gi >= 1 && !wait_warp(c, read, (gi - 1) & 1u, kErrVLoad)) return;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        load(v[e], at + (long long)(8 * e) * p.kv_heads, pr + 8 * e < ((w.valid >> 8) & 255), pq);
+    for (int e = 0; e < 4; ++e) {
+      const __half2 s2 = __half2half2(__ushort_as_half(k[e].s));
+      uint8_t* dst = row + 8 * e * 128;
+      const uint4 w = k[e].w;
+      *reinterpret_cast<uint4*>(dst + gx) = widen8(flip ? w.z : w.x, s2);
+      *reinterpret_cast<uint4*>(dst + (gx ^ 16u)) = widen8(flip ? w.w : w.y, s2);
+      *reinterpret_cast<uint4*>(dst + (gx ^ 32u)) = widen8(flip ? w.x : w.z, s2);
+      *reinterpret_cast<uint4*>(dst + (gx ^ 48u)) = widen8(flip ? w.y : w.w, s2);
     }
-    // ---- fill slot u
-    if (gi >= 2 && !wait_warp(c, freed + 32 * b, ph ^ 1u, kErrKLoad)) return;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) store(fill_row + b * 4 * kStageBytes + 8 * e * 128, k[e]);
     // the tensor core reads the slot through the async proxy
     ptx::fence_proxy_async_smem();
     __syncwarp();
-    if (lane == 0) ptx::mbar_arrive_cluster(kfull_leader + 32 * b);
-    if (gi + 1 < n) {
-      if (!map.get(c, gi + 1, &w)) return;
-      load_fill();
-    }
-    // ---- refill slot vs once QK^T has read it
-    if (!wait_warp(c, read + 32 * b, ph, kErrVLoad)) return;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) store(refill_row + b * 4 * kStageBytes + 8 * e * 128, v[e]);
-    ptx::fence_proxy_async_smem();
-    __syncwarp();
-    if (lane == 0) ptx::mbar_arrive_cluster(vfull_leader + 32 * b);
+    if (lane == 0) ptx::mbar_arrive_cluster(full_leader);
+    if (gi + 1 < n && !load(gi + 1)) return;
   }
 }
 
@@ -1066,7 +1067,7 @@ __device__ __forceinline__ bool kv4_qk_tile(const Ctx& c, uint32_t sbase, uint32
   constexpr uint32_t kIdesc = ptx::idesc_f16(0, 128, 128, 0);
   constexpr uint32_t kIdescRope = ptx::idesc_f16(Cfg<T>::kRopeFmt, 128, 128, 0);
   constexpr uint32_t kHi = ptx::sw128_desc_hi(1024);
-  const uint32_t ph = (gi >> 1) & 1u;
+  const uint32_t ph = (gi >> 1) & 1u;   // phase of what alternates by tile; the slots': B
   TileRows w;
   if (!map.get(c, gi, &w)) return false;
   if (w.valid & kFirst) {
@@ -1090,10 +1091,10 @@ __device__ __forceinline__ bool kv4_qk_tile(const Ctx& c, uint32_t sbase, uint32
   __syncwarp();
 #pragma unroll
   for (uint32_t u = 0; u < 4; ++u) {
-    if (!wait_warp(c, ptx::smem_u32(&bars->kfull[4 * B + u]), ph, kErrQK)) return false;
+    if (!wait_warp(c, ptx::smem_u32(&bars->kfull[u]), B, kErrQK)) return false;
     ptx::tc_fence_after();
     if (elect_one()) {
-      const uint32_t kb = ptx::sw128_desc_lo(sbase + S::kKRing + (4 * B + u) * kStageBytes, 16);
+      const uint32_t kb = ptx::sw128_desc_lo(sbase + S::kKRing + u * kStageBytes, 16);
       const uint32_t qa = ptx::sw128_desc_lo(sbase + S::kQ + 2 * (u & 1u) * kChunkBytes, 16);
 #pragma unroll
       for (int kk = 0; kk < 8; ++kk) {
@@ -1103,7 +1104,7 @@ __device__ __forceinline__ bool kv4_qk_tile(const Ctx& c, uint32_t sbase, uint32
         else
           ptx::mma_pair_f16(s_tmem, ptx::make_desc(qa + (kk >> 2) * 512 + (kk & 3) * 2, kHi), bd, kIdesc, 1u);
       }
-      ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->kempty[4 * B + u]), 0x3);
+      ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->kempty[u]), 0x3);
       if (u == 3) ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->s_full[B]), 0x3);
     }
     __syncwarp();
@@ -1129,17 +1130,16 @@ __device__ __forceinline__ bool kv4_pv_tile(const Ctx& c, uint32_t sbase, uint32
 #pragma unroll
   for (uint32_t u = 0; u < 4; ++u) {
     const uint32_t nh = u >> 1, th = u & 1u;
-    // one CTA's slot as QK^T had it (p_full is behind its fill), the other's refilled
-    if (!wait_warp(c, ptx::smem_u32(&bars->vfull[4 * B + u]), ph, kErrPV)) return false;
+    if (!wait_warp(c, ptx::smem_u32(&bars->vfull[u]), B, kErrPV)) return false;
     ptx::tc_fence_after();
     if (elect_one()) {
-      const uint32_t vb = ptx::sw128_desc_lo(sbase + S::kKRing + (4 * B + u) * kStageBytes, kChunkBytes);
+      const uint32_t vb = ptx::sw128_desc_lo(sbase + S::kKRing + (4 + u) * kStageBytes, kChunkBytes);
       const uint32_t pa = ptx::sw128_desc_lo(sbase + S::kP + B * S::kPBuf + th * kChunkBytes, 16);
 #pragma unroll
       for (int kk = 0; kk < 4; ++kk)
         ptx::mma_pair_f16(tmem + kColO + 128 * nh, ptx::make_desc(pa + kk * 2, kHi),
                           ptx::make_desc(vb + kk * 128, kHi), kIdesc, (first && th == 0 && kk == 0) ? 0u : 1u);
-      ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->vempty[4 * B + u]), 0x3);
+      ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->vempty[u]), 0x3);
       if (u == 3) ptx::mma_commit_pair_mc(ptx::smem_u32(&bars->o_done[B]), 0x3);
     }
     __syncwarp();
@@ -1620,34 +1620,37 @@ __device__ __forceinline__ void load_q_f16(const Params& p, int v, uint32_t rank
   auto conv = [](uint4 x) {
     return make_uint4(pair_to_h2<Out>(x.x), pair_to_h2<Out>(x.y), pair_to_h2<Out>(x.z), pair_to_h2<Out>(x.w));
   };
+  // sixteen 16-byte loads a round trip
 #pragma unroll 1
-  for (int cb = 0; cb < 4; ++cb) {   // 64 dims: 32 TMEM columns
-    uint4 x[8];
+  for (int cb = 0; cb < 2; ++cb) {   // 128 dims: 64 TMEM columns
+    uint4 x[16];
 #pragma unroll
-    for (int g = 0; g < 8; ++g) x[g] = real ? __ldg(qg + 8 * cb + g) : zero;
-    uint32_t w[32];
+    for (int g = 0; g < 16; ++g) x[g] = real ? __ldg(qg + 16 * cb + g) : zero;
 #pragma unroll
-    for (int g = 0; g < 8; ++g) {
-      const uint4 y = conv(x[g]);
-      w[4 * g] = y.x;
-      w[4 * g + 1] = y.y;
-      w[4 * g + 2] = y.z;
-      w[4 * g + 3] = y.w;
+    for (int h = 0; h < 2; ++h) {
+      uint32_t w[32];
+#pragma unroll
+      for (int g = 0; g < 8; ++g) {
+        const uint4 y = conv(x[8 * h + g]);
+        w[4 * g] = y.x;
+        w[4 * g + 1] = y.y;
+        w[4 * g + 2] = y.z;
+        w[4 * g + 3] = y.w;
+      }
+      ptx::tmem_st32(tmem + lane_off + kColQT + 64 * cb + 32 * h, w);
     }
-    ptx::tmem_st32(tmem + lane_off + kColQT + 32 * cb, w);
   }
-#pragma unroll 1
-  for (int bx = 2 * hf; bx < 2 * hf + 2; ++bx) {
-    uint4 x[8];
+  uint4 x[16], r[4];
 #pragma unroll
-    for (int g = 0; g < 8; ++g) x[g] = real ? __ldg(qg + 32 + 8 * bx + g) : zero;
+  for (int g = 0; g < 16; ++g) x[g] = real ? __ldg(qg + 32 + 16 * hf + g) : zero;
 #pragma unroll
-    for (int g = 0; g < 8; ++g)
-      *reinterpret_cast<uint4*>(qreg + bx * kChunkBytes + m * 128 + ((g ^ (m & 7)) << 4)) = conv(x[g]);
-  }
+  for (int g = 0; g < 4; ++g) r[g] = real ? __ldg(rg + 4 * hf + g) : zero;
 #pragma unroll
-  for (int g = 4 * hf; g < 4 * hf + 4; ++g)
-    *reinterpret_cast<uint4*>(qreg + 4 * kChunkBytes + m * 128 + ((g ^ (m & 7)) << 4)) = real ? __ldg(rg + g) : zero;
+  for (int g = 0; g < 16; ++g)
+    *reinterpret_cast<uint4*>(qreg + (2 * hf + (g >> 3)) * kChunkBytes + m * 128 + (((g & 7) ^ (m & 7)) << 4)) = conv(x[g]);
+#pragma unroll
+  for (int g = 0; g < 4; ++g)
+    *reinterpret_cast<uint4*>(qreg + 4 * kChunkBytes + m * 128 + (((4 * hf + g) ^ (m & 7)) << 4)) = r[g];
   ptx::tmem_wait_st();
 }
 
@@ -2275,7 +2278,7 @@ __device__ __forceinline__ void softmax_epilogue(const Params& p, const Ctx& c, 
 // producer, warp 3 P.V issuer, warps 4..7 softmax/epilogue, warp 8 Q loader
 // (warps 9..11 complete the third warpgroup).  For an FP8 cache the block has
 // 16 warps: warp 2 also prefetches Q, and warps 8..15 convert V to fp16.  For a
-// 4-bit cache warp 0 loads the rope rows, warp 2 finds the tiles' rows and warps 8..15
+// 4-bit cache warp 0 loads the rope rows, warp 2 finds the tiles' rows and warps 8..23
 // fill the slots of both GEMMs.  The
 // Cv variant has 16 warps too: warps 12..15 rewrite each landed V stage (tail
 // rows zeroed, bf16 -> fp16 with kF16); warps 9..11 are idle.  In the plain
@@ -2298,12 +2301,12 @@ mla_sm100_decode_kernel(const __grid_constant__ Params p) {
 
   if (threadIdx.x == 0) {
     // V operand stages: one expect-tx arrival (TMA), or FP8: kConvWarps converter warps x 2 CTAs
-    // (4-bit: a slot filled for QK^T by both CTAs' converters, refilled for P.V by one's)
-    const uint32_t n_vfull = Io<T>::kKv4   ? kRefillWarps
+    // (4-bit: two converter warps of each CTA)
+    const uint32_t n_vfull = Io<T>::kKv4   ? 4u
                              : Io<T>::kKv8 ? 2u * kConvWarps
                                            : (Io<T>::kConv ? 2u * kFixWarps : 1u);
     for (int s = 0; s < 8; ++s) {
-      ptx::mbar_init(ptx::smem_u32(&bars->kfull[s]), Io<T>::kKv4 ? 2u * kFillWarps : 1u);
+      ptx::mbar_init(ptx::smem_u32(&bars->kfull[s]), Io<T>::kKv4 ? 4u : 1u);
       ptx::mbar_init(ptx::smem_u32(&bars->kempty[s]), 1);
       ptx::mbar_init(ptx::smem_u32(&bars->vfull[s]), n_vfull);
       ptx::mbar_init(ptx::smem_u32(&bars->vempty[s]), 1);
@@ -2374,11 +2377,11 @@ mla_sm100_decode_kernel(const __grid_constant__ Params p) {
   // One role per warp: a lane blocked in mbarrier.try_wait holds back every
   // other lane of its warp.  Warpgroup 1 (warps 4..7) runs the softmax.
   if ((warp >> 2) == 1) {
-    ptx::setmaxnreg_inc<kRegsSoftmax>();
+    ptx::setmaxnreg_inc<regs_softmax<T>()>();
     softmax_epilogue<T>(p, c, rank, pair, smem, tmem, bars, warp & 3, lane);
-    ptx::setmaxnreg_dec<kRegsLow>();   // same budget as the other warps from here on
+    ptx::setmaxnreg_dec<regs_low<T>()>();   // same budget as the other warps from here on
   } else {
-    ptx::setmaxnreg_dec<kRegsLow>();
+    ptx::setmaxnreg_dec<regs_low<T>()>();
   if (warp == 0) {
     if (lane == 0) k_producer<T>(p, c, rank, pair, smem, sbase, bars);
   } else if (warp == 8 && !Io<T>::kKv8 && !Io<T>::kKv4) {
@@ -2419,7 +2422,7 @@ mla_sm100_decode_kernel(const __grid_constant__ Params p) {
       wait_bar(c, ptx::smem_u32(&bars->drain_pv), 0u, kErrDrain);
     }
   } else if (Io<T>::kKv4 && warp >= 8) {
-    // 4-bit: warps 8..15 widen the codes
+    // 4-bit: warps 8..23 widen the codes
     if constexpr (Io<T>::kKv4) kv4_converter<T>(p, c, rank, pair, smem, bars, warp - 8, lane);
   } else if (Io<T>::kKv8 && warp >= 8) {
     // FP8: warps 8..15 dequantize the V units
@@ -2838,36 +2841,46 @@ __global__ void __launch_bounds__(1024)
 mla_ragged_plan_kernel(const int* __restrict__ seqlens, int qb, int heads, int hgroups, int q_len, int kv_heads,
                        int max_len, uint32_t* __restrict__ cu, void* __restrict__ out, float* __restrict__ lse,
                        int out_elem_bytes) {
-  __shared__ uint32_t s_part[1024];
-  const int tid = threadIdx.x;
+  __shared__ uint32_t s_part[32];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int vb = qb * hgroups;
   auto tiles = [&](int v) -> uint32_t {
     const int len = qseq_len(seqlens, v / hgroups, q_len, kv_heads, max_len);
     return (uint32_t)((len + kTile - 1) / kTile);
   };
   const int per = (vb + 1023) / 1024;
-  const int v0 = tid * per, v1 = v0 + per < vb ? v0 + per : vb;
+  const int v0 = tid * per < vb ? tid * per : vb, v1 = v0 + per < vb ? v0 + per : vb;
   uint32_t sum = 0;
   for (int v = v0; v < v1; ++v) sum += tiles(v);
-  s_part[tid] = sum;
-  __syncthreads();
-  for (int off = 1; off < 1024; off <<= 1) {   // inclusive scan of the chunk sums
-    const uint32_t x = tid >= off ? s_part[tid - off] : 0u;
-    __syncthreads();
-    s_part[tid] += x;
-    __syncthreads();
+  uint32_t incl = sum;   // inclusive scan of the chunk sums
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t x = __shfl_up_sync(0xffffffffu, incl, off);
+    if (lane >= off) incl += x;
   }
-  uint32_t run = tid > 0 ? s_part[tid - 1] : 0u;
+  if (lane == 31) s_part[warp] = incl;
+  __syncthreads();
+  uint32_t before = s_part[lane];
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const uint32_t x = __shfl_up_sync(0xffffffffu, before, off);
+    if (lane >= off) before += x;
+  }
+  const uint32_t total = __shfl_sync(0xffffffffu, before, 31);
+  before = __shfl_sync(0xffffffffu, before, warp > 0 ? warp - 1 : 0);
+  uint32_t run = incl - sum + (warp > 0 ? before : 0u);
   for (int v = v0; v < v1; ++v) {
     cu[v] = run;
     run += tiles(v);
   }
-  if (tid == 1023) cu[vb] = s_part[1023];
-  for (int row = tid; row < qb * heads; row += 1024) {
-    if (qseq_len(seqlens, row / heads, q_len, kv_heads, max_len) > 0) continue;
-    uint4* o = reinterpret_cast<uint4*>(static_cast<uint8_t*>(out) + (size_t)row * kDim * out_elem_bytes);
-    for (int i = 0; i < kDim * out_elem_bytes / 16; ++i) o[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (lse != nullptr) lse[row] = -INFINITY;
+  if (tid == 1023) cu[vb] = total;
+  // query sequences without rows, a warp each
+  for (int qs = warp; qs < qb; qs += 32) {
+    if (qseq_len(seqlens, qs, q_len, kv_heads, max_len) > 0) continue;
+    uint4* o = reinterpret_cast<uint4*>(static_cast<uint8_t*>(out) + (size_t)qs * heads * kDim * out_elem_bytes);
+    for (int i = lane; i < heads * (kDim * out_elem_bytes / 16); i += 32) o[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (lse != nullptr)
+      for (int i = lane; i < heads; i += 32) lse[(size_t)qs * heads + i] = -INFINITY;
   }
 }
 
