@@ -12,8 +12,25 @@ namespace {
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 
 enum Int4Kernel { kSimt, kPair, kMma };
-// The warp-level kernel takes calls of up to this many query rows per KV head.
-constexpr int kMmaRows = 64;
+
+// Which of the two tensor-core kernels, by the time each is expected to take in us for
+// sequences of the maximal length (fits to measured calls, one B200; rows = query rows
+// per KV head):
+//   warp-level, 16 rows a CTA and two CTAs an SM: 16 + 4.0 per round of 64-row tiles;
+//   32 rows and one CTA: 16 + 3.1 per round (b128 s4096, 16 rows: 125, 32 rows: 194, pair
+//   kernel 240; b6 s3001, 3 positions x 40 heads: 47 against 99)
+//   pair kernel, 128 rows a pair: 45 + 2.9 per round of 128-row tiles, 25 more when
+//   ranges cross sequences (b64 s8192, 128 rows: 216 against 688; b1 s131072: 85 against 182)
+bool warp_level_is_faster(long long seqs, int q_len, int g, int max_len) {
+  const long long rows = (long long)q_len * g;
+  const int mt = rows <= 16 ? 1 : 2;
+  auto rounds = [](long long n, long long d) { return (double)((n + d - 1) / d); };
+  const double mma = 16. + (mt == 1 ? 4.0 : 3.1) * rounds(seqs * ((rows + 16 * mt - 1) / (16 * mt)) * ((max_len + 63) / 64),
+                                                          mt == 1 ? 296 : 148);
+  const long long vs = seqs * q_len * ((g + 127) / 128);
+  const double pair = 45. + 2.9 * rounds(vs * ((max_len + 127) / 128), 74) + (vs > 1 ? 25. : 0.);
+  return mma <= pair;
+}
 
 struct Int4Plan {
   Int4Kernel kernel;
@@ -52,7 +69,9 @@ int plan_call(const char* fn, int batch, int q_len, int heads, int kv_heads, int
     const bool covered = sm100_supports_ext(batch, q_len, heads, kv_heads, max_seqlen_kv);
     // block_H, query rows per CTA: up to 32 asks for the warp-level kernel, more for the pair kernel
     const int block_h = cfg != nullptr ? cfg->block_H : 0;
-    const bool mma = block_h > 0 ? block_h <= 32 : (rows <= kMmaRows || !covered);
+    const bool mma = block_h > 0 ? block_h <= 32
+                                 : !covered || warp_level_is_faster((long long)batch * kv_heads, q_len,
+                                                                    heads / kv_heads, max_seqlen_kv);
     if (mma) {
       p->kernel = kMma;
       p->mma = int4_mma_plan(batch, q_len, heads, kv_heads, max_seqlen_kv, (block_h > 0 ? block_h : rows) <= 16 ? 1 : 2,

@@ -2514,29 +2514,15 @@ __device__ __forceinline__ void store4_out(T* dst, float4 v) {
 constexpr int kCombineGroups = 4;
 constexpr int kCombinePer = 20;   // pieces per thread and round: 80 per round (B200: at most 74)
 
+// One row (head `head` of virtual sequence bb, split between the n pairs from pf), by a
+// whole CTA; s_lse and s_acc are its scratch.
 template <typename OutT>
-__global__ void __launch_bounds__(128 * kCombineGroups)
-mla_pair_combine_kernel(const float* __restrict__ part_lse, const float* __restrict__ part_o,
-                        OutT* __restrict__ out, float* __restrict__ lse_out, const uint32_t* cu,
-                        uint32_t total_fixed, int nt, int pairs, int vbatch, int heads, int hgroups,
-                        int fuse_max) {
+__device__ __forceinline__ void combine_row(const float* __restrict__ part_lse, const float* __restrict__ part_o,
+                                            OutT* __restrict__ out, float* __restrict__ lse_out, const TileMap& m,
+                                            int head, int bb, int pf, int n, int heads, int hgroups, float* s_lse,
+                                            float4 (*s_acc)[128]) {
   constexpr int G = kCombineGroups;
-  __shared__ float s_lse[kMaxPairs];
-  __shared__ float4 s_acc[G - 1][128];
-  const int head = blockIdx.x, bb = blockIdx.y;
   const int grp = threadIdx.x >> 7, tid = threadIdx.x & 127;   // piece group, column quad
-  ptx::grid_dep_wait();   // the decode kernel's partials are complete and visible
-  TileMap m;
-  m.cu = cu;
-  m.nt = (uint32_t)nt;
-  m.batch = vbatch;
-  m.total = cu != nullptr ? __ldg(cu + vbatch) : total_fixed;
-  m.pairs = effective_pairs((uint32_t)pairs, m.total);
-  if (m.first(bb) == m.first(bb + 1)) return;   // empty sequence (written by the plan kernel)
-  int pf, pl;
-  pairs_of_sequence(m, bb, &pf, &pl);
-  const int n = pl - pf + 1;
-  if (n <= fuse_max) return;   // whole, or merged by the decode kernel
   // piece k's slot (pair_slot without a division per piece): every pair after the
   // first starts its range inside the sequence, so the piece is that pair's first
   const size_t slot0 = pair_slot(m, pf, bb);
@@ -2587,7 +2573,7 @@ mla_pair_combine_kernel(const float* __restrict__ part_lse, const float* __restr
   }
   if (grp > 0) s_acc[grp - 1][tid] = acc;
   __syncthreads();
-  if (grp > 0) return;
+  if (grp > 0) return;   // (a caller that goes on to another row meets at a barrier first)
 #pragma unroll
   for (int g2 = 0; g2 < G - 1; ++g2) {
     const float4 o = s_acc[g2][tid];
@@ -2601,6 +2587,91 @@ mla_pair_combine_kernel(const float* __restrict__ part_lse, const float* __restr
   const size_t orow = (size_t)(bb / hgroups) * heads + hglob;
   store4_out(out + orow * kDim + 4 * tid, acc);
   if (lse_out != nullptr && tid == 0) lse_out[orow] = lse;
+}
+
+template <typename OutT>
+__global__ void __launch_bounds__(128 * kCombineGroups)
+mla_pair_combine_kernel(const float* __restrict__ part_lse, const float* __restrict__ part_o,
+                        OutT* __restrict__ out, float* __restrict__ lse_out, const uint32_t* cu, uint32_t total_fixed,
+                        int nt, int pairs, int vbatch, int heads, int hgroups, int fuse_max) {
+  __shared__ float s_lse[kMaxPairs];
+  __shared__ float4 s_acc[kCombineGroups - 1][128];
+  const int head = blockIdx.x, bb = blockIdx.y;
+  ptx::grid_dep_wait();   // the decode kernel's partials are complete and visible
+  TileMap m;
+  m.cu = cu;
+  m.nt = (uint32_t)nt;
+  m.batch = vbatch;
+  m.total = cu != nullptr ? __ldg(cu + vbatch) : total_fixed;
+  m.pairs = effective_pairs((uint32_t)pairs, m.total);
+  if (m.first(bb) == m.first(bb + 1)) return;   // empty sequence (written by the plan kernel)
+  int pf, pl;
+  pairs_of_sequence(m, bb, &pf, &pl);
+  const int n = pl - pf + 1;
+  if (n <= fuse_max) return;   // whole, or merged by the decode kernel
+  combine_row(part_lse, part_o, out, lse_out, m, head, bb, pf, n, heads, hgroups, s_lse, s_acc);
+}
+
+// The same for a ragged call of many sequences, whose host does not know which
+// sequences are split between many pairs: every CTA lists them (in order, so that all
+// CTAs hold the same list; each takes more than fuse_max pairs, so there are fewer than
+// kMaxPairs) and the CTAs share out the rows.  A grid of one CTA per head and sequence
+// spent 34 us on finding nothing to do at 64 sequences.
+template <typename OutT>
+__global__ void __launch_bounds__(128 * kCombineGroups)
+mla_ragged_combine_kernel(const float* __restrict__ part_lse, const float* __restrict__ part_o,
+                          OutT* __restrict__ out, float* __restrict__ lse_out, const uint32_t* cu, int pairs,
+                          int vbatch, int heads, int hgroups, int fuse_max) {
+  constexpr int kWarps = 4 * kCombineGroups;
+  __shared__ float s_lse[kMaxPairs];
+  __shared__ float4 s_acc[kCombineGroups - 1][128];
+  __shared__ int s_count[kWarps];
+  __shared__ int s_list[kMaxPairs];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  ptx::grid_dep_wait();
+  TileMap m;
+  m.cu = cu;
+  m.nt = 0;
+  m.batch = vbatch;
+  m.total = __ldg(cu + vbatch);
+  m.pairs = effective_pairs((uint32_t)pairs, m.total);
+  auto wide = [&](int v) -> bool {
+    if (v >= vbatch || m.first(v) == m.first(v + 1)) return false;
+    int pf, pl;
+    pairs_of_sequence(m, v, &pf, &pl);
+    return pl - pf + 1 > fuse_max;
+  };
+  // warp w looks at sequences [w per, (w + 1) per)
+  const int per = (vbatch + kWarps * 32 - 1) / (kWarps * 32) * 32;
+  int count = 0;
+  for (int k = 0; k < per; k += 32) count += __popc(__ballot_sync(0xffffffffu, wide(warp * per + k + lane)));
+  if (lane == 0) s_count[warp] = count;
+  __syncthreads();
+  int at = 0, total = 0;
+  for (int w = 0; w < kWarps; ++w) {
+    if (w < warp) at += s_count[w];
+    total += s_count[w];
+  }
+  if (count > 0) {
+    for (int k = 0; k < per; k += 32) {
+      const int v = warp * per + k + lane;
+      const bool is = wide(v);
+      const unsigned b = __ballot_sync(0xffffffffu, is);
+      const int i = at + __popc(b & ((1u << lane) - 1u));
+      if (is && i < kMaxPairs) s_list[i] = v;
+      at += __popc(b);
+    }
+  }
+  __syncthreads();
+  if (total > kMaxPairs) total = kMaxPairs;
+  for (int i = blockIdx.x; i < total * kHeads; i += gridDim.x) {
+    const int bb = s_list[i / kHeads], head = i % kHeads;
+    if ((bb % hgroups) * kHeads + head >= heads) continue;
+    int pf, pl;
+    pairs_of_sequence(m, bb, &pf, &pl);
+    combine_row(part_lse, part_o, out, lse_out, m, head, bb, pf, pl - pf + 1, heads, hgroups, s_lse, s_acc);
+    __syncthreads();   // the scratch is free for the next row
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -3296,8 +3367,9 @@ cudaError_t launch_sm100_combine(const DecodeArgs& a) {
   const int hg = qs.hg, vb = qs.vb;
   const uint32_t total = (uint32_t)vb * (uint32_t)nt;
   // a programmatic dependent of the decode kernel before it in the stream
+  const bool listed = a.cu_tiles != nullptr && vb > 8;   // (one sequence: 3 us less without the list)
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(kHeads, vb, 1);
+  cfg.gridDim = listed ? dim3(148 * 4, 1, 1) : dim3(kHeads, vb, 1);   // (four CTAs fit an SM)
   cfg.blockDim = dim3(128 * kCombineGroups, 1, 1);
   cfg.dynamicSmemBytes = 0;
   cfg.stream = a.stream;
@@ -3308,16 +3380,17 @@ cudaError_t launch_sm100_combine(const DecodeArgs& a) {
   cfg.numAttrs = 1;
   const float* pl = a.part_lse;
   const float* po = a.part_o;
-  const uint32_t* cu = a.cu_tiles;
   const int pairs = a.plan.bpc, g = qs.g, fm = kFuseMaxPieces;
-  if (a.out_dtype == MLA_DTYPE_F32)
-    return cudaLaunchKernelEx(&cfg, mla_pair_combine_kernel<float>, pl, po, static_cast<float*>(a.out), a.lse, cu,
-                              total, nt, pairs, vb, g, hg, fm);
-  if (a.dtype == MLA_DTYPE_BF16)
-    return cudaLaunchKernelEx(&cfg, mla_pair_combine_kernel<__nv_bfloat16>, pl, po,
-                              static_cast<__nv_bfloat16*>(a.out), a.lse, cu, total, nt, pairs, vb, g, hg, fm);
-  return cudaLaunchKernelEx(&cfg, mla_pair_combine_kernel<__half>, pl, po, static_cast<__half*>(a.out), a.lse, cu,
-                            total, nt, pairs, vb, g, hg, fm);
+  auto launch = [&](auto* out) {
+    using OutT = std::remove_reference_t<decltype(*out)>;
+    return listed ? cudaLaunchKernelEx(&cfg, mla_ragged_combine_kernel<OutT>, pl, po, out, a.lse,
+                                       (const uint32_t*)a.cu_tiles, pairs, vb, g, hg, fm)
+                  : cudaLaunchKernelEx(&cfg, mla_pair_combine_kernel<OutT>, pl, po, out, a.lse,
+                                       (const uint32_t*)a.cu_tiles, total, nt, pairs, vb, g, hg, fm);
+  };
+  if (a.out_dtype == MLA_DTYPE_F32) return launch(static_cast<float*>(a.out));
+  if (a.dtype == MLA_DTYPE_BF16) return launch(static_cast<__nv_bfloat16*>(a.out));
+  return launch(static_cast<__half*>(a.out));
 }
 
 cudaError_t launch_seqsplit_combine(const DecodeArgs& a, bool pieces, const PeerRows& x, void* out, float* lse,
