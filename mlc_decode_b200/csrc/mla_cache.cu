@@ -320,7 +320,7 @@ void launch_one(const CacheArgs& a, bool append, cudaStream_t s) {
 }
 
 int run(const char* fn, const CacheArgs& a, bool append, int form, int dtype, void* stream) {
-  if (a.tokens < 0 || a.rows < 1 || a.kv_heads < 1 || a.rows > INT32_MAX ||
+  if (a.tokens < 0 || a.rows < 1 || a.kv_heads < 1 || a.rows > INT32_MAX || a.tokens > (1ll << 31) ||
       a.tokens * a.kv_heads > (1ll << 33)) {
     set_error("%s: bad size (tokens %lld, cache rows %lld, kv_heads %d)", fn, a.tokens, a.rows, a.kv_heads);
     return MLA_ERR_ARG;
@@ -396,7 +396,7 @@ int32_t mla_cache_append(const void* kv, const void* k_pe, const int32_t* slots,
   a.kv_scale = kv_scale;
   uint32_t bits;
   memcpy(&bits, &kv_scale, sizeof(bits));
-  a.kv_recip = kv_scale > 1e-30f && kv_scale < 1e30f && (bits & 0x7fffffu) != 0x7fffffu ? 1.f / kv_scale : 0.f;
+  a.kv_recip = kv_scale > 1e-20f && kv_scale < 1e20f && (bits & 0x7fffffu) != 0x7fffffu ? 1.f / kv_scale : 0.f;
   a.positions = positions;
   a.turns = turns;
   a.gain = gain;

@@ -41,6 +41,7 @@
 namespace mla {
 namespace sm100 {   // (mla_sm100.cu)
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn();
+bool place_map(CUtensorMap* m, const CUtensorMap& form, const void* base);
 bool make_map_kv(CUtensorMap* m, const void* base, uint64_t cols, uint64_t kv_heads, uint64_t rows,
                  CUtensorMapDataType dt, uint32_t elem_bytes);
 }  // namespace sm100
@@ -683,25 +684,35 @@ cudaError_t device_facts(int* sms) {
   return cudaSuccess;
 }
 
-// The tensor maps of a call, or the ones the calling thread last made for the same key.
+// The tensor maps of a call: encoded for a shape (a thread keeps the last few shapes'),
+// then given the call's addresses.
 struct Maps {
   CUtensorMap codes, scales, kpe;
 };
 struct MapKey {
-  const void *codes, *scales, *kpe;
   long long rows;
   int kv_heads, dtype;
 };
 
-bool tensor_maps(const Int4Args& a, long long rows, Maps* m) {
-  MapKey key;
-  memset(&key, 0, sizeof(key));   // padding included: keys compare bytewise
-  key.codes = a.codes;
-  key.scales = a.scales;
-  key.kpe = a.k_pe;
-  key.rows = rows;
-  key.kv_heads = a.kv_heads;
-  key.dtype = a.dtype;
+bool encode_maps(const Int4Args& a, const MapKey& k, Maps* m) {
+  const CUtensorMapDataType dt =
+      k.dtype == MLA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  if (!sm100::make_map_kv(&m->codes, a.codes, kI4Bytes, k.kv_heads, k.rows, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1) ||
+      !sm100::make_map_kv(&m->kpe, a.k_pe, kPeDim, k.kv_heads, k.rows, dt, 2))
+    return false;
+  const auto fn = sm100::encode_fn();
+  if (fn == nullptr) return false;
+  const cuuint64_t dims[3] = {kI4Groups, (cuuint64_t)k.kv_heads, (cuuint64_t)k.rows};
+  const cuuint64_t strides[2] = {kI4Groups * 2, (cuuint64_t)k.kv_heads * kI4Groups * 2};
+  const cuuint32_t box[3] = {kI4Groups, 1, kTileR};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return fn(&m->scales, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(a.scales), dims, strides, box, estr,
+            CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+bool tensor_maps(const Int4Args& a, long long rows, MmaParams* p) {
+  const MapKey key{rows, a.kv_heads, a.dtype};
   struct Entry {
     MapKey key;
     Maps maps;
@@ -709,31 +720,20 @@ bool tensor_maps(const Int4Args& a, long long rows, Maps* m) {
   constexpr int kSlots = 8;
   thread_local Entry cache[kSlots];
   thread_local int filled = 0, next = 0;
-  for (int i = 0; i < filled; ++i)
-    if (memcmp(&cache[i].key, &key, sizeof(key)) == 0) {
-      *m = cache[i].maps;
-      return true;
-    }
-  const CUtensorMapDataType dt =
-      a.dtype == MLA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  if (!sm100::make_map_kv(&m->codes, a.codes, kI4Bytes, a.kv_heads, rows, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1) ||
-      !sm100::make_map_kv(&m->kpe, a.k_pe, kPeDim, a.kv_heads, rows, dt, 2))
-    return false;
-  const auto fn = sm100::encode_fn();
-  if (fn == nullptr) return false;
-  const cuuint64_t dims[3] = {kI4Groups, (cuuint64_t)a.kv_heads, (cuuint64_t)rows};
-  const cuuint64_t strides[2] = {kI4Groups * 2, (cuuint64_t)a.kv_heads * kI4Groups * 2};
-  const cuuint32_t box[3] = {kI4Groups, 1, kTileR};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  if (fn(&m->scales, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<__half*>(a.scales), dims, strides, box, estr,
-         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
-    return false;
-  cache[next].key = key;
-  cache[next].maps = *m;
-  next = (next + 1) % kSlots;
-  if (filled < kSlots) ++filled;
-  return true;
+  const Maps* m = nullptr;
+  for (int i = 0; i < filled && m == nullptr; ++i)
+    if (cache[i].key.rows == key.rows && cache[i].key.kv_heads == key.kv_heads && cache[i].key.dtype == key.dtype)
+      m = &cache[i].maps;
+  if (m == nullptr) {
+    Maps made;
+    if (!encode_maps(a, key, &made)) return false;
+    cache[next] = Entry{key, made};
+    m = &cache[next].maps;
+    next = (next + 1) % kSlots;
+    if (filled < kSlots) ++filled;
+  }
+  return sm100::place_map(&p->tm_codes, m->codes, a.codes) && sm100::place_map(&p->tm_scales, m->scales, a.scales) &&
+         sm100::place_map(&p->tm_kpe, m->kpe, a.k_pe);
 }
 
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
@@ -801,11 +801,7 @@ cudaError_t launch_int4_mma(Int4Args a, const Int4MmaPlan& plan, void* workspace
   p.groups = plan.groups;
   p.num_rows = a.block_table != nullptr ? a.num_pages * a.page_size : a.batch * a.max_seqlen;
   p.sl2 = a.softmax_scale * kLog2e;
-  Maps m;
-  if (!tensor_maps(a, p.num_rows, &m)) return cudaErrorInvalidValue;
-  p.tm_codes = m.codes;
-  p.tm_scales = m.scales;
-  p.tm_kpe = m.kpe;
+  if (!tensor_maps(a, p.num_rows, &p)) return cudaErrorInvalidValue;
   const bool bf = a.dtype == MLA_DTYPE_BF16;
   if (plan.row_tiles == 1)
     return bf ? launch_typed<__nv_bfloat16, 1>(p, plan.workers, stream) : launch_typed<__half, 1>(p, plan.workers, stream);

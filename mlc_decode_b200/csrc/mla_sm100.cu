@@ -2972,6 +2972,22 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
+// `form` (a map of the same shape) over the tensor at `base`, 16-byte aligned.
+bool place_map(CUtensorMap* m, const CUtensorMap& form, const void* base) {
+  static PFN_cuTensorMapReplaceAddress_v12000 fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    cudaDriverEntryPointQueryResult q{};
+    void* f = nullptr;
+    if (cudaGetDriverEntryPointByVersion("cuTensorMapReplaceAddress", &f, 12000, cudaEnableDefault, &q) ==
+            cudaSuccess &&
+        q == cudaDriverEntryPointSuccess)
+      fn = reinterpret_cast<PFN_cuTensorMapReplaceAddress_v12000>(f);
+  });
+  *m = form;
+  return fn != nullptr && fn(m, const_cast<void*>(base)) == CUDA_SUCCESS;
+}
+
 // 2D row-major [rows, cols] tensor, boxes of 64 rows x 128 bytes, 128-byte swizzle.
 bool make_map(CUtensorMap* m, const void* base, uint64_t cols, uint64_t rows, CUtensorMapDataType dt,
               uint32_t elem_bytes = 2) {
@@ -3216,12 +3232,10 @@ cudaError_t launch_form(const DecodeArgs& a, const sm100::Params& p) {
 
 namespace sm100 {
 
-// The six tensor maps of a call, encoded by the driver (cuTensorMapEncodeTiled, a
-// few microseconds of host time for all of them) or taken from a small per-thread
-// cache of the last calls' maps: a decode loop calls again and again with the same
-// tensors, and a map depends only on the key below.
+// The six tensor maps of a call.  Encoding them (cuTensorMapEncodeTiled) takes a few
+// microseconds of host time, so a thread keeps the maps of the last few shapes it met and
+// puts the call's addresses into copies of them.
 struct MapKey {
-  const void *q, *q_pe, *kv, *k_pe, *out, *part_o;
   long long part_rows, kv_rows;
   int g, qb, kv_heads, dtype, out_f32, form;   // form: 0 model type, 1 e4m3, 2 4-bit
   bool operator==(const MapKey& o) const { return memcmp(this, &o, sizeof(MapKey)) == 0; }
@@ -3231,65 +3245,54 @@ struct MapEntry {
   CUtensorMap kv, kpe, q, qpe, out, part;
 };
 
+// (4-bit: the latent codes are read without a tensor map, and so is Q)
+bool encode_maps(const DecodeArgs& a, const MapKey& k, MapEntry* e) {
+  const CUtensorMapDataType dt =
+      a.dtype == MLA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  const uint64_t rows = (uint64_t)k.kv_rows;
+  if (k.form == 1 && !make_map_kv(&e->kv, a.kv, kDim, k.kv_heads, rows, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1)) return false;
+  if (k.form == 0 && !make_map_kv(&e->kv, a.kv, kDim, k.kv_heads, rows, dt)) return false;
+  if (!make_map_kv(&e->kpe, a.k_pe, kPeDim, k.kv_heads, rows, dt)) return false;
+  if (k.form != 2 &&
+      (!make_map3(&e->q, a.q, kDim, k.g, k.qb, dt) || !make_map3(&e->qpe, a.q_pe, kPeDim, k.g, k.qb, dt)))
+    return false;
+  if (!(k.out_f32 ? make_map3(&e->out, a.out, kDim, k.g, k.qb, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4)
+                  : make_map3(&e->out, a.out, kDim, k.g, k.qb, dt)))
+    return false;
+  return a.part_o == nullptr ||
+         make_map(&e->part, a.part_o, kDim, (uint64_t)k.part_rows, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4);
+}
+
 bool tensor_maps(const DecodeArgs& a, const QShape& qs, Params* p) {
   MapKey key;
   memset(&key, 0, sizeof(key));   // padding included: keys compare bytewise
-  key.q = a.q;
-  key.q_pe = a.q_pe;
-  key.kv = a.kv;
-  key.k_pe = a.k_pe;
-  key.out = a.out;
-  key.part_o = a.part_o;
-  key.part_rows = a.part_o != nullptr ? a.plan.part_rows : 0;
+  key.part_rows = a.part_o != nullptr ? a.plan.part_rows : -1;
   key.kv_rows = a.block_table != nullptr ? (long long)a.num_pages * a.page_size : (long long)a.batch * a.seqlen_kv;
   key.g = qs.g;
   key.qb = qs.qb;
   key.kv_heads = qs.kv_heads;
   key.dtype = a.dtype;
   key.out_f32 = p->out_f32;
-  key.form = a.kv_scales != nullptr ? 2 : a.kv_fp8;
+  key.form = a.kv_scales != nullptr ? 2 : a.kv_fp8 ? 1 : 0;
   constexpr int kSlots = 8;
   thread_local MapEntry cache[kSlots];
   thread_local int filled = 0, next = 0;
-  for (int i = 0; i < filled; ++i) {
-    if (cache[i].key == key) {
-      p->tm_kv = cache[i].kv;
-      p->tm_kpe = cache[i].kpe;
-      p->tm_q = cache[i].q;
-      p->tm_qpe = cache[i].qpe;
-      p->tm_out = cache[i].out;
-      p->tm_part = cache[i].part;
-      return true;
-    }
+  const MapEntry* e = nullptr;
+  for (int i = 0; i < filled && e == nullptr; ++i)
+    if (cache[i].key == key) e = &cache[i];
+  if (e == nullptr) {
+    MapEntry made{};
+    made.key = key;
+    if (!encode_maps(a, key, &made)) return false;
+    cache[next] = made;
+    e = &cache[next];
+    next = (next + 1) % kSlots;
+    if (filled < kSlots) ++filled;
   }
-  const CUtensorMapDataType dt =
-      a.dtype == MLA_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-  const uint64_t kv_rows = (uint64_t)key.kv_rows;
-  // (4-bit: the latent codes are read without a tensor map, and so is Q)
-  const bool ok_kv = key.form == 2 ? true : a.kv_fp8 ? make_map_kv(&p->tm_kv, a.kv, kDim, qs.kv_heads, kv_rows,
-                                            CU_TENSOR_MAP_DATA_TYPE_UINT8, 1)
-                               : make_map_kv(&p->tm_kv, a.kv, kDim, qs.kv_heads, kv_rows, dt);
-  if (!ok_kv || !make_map_kv(&p->tm_kpe, a.k_pe, kPeDim, qs.kv_heads, kv_rows, dt)) return false;
-  if (key.form != 2 && (!make_map3(&p->tm_q, a.q, kDim, qs.g, qs.qb, dt) ||
-                        !make_map3(&p->tm_qpe, a.q_pe, kPeDim, qs.g, qs.qb, dt)))
-    return false;
-  if (!(p->out_f32 ? make_map3(&p->tm_out, a.out, kDim, qs.g, qs.qb, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4)
-                   : make_map3(&p->tm_out, a.out, kDim, qs.g, qs.qb, dt)))
-    return false;
-  if (a.part_o != nullptr &&
-      !make_map(&p->tm_part, a.part_o, kDim, (uint64_t)a.plan.part_rows, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4))
-    return false;
-  MapEntry& e = cache[next];
-  e.key = key;
-  e.kv = p->tm_kv;
-  e.kpe = p->tm_kpe;
-  e.q = p->tm_q;
-  e.qpe = p->tm_qpe;
-  e.out = p->tm_out;
-  e.part = p->tm_part;
-  next = (next + 1) % kSlots;
-  if (filled < kSlots) ++filled;
-  return true;
+  return (key.form == 2 || (place_map(&p->tm_kv, e->kv, a.kv) && place_map(&p->tm_q, e->q, a.q) &&
+                            place_map(&p->tm_qpe, e->qpe, a.q_pe))) &&
+         place_map(&p->tm_kpe, e->kpe, a.k_pe) && place_map(&p->tm_out, e->out, a.out) &&
+         (a.part_o == nullptr || place_map(&p->tm_part, e->part, a.part_o));
 }
 
 }  // namespace sm100
