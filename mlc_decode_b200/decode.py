@@ -56,6 +56,13 @@ def _on_device(device, call, *args):
             call(*args, torch._C._cuda_getCurrentRawStream(device.index))
 
 
+def _not_capturing(what):
+    """A buffer made inside a graph capture holds its first values only once the graph has
+    run: an eager call before that would read whatever the memory held."""
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError(f"{what} of this object is made by its first call on a device: make that call before the capture")
+
+
 class MlaDecodeKernel:
     """Absorbed-MLA decode for one (batch, heads, kv_heads, kv_ctx, dim, pe_dim).
 
@@ -476,8 +483,9 @@ class MlaPagedDecodeKernel:
         ``kv_codes`` uint8 [..., kv_heads, 256] and ``kv_scales`` float16 [..., kv_heads, 16]
         (leading dims as ``__call__``'s kv_cache) hold the rows as ``cache_append`` writes
         them: 16 groups of 32 dims, each dim (code - 8) x its group's scale.  q, q_pe,
-        k_pe_cache and out keep the model's type; bfloat16 queries must lie within fp16's
-        range (the scores are fp16 products with fp32 sums).
+        k_pe_cache and out keep the model's type; bfloat16 queries and the rows' values must
+        lie within fp16's range (the scores are fp16 products with fp32 sums).  The first call
+        on a device makes the workspace and precedes any graph capture.
         """
         b, h, smax, ql, kvh = self.batch, self.heads, self.max_seqlen_kv, self.q_len, self.kv_heads
         dtype = q.dtype if isinstance(q, torch.Tensor) else None
@@ -524,6 +532,7 @@ class MlaPagedDecodeKernel:
             with self._lock:
                 ws = self._ws.get(key)
                 if ws is None:
+                    _not_capturing("the 4-bit workspace")
                     with torch.cuda.device(device):   # (the plan counts the device's SMs)
                         n = capi.int4kv_workspace_bytes(self.batch, self.q_len, self.heads, self.kv_heads,
                                                         self.max_seqlen_kv, _DTYPES[dtype], self._ccfg)
@@ -543,7 +552,8 @@ class MlaPagedDecodeKernel:
         ``extend_block_tables``) are updated in place; a request whose table row or free list
         is full keeps its length.  With ``rotary`` q_pe (into this object's scratch, q_pe
         itself stays) and k_pe turn to their rows' positions.  Like the workspace, the scratch
-        is this object's: calls of one object are serialised by the caller.
+        is this object's: calls of one object are serialised by the caller, and the first call
+        on a device precedes any graph capture.
         """
         from . import paged
 
@@ -590,7 +600,12 @@ class MlaPagedDecodeKernel:
         scale = self._ccfg.softmax_scale
         if not (scale >= 0 and math.isfinite(scale)):
             raise ValueError(f"softmax_scale must be finite and > 0, got {scale}")
-        self._int4_workspace(dev, dtype) if kv_scales is not None else self._workspace(dev, dtype)
+        if kv_scales is not None:
+            self._int4_workspace(dev, dtype)
+        else:
+            if (dev.index, dtype) not in self._ws:
+                _not_capturing("the workspace")
+            self._workspace(dev, dtype)
         slots, positions, all_new, turned = self._step_scratch(dev, dtype)
         paged.extend_block_tables(block_table, cache_seqlens, all_new if new_lens is None else new_lens, free_pages,
                                   free_pos, cache_seqlens, free_pos, slots, positions,
@@ -614,6 +629,7 @@ class MlaPagedDecodeKernel:
             with self._lock:
                 s = self._ws.get(key)
                 if s is None:
+                    _not_capturing("the step's scratch")
                     n = self.batch * self.q_len
                     s = self._ws[key] = (torch.empty(n, dtype=torch.int32, device=device),
                                          torch.empty(n, dtype=torch.int32, device=device),

@@ -15,7 +15,7 @@ import threading
 import torch
 
 from . import capi
-from .decode import _DTYPES, _FP8, DIM, PE_DIM, _check_tensor, _fits, _on_device
+from .decode import _DTYPES, _FP8, DIM, PE_DIM, _check_tensor, _fits, _not_capturing, _on_device
 
 INT4_GROUP = 32                      # dims per scale of the 4-bit form
 INT4_GROUPS = DIM // INT4_GROUP      # scales per row
@@ -119,7 +119,7 @@ class Rotary:
     [tokens]; dims [offset, offset + rot_dim) turn, the others are copied; out may be x.
     ``interleaved``: pairs are dims (2 i, 2 i + 1), else (i, i + rot_dim / 2).  ``scaling``: see
     ``rotary_frequencies``.  The frequencies are uploaded by the first call on a device (make
-    it, or ``rot.turns(device)``, before a graph capture).
+    it, or ``rot.turns(device)``, before a graph capture: a capture refuses).
     """
 
     def __init__(self, rot_dim=PE_DIM, base=10000.0, interleaved=True, scaling=None):
@@ -148,6 +148,7 @@ class Rotary:
             with self._lock:
                 t = self._dev.get(device)
                 if t is None:
+                    _not_capturing("the frequencies' copy")
                     t = self._dev[device] = torch.tensor(self._turns, dtype=torch.float64, device=device)
         return t
 

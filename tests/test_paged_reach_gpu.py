@@ -8,7 +8,7 @@ import torch
 from mlc_decode_b200 import MlaPagedDecodeKernel, Rotary, cache_append, cache_gather, extend_block_tables
 from oracle import mla_oracle as O
 from oracle import paged_oracle as P
-from tests.test_int4_gpu import KERNELS, _caches, _check, _inputs
+from test_int4_gpu import KERNELS, _caches, _check, _inputs
 
 pytestmark = pytest.mark.gpu
 
@@ -207,3 +207,39 @@ def test_prompt_rows_in_a_graph(batch, per):
         turned = torch.empty_like(pe)
         rot(pe, positions, turned)
         assert torch.equal(back_pe[has], turned[has])
+
+
+def _step_args(b, h, int4):
+    dt = torch.bfloat16
+    z = lambda *shape, dtype=dt: torch.zeros(*shape, dtype=dtype, device="cuda")   # noqa: E731
+    args = dict(q=z(b, h, 512), q_pe=z(b, h, 64), kv=z(b, 1, 512), k_pe=z(b, 1, 64), k_pe_cache=z(4, 64, 1, 64),
+                block_table=z(b, 2, dtype=torch.int32) - 1, cache_seqlens=z(b, dtype=torch.int32),
+                free_pages=torch.arange(4, dtype=torch.int32, device="cuda"), free_pos=z(1, dtype=torch.int32),
+                out=z(b, h, 512))
+    if int4:
+        return dict(args, kv_cache=z(4, 64, 1, 256, dtype=torch.uint8), kv_scales=z(4, 64, 1, 16, dtype=torch.half))
+    return dict(args, kv_cache=z(4, 64, 1, 512))
+
+
+@pytest.mark.parametrize("int4", [False, True])
+def test_first_call_inside_a_capture_is_refused(int4):
+    """The workspace, the step's scratch and a rotary's frequencies are made (and given their
+    first values) by an eager call; a capture that would make them is refused."""
+    args = _step_args(2, 16, int4)
+    k, rot = MlaPagedDecodeKernel(2, 16, 128), Rotary(64)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        args["out"].zero_()
+        with pytest.raises(RuntimeError, match="before the capture"):
+            k.step(**args)
+        with pytest.raises(RuntimeError, match="before the capture"):
+            rot(args["q_pe"], args["cache_seqlens"], args["q_pe"])
+    graph.replay()
+    assert args["cache_seqlens"].tolist() == [0, 0]
+    k.step(**args, rotary=rot)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        k.step(**args, rotary=rot)
+    graph.replay()
+    assert args["cache_seqlens"].tolist() == [2, 2]
