@@ -616,7 +616,7 @@ int paged_layout(const char* fn, int batch, int q_len, int heads, int kv_heads, 
   const size_t rows = (size_t)L->plan.part_rows;
   L->counters_off = kStatusBytes;
   L->cu_off = L->counters_off + counter_bytes(qb, g);
-  L->lse_off = L->cu_off + align_up((vb + 1) * sizeof(uint32_t), 256);
+  L->lse_off = L->cu_off + align_up((vb + 2) * sizeof(uint32_t), 256);
   L->o_off = L->lse_off + align_up(rows * sizeof(float), 256);
   L->total = L->o_off + rows * kDim * sizeof(float);
   return MLA_OK;

@@ -17,19 +17,22 @@ enum Int4Kernel { kSimt, kPair, kMma };
 // sequences of the maximal length (fits to measured calls, one B200; rows = query rows
 // per KV head):
 //   warp-level, 16 rows a CTA and two CTAs an SM: 16 + 4.0 per round of 64-row tiles;
-//   32 rows and one CTA: 16 + 3.1 per round (b128 s4096, 16 rows: 125, 32 rows: 194, pair
-//   kernel 240; b6 s3001, 3 positions x 40 heads: 47 against 99)
-//   pair kernel, 128 rows a pair: 45 + 2.9 per round of 128-row tiles, 25 more when
-//   ranges cross sequences (b64 s8192, 128 rows: 216 against 688; b1 s131072: 85 against 182)
+//   32 rows and one CTA: 16 + 3.1 per round;
+//   pair kernel, 128 rows a pair: 30 + 2.9 per round of 128-row tiles, and 15 or 45 to merge
+//   sequences cut in many or few pieces, unless each has a pair of its own.
+// Measured, warp-level : pair, L2 flushed: b128 s4096, 16 rows 130 : 219, 32 rows 200 : 221, 64
+// rows 370 : 223; b64 s8192, 128 rows 693 : 207; b1 s131072, 128 rows 185 : 82, 16 rows
+// 54 : 82; b6 s3001, 3 positions x 40 heads 50 : 76; b1 s300, 16 rows 17 : 43.
 bool warp_level_is_faster(long long seqs, int q_len, int g, int max_len) {
   const long long rows = (long long)q_len * g;
   const int mt = rows <= 16 ? 1 : 2;
   auto rounds = [](long long n, long long d) { return (double)((n + d - 1) / d); };
   const double mma = 16. + (mt == 1 ? 4.0 : 3.1) * rounds(seqs * ((rows + 16 * mt - 1) / (16 * mt)) * ((max_len + 63) / 64),
                                                           mt == 1 ? 296 : 148);
-  const long long vs = seqs * q_len * ((g + 127) / 128);
-  const double pair = 45. + 2.9 * rounds(vs * ((max_len + 127) / 128), 74) + (vs > 1 ? 25. : 0.);
-  return mma <= pair;
+  const long long vs = seqs * q_len * ((g + 127) / 128), nt = (max_len + 127) / 128;
+  const double ranges = rounds(vs * nt, 74), split = 30. + 2.9 * ranges + (nt <= 3 * ranges ? 45. : 15.);
+  const double whole = 30. + 2.9 * nt;
+  return mma <= (vs <= 74 && whole < split ? whole : split);
 }
 
 struct Int4Plan {

@@ -411,12 +411,16 @@ struct TileMap {
   const uint32_t* cu;
   uint32_t nt, total, pairs;
   int batch;
+  bool whole = false;   // ragged: pair v takes virtual sequence v (the plan kernel's choice)
   __device__ __forceinline__ uint32_t first(int v) const {
     return cu != nullptr ? __ldg(cu + v) : (uint32_t)v * nt;
   }
-  __device__ __forceinline__ uint32_t range_start(int pp) const { return (uint32_t)pp * total / pairs; }
+  __device__ __forceinline__ uint32_t range_start(int pp) const {
+    return whole ? first(pp) : (uint32_t)pp * total / pairs;
+  }
   // pair whose range holds tile x
   __device__ __forceinline__ int pair_of(uint32_t x) const {
+    if (whole) return seq_of(x);
     return (int)(((x + 1) * pairs + total - 1) / total) - 1;
   }
   // sequence holding tile x (x < total): the last v with first(v) <= x
@@ -438,14 +442,18 @@ __device__ __forceinline__ uint32_t effective_pairs(uint32_t launched, uint32_t 
   return pp > 0 ? pp : 1u;
 }
 
-__device__ __forceinline__ TileMap tile_map(const Params& p) {
+__device__ __forceinline__ TileMap tile_map(const uint32_t* cu, int nt, uint32_t total, int batch, int pairs) {
   TileMap m;
-  m.cu = p.cu_tiles;
-  m.nt = (uint32_t)p.nt;
-  m.batch = p.batch;
-  m.total = p.cu_tiles != nullptr ? __ldg(p.cu_tiles + p.batch) : p.total_tiles;
-  m.pairs = effective_pairs((uint32_t)p.pairs, m.total);
+  m.cu = cu;
+  m.nt = (uint32_t)nt;
+  m.batch = batch;
+  m.total = cu != nullptr ? __ldg(cu + batch) : total;
+  m.whole = cu != nullptr && __ldg(cu + batch + 1) != 0u;
+  m.pairs = m.whole ? (uint32_t)batch : effective_pairs((uint32_t)pairs, m.total);
   return m;
+}
+__device__ __forceinline__ TileMap tile_map(const Params& p) {
+  return tile_map(p.cu_tiles, p.nt, p.total_tiles, p.batch, p.pairs);
 }
 
 // Iterates the pieces of pair `pair`'s tile range; empty sequences are skipped.
@@ -460,7 +468,7 @@ struct PieceIter {
     } else {
       t = t1 = m.total;   // a pair past the ones that own tiles
     }
-    v = t < t1 ? m.seq_of(t) : 0;
+    v = t < t1 ? (m.whole ? pair : m.seq_of(t)) : 0;
   }
   __device__ bool any() const { return t < t1; }   // (a ragged call may give a pair no tiles)
   __device__ bool next(Piece* pc) {
@@ -2361,6 +2369,8 @@ mla_sm100_decode_kernel(const __grid_constant__ Params p) {
   ptx::cluster_sync();
   ptx::tc_fence_after();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(tmem_slot);
+  // (a ragged call: set up while the plan kernel was running, whose results are read from here on)
+  if (p.cu_tiles != nullptr) ptx::grid_dep_wait();
   // a combine launch queued behind this grid may be set up now (it waits for this
   // grid's completion before it reads anything)
   if (threadIdx.x == 0) ptx::grid_dep_launch();
@@ -2598,12 +2608,7 @@ mla_pair_combine_kernel(const float* __restrict__ part_lse, const float* __restr
   __shared__ float4 s_acc[kCombineGroups - 1][128];
   const int head = blockIdx.x, bb = blockIdx.y;
   ptx::grid_dep_wait();   // the decode kernel's partials are complete and visible
-  TileMap m;
-  m.cu = cu;
-  m.nt = (uint32_t)nt;
-  m.batch = vbatch;
-  m.total = cu != nullptr ? __ldg(cu + vbatch) : total_fixed;
-  m.pairs = effective_pairs((uint32_t)pairs, m.total);
+  const TileMap m = tile_map(cu, nt, total_fixed, vbatch, pairs);
   if (m.first(bb) == m.first(bb + 1)) return;   // empty sequence (written by the plan kernel)
   int pf, pl;
   pairs_of_sequence(m, bb, &pf, &pl);
@@ -2629,12 +2634,8 @@ mla_ragged_combine_kernel(const float* __restrict__ part_lse, const float* __res
   __shared__ int s_list[kMaxPairs];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   ptx::grid_dep_wait();
-  TileMap m;
-  m.cu = cu;
-  m.nt = 0;
-  m.batch = vbatch;
-  m.total = __ldg(cu + vbatch);
-  m.pairs = effective_pairs((uint32_t)pairs, m.total);
+  const TileMap m = tile_map(cu, 0, 0u, vbatch, pairs);
+  if (m.whole) return;
   auto wide = [&](int v) -> bool {
     if (v >= vbatch || m.first(v) == m.first(v + 1)) return false;
     int pf, pl;
@@ -2727,12 +2728,7 @@ mla_seqsplit_combine_kernel(const float* __restrict__ part_lse, const float* __r
   const int grp = threadIdx.x >> 7, tid = threadIdx.x & 127, lane = threadIdx.x & 31;
   const bool pieces = fuse_max >= 0;
   ptx::grid_dep_wait();   // the decode kernel's pieces / rows are complete and visible
-  TileMap m;
-  m.cu = cu;
-  m.nt = (uint32_t)nt;
-  m.batch = vbatch;
-  m.total = !pieces ? 0u : (cu != nullptr ? __ldg(cu + vbatch) : total_fixed);
-  m.pairs = effective_pairs((uint32_t)pairs, m.total);
+  const TileMap m = pieces ? tile_map(cu, nt, total_fixed, vbatch, pairs) : tile_map(nullptr, nt, 0u, vbatch, pairs);
   const int rows = vbatch * kHeads;
   const size_t bh = (size_t)(vbatch / hgroups) * heads;   // output rows
   float* own = x.bufs[x.rank] + ((size_t)x.par * x.world + x.rank) * x.chunk;
@@ -2902,17 +2898,33 @@ mla_seqsplit_combine_kernel(const float* __restrict__ part_lse, const float* __r
 }
 
 // ---------------------------------------------------------------------------
+// Whether a ragged call over `vb` sequences of `total` tiles, the longest of `longest`, gives
+// every sequence a pair of its own rather than equal ranges of the tile list.  It saves the
+// pieces' stores and their merges, which cost as much as 18 tiles when sequences are cut
+// in two or three (merged by the pair that ends last) and 6 when they are cut in more
+// (merged by the combine launch): 4-bit, 128 heads, whole against ranges in us, 64 sequences
+// of 64 tiles 199 : 234, 64 of 128 366 : 388, 40 of 16 54 : 93, 20 of 8 38 : 87, 1 of 3
+// 28 : 42; 3 of 8 38 : 35, 1 of 12 44 : 29.
+__device__ __forceinline__ bool whole_sequences(int vb, uint32_t total, uint32_t longest, int pairs) {
+  if (vb > pairs) return false;
+  const uint32_t range = total / effective_pairs((uint32_t)pairs, total);
+  return longest <= range + (longest <= 3u * range ? 18u : 6u);
+}
+
 // Plan of a ragged call (per-sequence KV lengths), one CTA: cu[v] = first tile of
 // virtual sequence v (qb x head groups + 1 entries, qb query sequences of `heads`
-// rows) over the lengths qseq_len gives (seqlens nullptr: max_len for all); query
-// sequences with no KV rows get out = 0 and lse = -inf here (the decode kernel
+// rows) over the lengths qseq_len gives (seqlens nullptr: max_len for all); cu[vb + 1] =
+// 1 when every sequence goes to a pair of its own (whole_sequences; `whole_pairs` pairs in
+// all, 0: never).  Query sequences with no KV rows get out = 0 and lse = -inf here (the decode kernel
 // never visits them).
 // ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(1024)
 mla_ragged_plan_kernel(const int* __restrict__ seqlens, int qb, int heads, int hgroups, int q_len, int kv_heads,
                        int max_len, uint32_t* __restrict__ cu, void* __restrict__ out, float* __restrict__ lse,
-                       int out_elem_bytes) {
-  __shared__ uint32_t s_part[32];
+                       int out_elem_bytes, int whole_pairs) {
+  __shared__ uint32_t s_part[32], s_max;
+  ptx::grid_dep_launch();   // the decode launch behind may be set up (it waits for this grid)
+  if (threadIdx.x == 0) s_max = 0u;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int vb = qb * hgroups;
   auto tiles = [&](int v) -> uint32_t {
@@ -2921,8 +2933,12 @@ mla_ragged_plan_kernel(const int* __restrict__ seqlens, int qb, int heads, int h
   };
   const int per = (vb + 1023) / 1024;
   const int v0 = tid * per < vb ? tid * per : vb, v1 = v0 + per < vb ? v0 + per : vb;
-  uint32_t sum = 0;
-  for (int v = v0; v < v1; ++v) sum += tiles(v);
+  uint32_t sum = 0, longest = 0;
+  for (int v = v0; v < v1; ++v) {
+    const uint32_t n = tiles(v);
+    sum += n;
+    longest = n > longest ? n : longest;
+  }
   uint32_t incl = sum;   // inclusive scan of the chunk sums
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -2931,6 +2947,8 @@ mla_ragged_plan_kernel(const int* __restrict__ seqlens, int qb, int heads, int h
   }
   if (lane == 31) s_part[warp] = incl;
   __syncthreads();
+  longest = __reduce_max_sync(0xffffffffu, longest);
+  if (lane == 0 && longest > 0u) atomicMax(&s_max, longest);
   uint32_t before = s_part[lane];
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -2945,6 +2963,9 @@ mla_ragged_plan_kernel(const int* __restrict__ seqlens, int qb, int heads, int h
     run += tiles(v);
   }
   if (tid == 1023) cu[vb] = total;
+  __syncthreads();
+  if (tid == 0)
+    cu[vb + 1] = whole_sequences(vb, total, s_max, whole_pairs);
   // query sequences without rows, a warp each
   for (int qs = warp; qs < qb; qs += 32) {
     if (qseq_len(seqlens, qs, q_len, kv_heads, max_len) > 0) continue;
@@ -3195,7 +3216,7 @@ bool sm100_coop_available() {
 template <typename K>
 cudaError_t launch_variant(const sm100::Params& p, int pairs, cudaStream_t stream) {
   using namespace sm100;
-  if (!p.coop) {
+  if (!p.coop && p.cu_tiles == nullptr) {
     mla_sm100_decode_kernel<K><<<2 * pairs, threads_of<K>(), Smem<K>::kBytes, stream>>>(p);
     return cudaGetLastError();
   }
@@ -3205,8 +3226,13 @@ cudaError_t launch_variant(const sm100::Params& p, int pairs, cudaStream_t strea
   cfg.dynamicSmemBytes = Smem<K>::kBytes;
   cfg.stream = stream;
   cudaLaunchAttribute attr{};
-  attr.id = cudaLaunchAttributeCooperative;
-  attr.val.cooperative = 1;
+  if (p.coop) {
+    attr.id = cudaLaunchAttributeCooperative;
+    attr.val.cooperative = 1;
+  } else {   // a programmatic dependent of the plan kernel
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+  }
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   return cudaLaunchKernelEx(&cfg, mla_sm100_decode_kernel<K>, p);
@@ -3467,7 +3493,8 @@ cudaError_t launch_sm100_ragged_plan(const DecodeArgs& a) {
   if (a.block_table != nullptr && (long long)a.max_pages * a.page_size < cap) cap = a.max_pages * a.page_size;
   const QShape qs = qshape(a);
   sm100::mla_ragged_plan_kernel<<<1, 1024, 0, a.stream>>>(a.seqlens, qs.qb, qs.g, qs.hg, qs.q_len, qs.kv_heads,
-                                                          cap, a.cu_tiles, a.out, a.lse, elem);
+                                                          cap, a.cu_tiles, a.out, a.lse, elem,
+                                                          a.kv_scales != nullptr ? a.plan.bpc : 0);
   return cudaGetLastError();
 }
 
