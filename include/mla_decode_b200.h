@@ -360,8 +360,9 @@ int32_t mla_decode_ext_fp8kv(const void* q, const void* q_pe, const void* kv_fp8
  * query positions, KV heads, cfg) as in mla_decode_ext.  Rows past a sequence's length
  * are not read; a row on a page outside [0, num_pages) reads as zeros.
  * The tensor-core kernels take the products in float16 with float32 sums: a row's value
- * (n - 8) s, a softmax weight and a bfloat16 query are rounded to float16 once each, and
- * queries and values must lie within its range (the CUDA-core kernel, cfg kernel
+ * (n - 8) s (the warp-level kernel's scores take n - 8 itself), a softmax weight and a
+ * bfloat16 query are rounded to float16 once each, and queries and values must lie within
+ * its range (the CUDA-core kernel, cfg kernel
  * MLA_KERNEL_SIMT, computes in float32).  cfg block_H, query rows per CTA, chooses
  * between them: up to 16 or 32 the warp-level kernel, more the CTA-pair kernel, 0 the
  * faster one for the shape.

@@ -13,7 +13,11 @@
 // * The fragments of mma.m16n8k16 are widened straight from the stage's codes: no
 //   fp16 copy of the tile exists.  For S a thread's code word (8 dims of one row) is its
 //   B fragment of two k-steps, with the dims of Q's A fragment (kept in registers)
-//   permuted to match.  For P.V the words of two rows are interleaved by 16-bit halves,
+//   permuted to match.  The two k-steps are one scale group: their MMAs take the bare
+//   codes n - 8 and a float32 product with the scale follows, so the scores have no
+//   rounding of the row values (values rounded to fp16 first: 130 us instead of 133 at
+//   b128 h16 s4096, and an error of 2e-4 in the log-sum-exp of short sequences).  For P.V the
+//   values are rounded to fp16 once, as the weights are, and the words of two rows are interleaved by 16-bit halves,
 //   so that a field pair is one dim of two neighbouring rows; column n of block e is dim
 //   8 n + e of the warp's 64, which leaves each thread with 16 neighbouring output dims.
 // * Eight warps: for S two row halves x four quarters of the dims (the quarters' sums
@@ -23,9 +27,10 @@
 //   sequence cut by a range's end leaves float32 partials that the combine launch merges.
 //   Every CTA sums the lengths itself: no plan launch.
 //
-// Bound: at 16 rows the issue slots of the widening (13 instructions per 8 codes, once
-// for S and once for P.V) and mma.sync's 1,024 products a cycle and SM; above, the
-// latter.  Bytes would allow 6 TB/s.
+// Bound: the issue slots of the widening (13 instructions per 8 codes, once for S and
+// once for P.V) with the latencies that 16 warps an SM leave uncovered (issue slots 55 %,
+// integer pipe 45 %, tensor pipe 30 % busy at b128 h16 s4096: 121 us, 1.8 TB/s).
+// S of the next tile beside P.V of this one between the same two barriers: no faster.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 #include <math.h>
@@ -154,16 +159,22 @@ __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ uint32_t h2u(__half2 h) { return *reinterpret_cast<uint32_t*>(&h); }
 __device__ __forceinline__ __half2 u2h(uint32_t w) { return *reinterpret_cast<__half2*>(&w); }
 
-// Field pairs 0..3 of a word whose nibbles j and j + 4 are the pair's two codes, times
-// s2: 1024 + n and 64 + n are exact in fp16, so are the differences n - 8; the product
-// rounds once.
-__device__ __forceinline__ void widen4(uint32_t w, __half2 s2, uint32_t (&o)[4]) {
+// Field pairs 0..3 of a word whose nibbles j and j + 4 are the pair's two codes, as
+// n - 8: 1024 + n and 64 + n are exact in fp16, so are the differences.
+__device__ __forceinline__ void codes4(uint32_t w, uint32_t (&o)[4]) {
   const uint32_t v = w >> 8;
   const __half2 c0 = u2h(0x64086408u), c1 = u2h(0x54805480u);   // 1032, 72
-  o[0] = h2u(__hmul2(__hsub2(u2h((w & 0x000f000fu) | 0x64006400u), c0), s2));
-  o[1] = h2u(__hmul2(__hsub2(u2h((w & 0x00f000f0u) | 0x54005400u), c1), s2));
-  o[2] = h2u(__hmul2(__hsub2(u2h((v & 0x000f000fu) | 0x64006400u), c0), s2));
-  o[3] = h2u(__hmul2(__hsub2(u2h((v & 0x00f000f0u) | 0x54005400u), c1), s2));
+  o[0] = h2u(__hsub2(u2h((w & 0x000f000fu) | 0x64006400u), c0));
+  o[1] = h2u(__hsub2(u2h((w & 0x00f000f0u) | 0x54005400u), c1));
+  o[2] = h2u(__hsub2(u2h((v & 0x000f000fu) | 0x64006400u), c0));
+  o[3] = h2u(__hsub2(u2h((v & 0x00f000f0u) | 0x54005400u), c1));
+}
+
+// The same times s2 (one rounding).
+__device__ __forceinline__ void widen4(uint32_t w, __half2 s2, uint32_t (&o)[4]) {
+  codes4(w, o);
+#pragma unroll
+  for (int k = 0; k < 4; ++k) o[k] = h2u(__hmul2(u2h(o[k]), s2));
 }
 
 template <typename T>
@@ -383,7 +394,9 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
         // ---- S, this warp's rows [32 tq, +32) and dims [128 dq, +128) (and 16 rope dims)
 #pragma unroll
         for (int nb = 0; nb < 4; ++nb) {
-          const uint2 sc = *reinterpret_cast<const uint2*>(scales + (32 * tq + 8 * nb + qr) * 32 + dq * 8);
+          // the scales of this thread's two columns (rows of the tile), four groups each
+          const uint2 sc0 = *reinterpret_cast<const uint2*>(scales + (32 * tq + 8 * nb + 2 * t) * 32 + dq * 8);
+          const uint2 sc1 = *reinterpret_cast<const uint2*>(scales + (32 * tq + 8 * nb + 2 * t + 1) * 32 + dq * 8);
           float c[MT][4];
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt) c[mt][0] = c[mt][1] = c[mt][2] = c[mt][3] = 0.f;
@@ -394,13 +407,20 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
 #pragma unroll
           for (int jj = 0; jj < 4; ++jj) {
             const uint32_t w = *reinterpret_cast<const uint32_t*>(smem + ((stage + k_off) ^ (16u * jj)) + 1024 * nb);
-            const uint32_t s16 = jj < 2 ? sc.x : sc.y;
+            const __half2 a0 = u2h(jj < 2 ? sc0.x : sc0.y), a1 = u2h(jj < 2 ? sc1.x : sc1.y);
+            const float s0 = (jj & 1) ? __high2float(a0) : __low2float(a0);
+            const float s1 = (jj & 1) ? __high2float(a1) : __low2float(a1);
             uint32_t f[4];
-            widen4(w, u2h(__byte_perm(s16, 0, (jj & 1) ? 0x3232 : 0x1010)), f);
+            codes4(w, f);
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-              mma16816<__half>(c[mt], qf[mt][2 * jj], f[0], f[1]);
-              mma16816<__half>(c[mt], qf[mt][2 * jj + 1], f[2], f[3]);
+              float x[4] = {0.f, 0.f, 0.f, 0.f};
+              mma16816<__half>(x, qf[mt][2 * jj], f[0], f[1]);
+              mma16816<__half>(x, qf[mt][2 * jj + 1], f[2], f[3]);
+              c[mt][0] = fmaf(x[0], s0, c[mt][0]);
+              c[mt][1] = fmaf(x[1], s1, c[mt][1]);
+              c[mt][2] = fmaf(x[2], s0, c[mt][2]);
+              c[mt][3] = fmaf(x[3], s1, c[mt][3]);
             }
           }
 #pragma unroll

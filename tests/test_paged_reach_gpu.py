@@ -243,3 +243,26 @@ def test_first_call_inside_a_capture_is_refused(int4):
         k.step(**args, rotary=rot)
     graph.replay()
     assert args["cache_seqlens"].tolist() == [2, 2]
+
+
+@pytest.mark.parametrize("kernel", ["simt", "mma16", "mma32"])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_scores_of_short_sequences_are_exact_products(kernel, dtype):
+    """Sequences of a few rows, where one score is the log-sum-exp: codes times scales are not
+    rounded in the scores.  What is left: float32 sums of 576 products (off by at most 2^-23
+    of the magnitudes' sum each, 2^-13 of it together at the very worst; a random walk of
+    their roundings stays below 2^-20 of it), a float32 exponential and logarithm (1e-6)."""
+    b, h, lens = 6, 16, [1, 2, 3, 5, 1, 8]
+    q, qp, n, s, kp = _inputs(b, 1, h, 1, 8, dtype, seed=31)
+    codes, scales, pe, _ = _caches(n, s, kp, lens, 0, seed=1)
+    k = MlaPagedDecodeKernel(b, h, 8, cfg=KERNELS[kernel])
+    qq, qpp = q.cuda().squeeze(1), qp.cuda().squeeze(1)
+    out, lse = torch.empty_like(qq), torch.empty(b, h, device="cuda")
+    k.decode_int4(qq, qpp, codes, scales, pe, torch.tensor(lens, dtype=torch.int32, device="cuda"), out, lse)
+    for i, m in enumerate(lens):
+        v = P.dequantise_int4(n[i], s[i])[:m, 0]
+        qd, qpd, kd = (t.double().numpy() for t in (q[i, 0], qp[i, 0], kp[i, :m, 0]))
+        _, ref, _, _ = P.decode(qd, qpd, v, kd, SCALE)
+        sums = (np.abs(qd) @ np.abs(v).T + np.abs(qpd) @ np.abs(kd).T).max(-1) * SCALE
+        err = np.abs(lse[i].double().cpu().numpy() - ref)
+        assert (err <= 2.0 ** -20 * sums + 1e-6 * (1 + np.abs(ref))).all(), (i, err.max())
