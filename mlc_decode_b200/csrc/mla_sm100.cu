@@ -31,6 +31,8 @@
 //    the output, the hi/lo pair keeps it near fp32 accuracy.  O is rescaled
 //    only when a row max grows by more than 2^8 (exact: the final
 //    normalisation uses the same stale max), so the accumulator stays in TMEM.
+//  * A 4-bit latent cache (Kv4) has no K or V TMA: sixteen converter warps widen codes
+//    from registers into eight operand slots, one tile of both GEMMs.
 //  * Work: pair p takes the flattened tile range [p*T/P, (p+1)*T/P) over all
 //    sequences (T = batch x tiles per sequence).  A range that covers a whole
 //    sequence writes `out` directly; partial ranges write float32 partials to
@@ -162,9 +164,10 @@ struct Cv {};
 // registers: 16-byte global loads a tile ahead, no staging in shared memory.  Two
 // warps own one operand slot of 16 KB: four K units (this CTA's 64 rows x 128 dims) and four
 // V units (128 of this CTA's dims of 64 rows), and refill it as soon as its GEMM has
-// read it.  (Slots shared by both GEMMs, a value widened 1.5 times instead of twice, were
-// held from QK^T's fill to P.V's end: 5.1 us a tile pass with room for two, 279 us at
-// b64 h128 s8192.)  Q's latent dims are fp16, the rope dims run in T.
+// read it: 2.6 us a tile pass, bound by the chain of hand-offs (the tensor pipe is busy a
+// third of it, the issue slots 38 %).  (Slots shared by both GEMMs, a value widened 1.5 times instead of twice, were
+// held from QK^T's fill to P.V's end: 5.1 us a tile pass with room for two.  Eight
+// softmax warps of half a row's columns: 10 % more a call.)  Q's latent dims are fp16, the rope dims run in T.
 template <typename T>
 struct Kv4 {};
 template <typename K>
