@@ -49,11 +49,12 @@ def _fits(t, shape, dtype, index):
 def _on_device(device, call, *args):
     """``call(*args, stream)`` with ``device`` current, on its current stream (the raw handle:
     a Stream object costs a microsecond)."""
-    if torch.cuda.current_device() == device.index:
-        call(*args, torch._C._cuda_getCurrentRawStream(device.index))
+    index = device.index
+    if torch._C._cuda_getDevice() == index:
+        call(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
         with torch.cuda.device(device):
-            call(*args, torch._C._cuda_getCurrentRawStream(device.index))
+            call(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
 def _not_capturing(what):
@@ -506,16 +507,31 @@ class MlaPagedDecodeKernel:
             table_ptr = block_table.data_ptr()
             lead = (num_pages, page_size, kvh)
         index = dev.index
-        for name, t, shape, want in (("q", q, (*qshape, DIM), dtype), ("q_pe", q_pe, (*qshape, PE_DIM), dtype),
-                                     ("out", out, (*qshape, DIM), dtype),
-                                     ("kv_codes", kv_codes, (*lead, DIM // 2), torch.uint8),
-                                     ("kv_scales", kv_scales, (*lead, DIM // 32), torch.float16),
-                                     ("k_pe_cache", k_pe_cache, (*lead, PE_DIM), dtype),
-                                     ("lse", lse, qshape, torch.float32),
-                                     ("cache_seqlens", cache_seqlens, (b,), torch.int32),
-                                     ("block_table", block_table, (b, max_pages), torch.int32)):
-            if not _fits(t, shape, want, index) and not (t is None and name in ("lse", "cache_seqlens", "block_table")):
-                _check_tensor(name, t, shape, want, dev)
+        rows = (*qshape, DIM)
+        # all at once; one by one, with names, only if something is wrong
+        if not (type(q) is type(q_pe) is type(out) is type(kv_codes) is type(kv_scales) is type(k_pe_cache)
+                is torch.Tensor and q_pe.dtype is out.dtype is k_pe_cache.dtype is dtype
+                and kv_codes.dtype is torch.uint8 and kv_scales.dtype is torch.float16
+                and q.shape == out.shape == rows and q_pe.shape == (*qshape, PE_DIM)
+                and kv_codes.shape == (*lead, DIM // 2) and kv_scales.shape == (*lead, DIM // 32)
+                and k_pe_cache.shape == (*lead, PE_DIM)
+                and q.get_device() == q_pe.get_device() == out.get_device() == kv_codes.get_device()
+                == kv_scales.get_device() == k_pe_cache.get_device() == index
+                and q.is_contiguous() and q_pe.is_contiguous() and out.is_contiguous() and kv_codes.is_contiguous()
+                and kv_scales.is_contiguous() and k_pe_cache.is_contiguous()
+                and (lse is None or _fits(lse, qshape, torch.float32, index))
+                and (cache_seqlens is None or _fits(cache_seqlens, (b,), torch.int32, index))
+                and (block_table is None or _fits(block_table, (b, max_pages), torch.int32, index))):
+            for name, t, shape, want in (("q", q, rows, dtype), ("q_pe", q_pe, (*qshape, PE_DIM), dtype),
+                                         ("out", out, rows, dtype),
+                                         ("kv_codes", kv_codes, (*lead, DIM // 2), torch.uint8),
+                                         ("kv_scales", kv_scales, (*lead, DIM // 32), torch.float16),
+                                         ("k_pe_cache", k_pe_cache, (*lead, PE_DIM), dtype),
+                                         ("lse", lse, qshape, torch.float32),
+                                         ("cache_seqlens", cache_seqlens, (b,), torch.int32),
+                                         ("block_table", block_table, (b, max_pages), torch.int32)):
+                if t is not None or name not in ("lse", "cache_seqlens", "block_table"):
+                    _check_tensor(name, t, shape, want, dev)
         ws = self._ws.get((index, dtype, "int4"))
         if ws is None:
             ws = self._int4_workspace(dev, dtype)

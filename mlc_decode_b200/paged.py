@@ -42,16 +42,31 @@ def extend_block_tables(block_table, cache_seqlens, new_lens, free_pages, free_p
         raise ValueError("block_table must be an int32 tensor [batch, max_pages]")
     b, max_pages = block_table.shape
     dev = block_table.device
-    i32 = torch.int32
-    _check_tensor("block_table", block_table, (b, max_pages), i32, None)
-    n, nf = (t.numel() if isinstance(t, torch.Tensor) else -1 for t in (slots, free_pages))
-    index = dev.index
-    for name, t, k in (("cache_seqlens", cache_seqlens, b), ("new_lens", new_lens, b), ("free_pages", free_pages, nf),
-                       ("free_pos", free_pos, 1), ("new_seqlens", new_seqlens, b), ("new_free_pos", new_free_pos, 1),
-                       ("slots", slots, n), ("positions", positions, n), ("cu_new", cu_new, b + 1)):
-        if not (type(t) is torch.Tensor and t.dtype is i32 and t.get_device() == index and t.numel() == k
-                and t.dim() == 1 and t.is_contiguous()) and not (t is None and name == "cu_new"):
-            _check_tensor(name, t, (k,), i32, dev)
+    i32, index = torch.int32, dev.index
+    # all at once; one by one, with names, only if something is wrong
+    if not (type(cache_seqlens) is type(new_lens) is type(free_pages) is type(free_pos) is type(new_seqlens)
+            is type(new_free_pos) is type(slots) is type(positions) is torch.Tensor and dev.type == "cuda"
+            and block_table.dtype is cache_seqlens.dtype is new_lens.dtype is free_pages.dtype is free_pos.dtype
+            is new_seqlens.dtype is new_free_pos.dtype is slots.dtype is positions.dtype is i32
+            and cache_seqlens.shape == new_lens.shape == new_seqlens.shape == (b,)
+            and free_pos.shape == new_free_pos.shape == (1,) and slots.shape == positions.shape
+            and slots.dim() == free_pages.dim() == 1
+            and cache_seqlens.get_device() == new_lens.get_device() == free_pages.get_device()
+            == free_pos.get_device() == new_seqlens.get_device() == new_free_pos.get_device() == slots.get_device()
+            == positions.get_device() == index
+            and block_table.is_contiguous() and cache_seqlens.is_contiguous() and new_lens.is_contiguous()
+            and free_pages.is_contiguous() and free_pos.is_contiguous() and new_seqlens.is_contiguous()
+            and new_free_pos.is_contiguous() and slots.is_contiguous() and positions.is_contiguous()
+            and (cu_new is None or _fits(cu_new, (b + 1,), i32, index))):
+        _check_tensor("block_table", block_table, (b, max_pages), i32, None)
+        n, nf = (t.numel() if isinstance(t, torch.Tensor) else -1 for t in (slots, free_pages))
+        for name, t, k in (("cache_seqlens", cache_seqlens, b), ("new_lens", new_lens, b),
+                           ("free_pages", free_pages, nf), ("free_pos", free_pos, 1),
+                           ("new_seqlens", new_seqlens, b), ("new_free_pos", new_free_pos, 1), ("slots", slots, n),
+                           ("positions", positions, n), ("cu_new", cu_new, b + 1)):
+            if t is not None or name != "cu_new":
+                _check_tensor(name, t, (k,), i32, dev)
+    n, nf = slots.numel(), free_pages.numel()
     nbytes = capi.block_tables_workspace_bytes(b, n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
     _on_device(dev, capi.extend_block_tables, block_table.data_ptr(), cache_seqlens.data_ptr(), new_lens.data_ptr(),
@@ -158,20 +173,29 @@ class Rotary:
         n, h, d = shape = x.shape
         if not 0 <= int(offset) <= d - self.rot_dim:
             raise ValueError(f"dims [{offset}, {offset} + {self.rot_dim}) must lie inside the head's {d}")
-        dev = x.device
-        if not _fits(x, shape, x.dtype, dev.index) or dev.type != "cuda":
-            _check_rows("x", x, shape, x.dtype, None)
-        if not _fits(out, shape, x.dtype, dev.index):
-            _check_rows("out", out, shape, x.dtype, dev, written=True)
-        if not _fits(positions, (n,), torch.int32, dev.index):
+        dev, dtype = x.device, x.dtype
+        index = dev.index
+        dense = _fits(x, shape, dtype, index)
+        if not dense:
+            _check_rows("x", x, shape, dtype, None)
+        if not _fits(out, shape, dtype, index):
+            dense = False
+            _check_rows("out", out, shape, dtype, dev, written=True)
+        if not _fits(positions, (n,), torch.int32, index):
             _check_tensor("positions", positions, (n,), torch.int32, dev)
         if n == 0:
             return
-        xp, op, xs, os_ = x.data_ptr(), out.data_ptr(), x.stride(), out.stride()
-        if xs != os_ if xp == op else _ranges_meet(x, out):
+        xp, op = x.data_ptr(), out.data_ptr()
+        if dense:     # the same strides; apart if the starts are a whole tensor apart
+            xs = os_ = (h * d, d)
+            meet = xp != op and abs(xp - op) < n * h * d * dtype.itemsize
+        else:
+            xs, os_ = x.stride(), out.stride()
+            meet = xs != os_ if xp == op else _ranges_meet(x, out)
+        if meet:
             raise ValueError("out must be x itself or must not overlap it")
         _on_device(dev, capi.rotary, xp, op, positions.data_ptr(), self.turns(dev).data_ptr(), self.gain, n, h, d,
-                   self.rot_dim, int(offset), self.interleaved, xs[0], xs[1], os_[0], os_[1], _ROTARY_DTYPES[x.dtype])
+                   self.rot_dim, int(offset), self.interleaved, xs[0], xs[1], os_[0], os_[1], _ROTARY_DTYPES[dtype])
 
 
 def _ranges_meet(a, b):
@@ -259,6 +283,54 @@ def _check_dense(kv, k_pe, slots, written):
     return n, h, dtype
 
 
+def _quick_rows(kv, k_pe, slots, kv_cache, k_pe_cache, kv_scale, kv_scales):
+    """(tokens, KV heads, cache rows, form, type, strides) of arguments that are all dense and as
+    they should be, in one go; None for any others, which the checks above then take up (a
+    third of the time of a call of 64 rows went into them)."""
+    if not (type(kv) is type(k_pe) is type(slots) is type(kv_cache) is type(k_pe_cache) is torch.Tensor):
+        return None
+    dtype, index, lead, shape = kv.dtype, kv.get_device(), kv_cache.shape, kv.shape
+    if dtype not in _DTYPES or index < 0 or len(lead) != 4 or len(shape) != 3:
+        return None
+    n, h, width = shape
+    pages, page, kvh, held = lead
+    if kv_scales is not None:
+        if not (kv_scale is None and held == INT4_BYTES and kv_cache.dtype is torch.uint8
+                and _fits(kv_scales, (pages, page, kvh, INT4_GROUPS), torch.float16, index)):
+            return None
+        form = capi.MLA_CACHE_INT4
+    elif held != DIM:
+        return None
+    elif kv_scale is not None:
+        if kv_cache.dtype is not _FP8 and kv_cache.dtype is not torch.uint8:
+            return None
+        form = capi.MLA_CACHE_FP8
+    elif kv_cache.dtype is dtype:
+        form = capi.MLA_CACHE_MODEL
+    else:
+        return None
+    if (width == DIM and h == kvh and k_pe.dtype is dtype and k_pe_cache.dtype is dtype and slots.dtype is torch.int32
+            and k_pe.shape == (n, h, PE_DIM) and slots.shape == (n,) and k_pe_cache.shape == (pages, page, kvh, PE_DIM)
+            and kv.is_contiguous() and k_pe.is_contiguous() and slots.is_contiguous() and kv_cache.is_contiguous()
+            and k_pe_cache.is_contiguous() and k_pe.get_device() == index and slots.get_device() == index
+            and kv_cache.get_device() == index and k_pe_cache.get_device() == index
+            and (kv.data_ptr() | k_pe.data_ptr()) & 15 == 0):
+        return n, h, pages * page, form, dtype, (h * DIM, DIM, h * PE_DIM, PE_DIM)
+    return None
+
+
+def _rows(kv, k_pe, slots, kv_cache, k_pe_cache, kv_scale, kv_scales, written):
+    """What ``_quick_rows`` returns, of any arguments; raises for wrong ones."""
+    got = _quick_rows(kv, k_pe, slots, kv_cache, k_pe_cache, kv_scale, kv_scales)
+    if got is None:
+        n, h, dtype = _check_dense(kv, k_pe, slots, written)
+        form, rows, kvh = _check_cache(kv_cache, k_pe_cache, kv_scale, kv_scales, dtype, kv.device)
+        if kvh != h:
+            raise ValueError(f"kv has {h} KV heads, the cache {kvh}")
+        got = n, h, rows, form, dtype, (*_strides(kv), *_strides(k_pe))
+    return got
+
+
 def cache_append(kv, k_pe, slots, kv_cache, k_pe_cache, kv_scale=None, kv_scales=None, rotary=None, positions=None):
     """Write rows kv [tokens, kv_heads, 512] and k_pe [tokens, kv_heads, 64] to cache rows
     ``slots`` (int32 [tokens]; outside the cache, e.g. -1: skipped; slots are distinct).
@@ -269,11 +341,8 @@ def cache_append(kv, k_pe, slots, kv_cache, k_pe_cache, kv_scale=None, kv_scales
     ``rotary`` (a ``Rotary`` of 64 dims) and ``positions`` (int32 [tokens]) k_pe turns on the
     way.  kv and k_pe may be strided (rows on 16-byte boundaries).
     """
-    n, h, dtype = _check_dense(kv, k_pe, slots, False)
+    n, h, rows, form, dtype, strides = _rows(kv, k_pe, slots, kv_cache, k_pe_cache, kv_scale, kv_scales, False)
     dev = kv.device
-    form, rows, kvh = _check_cache(kv_cache, k_pe_cache, kv_scale, kv_scales, dtype, dev)
-    if kvh != h:
-        raise ValueError(f"kv has {h} KV heads, the cache {kvh}")
     if (rotary is None) != (positions is None):
         raise ValueError("rotary and positions go together")
     turns, gain, inter = None, 1.0, False
@@ -286,7 +355,7 @@ def cache_append(kv, k_pe, slots, kv_cache, k_pe_cache, kv_scale=None, kv_scales
     _on_device(dev, capi.cache_append, kv.data_ptr(), k_pe.data_ptr(), slots.data_ptr(), kv_cache.data_ptr(),
                None if kv_scales is None else kv_scales.data_ptr(), k_pe_cache.data_ptr(),
                1.0 if kv_scale is None else float(kv_scale), None if rotary is None else positions.data_ptr(), turns, gain,
-               inter, n, h, rows, *_strides(kv), *_strides(k_pe), form, _DTYPES[dtype])
+               inter, n, h, rows, *strides, form, _DTYPES[dtype])
 
 
 def cache_gather(slots, kv_cache, k_pe_cache, kv, k_pe, kv_scale=None, kv_scales=None):
@@ -294,12 +363,8 @@ def cache_gather(slots, kv_cache, k_pe_cache, kv, k_pe, kv_scale=None, kv_scales
     kv_heads, 64]: what the cache stands for, in the model's type (zeros for a slot outside
     the cache).  The cache and its forms as in ``cache_append``.
     """
-    n, h, dtype = _check_dense(kv, k_pe, slots, True)
-    dev = kv.device
-    form, rows, kvh = _check_cache(kv_cache, k_pe_cache, kv_scale, kv_scales, dtype, dev)
-    if kvh != h:
-        raise ValueError(f"kv has {h} KV heads, the cache {kvh}")
-    _on_device(dev, capi.cache_gather, slots.data_ptr(), kv_cache.data_ptr(),
+    n, h, rows, form, dtype, strides = _rows(kv, k_pe, slots, kv_cache, k_pe_cache, kv_scale, kv_scales, True)
+    _on_device(kv.device, capi.cache_gather, slots.data_ptr(), kv_cache.data_ptr(),
                None if kv_scales is None else kv_scales.data_ptr(), k_pe_cache.data_ptr(),
-               1.0 if kv_scale is None else float(kv_scale), kv.data_ptr(), k_pe.data_ptr(), n, h, rows, *_strides(kv),
-               *_strides(k_pe), form, _DTYPES[dtype])
+               1.0 if kv_scale is None else float(kv_scale), kv.data_ptr(), k_pe.data_ptr(), n, h, rows, *strides,
+               form, _DTYPES[dtype])
