@@ -266,3 +266,27 @@ def test_scores_of_short_sequences_are_exact_products(kernel, dtype):
         sums = (np.abs(qd) @ np.abs(v).T + np.abs(qpd) @ np.abs(kd).T).max(-1) * SCALE
         err = np.abs(lse[i].double().cpu().numpy() - ref)
         assert (err <= 2.0 ** -20 * sums + 1e-6 * (1 + np.abs(ref))).all(), (i, err.max())
+
+
+@pytest.mark.parametrize("kernel", ["mma16", "mma32"])
+@pytest.mark.parametrize("b, h, q_len, smax", [(1, 16, 1, 300), (1, 1, 1, 512), (5, 40, 2, 512), (3, 100, 1, 513),
+                                               (40, 16, 1, 500), (2, 48, 3, 129)])
+def test_short_sequences_cut_over_ctas(kernel, b, h, q_len, smax):
+    """Sequences of a few tiles, cut over CTAs and merged: call after call with other lengths,
+    the same values each time."""
+    q, qp, n, s, kp = _inputs(b, q_len, h, 1, smax, "fp16", seed=b + h)
+    k = MlaPagedDecodeKernel(b, h, smax, cfg=KERNELS[kernel], q_len=q_len)
+    qq, qpp = (t.cuda().squeeze(1) if q_len == 1 else t.cuda() for t in (q, qp))
+    out, lse = torch.empty_like(qq), torch.empty(qq.shape[:-1], device="cuda")
+    rng = np.random.default_rng(smax)
+    for it in range(4):
+        lens = [smax] * b if it == 0 else rng.integers(0, smax + 1, b).tolist()
+        codes, scales, pe, table = _caches(n, s, kp, lens, 64, seed=it)
+        sl = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        out.fill_(float("nan"))
+        k.decode_int4(qq, qpp, codes, scales, pe, sl, out, lse, block_table=table)
+        _check(out.view(b, q_len, h, 512), lse.view(b, q_len, h), q, qp, n, s, kp, lens, "fp16")
+        first = out.clone()
+        k.decode_int4(qq, qpp, codes, scales, pe, sl, out, block_table=table)
+        assert torch.equal(out, first)
+    assert k.device_status(torch.device("cuda"), torch.float16) == 0
