@@ -9,8 +9,8 @@
 // lane's eight codes are one 32-bit word and a warp stores whole 128-byte lines; lane l
 // also turns rope pair l.  A gather long enough to fill the GPU has the loads of two rows
 // in flight per warp (131072 4-bit rows 39 us, 41 with one); an append, which computes
-// more, does better with one row and more warps (58 us against 62 and 94 with two and
-// four).
+// more, has one row and more warps (39 us for as many, 45 with the rope part turned; with
+// a slower quantisation 58, and 62 and 94 with two and four rows a warp).
 #include <cuda_fp8.h>
 #include <string.h>
 
@@ -85,13 +85,14 @@ __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
 // infinities as the largest code.
 // max / 7 as a product with 1 / 7, off by 2^-23, rounds to the same half: the maximum has
 // at most 11 bits, so max / 7 is no closer than 2^-12 / 7 of itself to the middle of two
-// normal halves.  f / s is f times an approximate reciprocal, off by less than 2e-6: it
-// rounds to the same integer unless it lies within 1e-5 of a half.  There, in groups that
-// are not finite and where the scale is below fp16's normal range (the only groups whose
-// quotients may pass 7.5) the lane divides.  A fused product and sum with 1.5 x 2^23 rounds to
-// the integer; the codes of the even and of the odd dims are summed with their nibbles'
-// weights as floats (below 2^16, exact): the float pipe has twice the rate of the
-// integer one, which bounded this kernel.
+// normal halves.  f / s is f times an approximate reciprocal, off by less than 2e-6.  Both have
+// at most 11 bits, so 2 f and (2 n + 1) s are multiples of s's last bit and f / s is a
+// tie n + 1/2 exactly or at least 2^-12 away from it: rounded to a multiple of 2^-13 first
+// (a sum with 1.5 x 2^10) it is the tie again or stays on its side, and a sum with 1.5 x 2^23
+// then rounds to the integer as the exact quotient would.  The sums' bits are a constant
+// plus the integer; their nibbles are put together as integers, modulo 2^32.  Groups that
+// are not finite or whose scale is below fp16's normal range (the only ones whose
+// quotients may pass 7.5) are divided.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(uint4 x, __half* scale) {
   const uint32_t m2 = max_abs2<T>(max_abs2<T>(x.x, x.y), max_abs2<T>(x.z, x.w));
@@ -107,33 +108,24 @@ __device__ __forceinline__ uint32_t quantise8(uint4 x, __half* scale) {
   float sf = __half2float(s);
   float inv;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(sf));
-  constexpr float kMagic = 12582912.f;               // 1.5 x 2^23: a sum's last bit counts ones
-  float even = 34952.f, odd = 34952.f;               // 0x8888: n + 8 is the code
-  float far = 0.f;                                   // largest distance from an integer
+  constexpr float kGrid = 1536.f, kRound = 12582912.f - kGrid;
+  constexpr uint32_t kBits = 0x4b400000u;            // of 12582912.f
+  constexpr int kOrder[8] = {7, 5, 3, 1, 6, 4, 2, 0};   // dims of the nibbles, highest first
+  uint32_t w = 0;
 #pragma unroll
-  for (int k = 0; k < 8; ++k) {
-    const float minus_n = kMagic - fmaf(f[k], inv, kMagic);
-    far = fmaxf(far, fabsf(fmaf(f[k], inv, minus_n)));
-    const float weight = -(float)(1 << (4 * (k >> 1)));
-    if (k & 1)
-      odd = fmaf(minus_n, weight, odd);
-    else
-      even = fmaf(minus_n, weight, even);
-  }
-  // 2^23 + a 16-bit integer has it in its last bits
-  uint32_t w = __byte_perm(__float_as_uint(even + 8388608.f), __float_as_uint(odd + 8388608.f), 0x5410);
-  if (far > 0.49999f || !(sf >= 6.103515625e-5f && sf < INFINITY)) {
-    // (the four lanes of a group agree on the scale: all of them or none pass the second test)
-    if (!(sf >= 6.103515625e-5f && sf < INFINITY)) {
-      m = 0.f;                                       // the largest of the numbers' magnitudes
+  for (int k = 0; k < 8; ++k)
+    w = w * 16u + __float_as_uint(__fadd_rn(fmaf(f[kOrder[k]], inv, kGrid), kRound));
+  w += 0x88888888u - kBits * 0x11111111u;
+  // (the four lanes of a group agree on the scale: all of them or none)
+  if (!(sf >= 6.103515625e-5f && sf < INFINITY)) {
+    m = 0.f;                                         // the largest of the numbers' magnitudes
 #pragma unroll
-      for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(f[k]));
-      const unsigned group = 0xfu << (threadIdx.x & 28);
-      m = fmaxf(m, __shfl_xor_sync(group, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(group, m, 2));
-      s = __float2half_rn(fminf(__fdiv_rn(m, 7.f), 65504.f));
-      sf = __half2float(s);
-    }
+    for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(f[k]));
+    const unsigned group = 0xfu << (threadIdx.x & 28);
+    m = fmaxf(m, __shfl_xor_sync(group, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(group, m, 2));
+    s = __float2half_rn(fminf(__fdiv_rn(m, 7.f), 65504.f));
+    sf = __half2float(s);
     w = 0x88888888u;
     if (sf > 0.f) {
       w = 0;
