@@ -9,7 +9,7 @@
 // lane's eight codes are one 32-bit word and a warp stores whole 128-byte lines; lane l
 // also turns rope pair l.  A gather long enough to fill the GPU has the loads of two rows
 // in flight per warp (131072 4-bit rows 39 us, 41 with one); an append, which computes
-// more, has one row and more warps (39 us for as many, 45 with the rope part turned; with
+// more, has one row and more warps (37 us for as many, 41 with the rope part turned; with
 // a slower quantisation 58, and 62 and 94 with two and four rows a warp).
 #include <cuda_fp8.h>
 #include <string.h>
@@ -65,18 +65,19 @@ __device__ __forceinline__ uint32_t code_of(float f, float s) {
   return f == f ? (uint32_t)((int)fminf(fmaxf(r, -8.f), 7.f) + 8) : 8u;
 }
 
-// The larger of two pairs' magnitudes, element by element; NaN wins.
+// The largest magnitude of eight values; NaN wins.
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
 template <typename T>
-__device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
-  a &= 0x7fff7fffu;
-  b &= 0x7fff7fffu;
-  if constexpr (std::is_same<T, __half>::value) {
-    const __half2 m = __hmax2_nan(*reinterpret_cast<__half2*>(&a), *reinterpret_cast<__half2*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&m);
-  } else {
-    const __nv_bfloat162 m = __hmax2_nan(*reinterpret_cast<__nv_bfloat162*>(&a), *reinterpret_cast<__nv_bfloat162*>(&b));
-    return *reinterpret_cast<const uint32_t*>(&m);
-  }
+__device__ __forceinline__ float max_abs8(uint4 x) {
+  using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+  auto abs2 = [](uint32_t w) { return __habs2(*reinterpret_cast<const T2*>(&w)); };
+  const T2 m = __hmax2_nan(__hmax2_nan(abs2(x.x), abs2(x.y)), __hmax2_nan(abs2(x.z), abs2(x.w)));
+  const float2 f = Elt<T>::to2(*reinterpret_cast<const uint32_t*>(&m));
+  return max_nan(f.x, f.y);
 }
 
 // This lane's eight dims as codes (low nibble first: dims 0 2 4 6 1 3 5 7) and its
@@ -95,13 +96,9 @@ __device__ __forceinline__ uint32_t max_abs2(uint32_t a, uint32_t b) {
 // quotients may pass 7.5) are divided.
 template <typename T>
 __device__ __forceinline__ uint32_t quantise8(uint4 x, __half* scale) {
-  const uint32_t m2 = max_abs2<T>(max_abs2<T>(x.x, x.y), max_abs2<T>(x.z, x.w));
-  const float2 mm = Elt<T>::to2(m2);
-  float m = mm.x > mm.y || mm.x != mm.x ? mm.x : mm.y;   // (NaN wins)
-  float o = __shfl_xor_sync(0xffffffffu, m, 1);
-  m = o > m || o != o ? o : m;
-  o = __shfl_xor_sync(0xffffffffu, m, 2);
-  m = o > m || o != o ? o : m;
+  float m = max_abs8<T>(x);
+  m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+  m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
   float f[8];
   unpack8<T>(x, f);
   __half s = __float2half_rn(m * (1.f / 7.f));
