@@ -66,11 +66,6 @@ __device__ __forceinline__ uint32_t code_of(float f, float s) {
 }
 
 // The largest magnitude of eight values; NaN wins.
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float r;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
-  return r;
-}
 template <typename T>
 __device__ __forceinline__ float max_abs8(uint4 x) {
   using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;

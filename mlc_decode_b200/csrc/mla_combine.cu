@@ -20,7 +20,7 @@ constexpr int kMaxSplits = 8192;
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
-  for (int off = 16; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, off));
+  for (int off = 16; off > 0; off >>= 1) v = max_nan(v, __shfl_xor_sync(0xffffffffu, v, off));
   return v;
 }
 __device__ __forceinline__ float warp_sum(float v) {
@@ -66,18 +66,18 @@ mla_combine_kernel(const float* __restrict__ part_lse, const float* __restrict__
   const int lane = tid & 31, warp = tid >> 5;
 
   float mx = -INFINITY;
-  for (int k = tid; k < ns; k += kThreads) mx = fmaxf(mx, part_lse[(size_t)k * lse_stride + row]);
+  for (int k = tid; k < ns; k += kThreads) mx = max_nan(mx, part_lse[(size_t)k * lse_stride + row]);
   mx = warp_max(mx);
   if (lane == 0) s_red[warp] = mx;
   __syncthreads();
   if (tid == 0) {
     float v = s_red[0];
-    for (int w = 1; w < kThreads / 32; ++w) v = fmaxf(v, s_red[w]);
+    for (int w = 1; w < kThreads / 32; ++w) v = max_nan(v, s_red[w]);
     s_bcast = v;
   }
   __syncthreads();
   mx = s_bcast;
-  const bool all_empty = !(mx > -INFINITY);
+  const bool all_empty = mx == -INFINITY;
   const float msafe = all_empty ? 0.f : mx;
 
   float sum = 0.f;

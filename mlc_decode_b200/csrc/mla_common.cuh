@@ -47,6 +47,15 @@ template <> struct Elt<__nv_bfloat16> {
   }
 };
 
+// The larger of two; NaN wins (fmaxf drops it).  The largest LSE of a sequence's pieces
+// goes through this one: a query row that is NaN has only NaN pieces, and a maximum that
+// dropped them would pass the row off as one that sees nothing (zeros, LSE -inf).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
 // ---------------------------------------------------------------------------
 // split planner: _split_plan (mla_decode.py:9-30)
 // ---------------------------------------------------------------------------

@@ -622,10 +622,10 @@ mla_int4_mma_combine_kernel(Int4Args a, const int2* __restrict__ info, int g, in
     __syncthreads();
     // every warp reduces the pieces' LSEs itself
     float mx = -INFINITY;
-    for (int k = lane; k < n; k += 32) mx = fmaxf(mx, s_w[k]);
+    for (int k = lane; k < n; k += 32) mx = max_nan(mx, s_w[k]);
 #pragma unroll
-    for (int off = 16; off > 0; off >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, off));
-    const bool any = mx > -INFINITY || mx != mx;
+    for (int off = 16; off > 0; off >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, off));
+    const bool any = mx != -INFINITY;
     float sum = 0.f;
     if (any)
       for (int k = lane; k < n; k += 32) sum += exp2f((s_w[k] - mx) * kLog2e);

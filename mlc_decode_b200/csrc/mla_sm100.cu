@@ -2554,9 +2554,9 @@ __device__ __forceinline__ void combine_row(const float* __restrict__ part_lse, 
   // the sequence's LSE: every warp reduces the n piece LSEs itself (lanes over pieces)
   const int lane = threadIdx.x & 31;
   float mx = -INFINITY;
-  for (int k = lane; k < n; k += 32) mx = fmaxf(mx, s_lse[k]);
+  for (int k = lane; k < n; k += 32) mx = max_nan(mx, s_lse[k]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+  for (int o = 16; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   float sum = 0.f;
   if (mx != -INFINITY)
     for (int k = lane; k < n; k += 32) sum += exp2f((s_lse[k] - mx) * kLog2e);
@@ -2771,9 +2771,9 @@ mla_seqsplit_combine_kernel(const float* __restrict__ part_lse, const float* __r
       for (int k = threadIdx.x; k < n; k += 128 * G) s_lse[k] = __ldcg(part_lse + slot(k) * kHeads + head);
       __syncthreads();
       float mx = -INFINITY;
-      for (int k = lane; k < n; k += 32) mx = fmaxf(mx, s_lse[k]);
+      for (int k = lane; k < n; k += 32) mx = max_nan(mx, s_lse[k]);
 #pragma unroll
-      for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+      for (int o = 16; o > 0; o >>= 1) mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, o));
       float sum = 0.f;
       if (mx != -INFINITY)
         for (int k = lane; k < n; k += 32) sum += exp2f((s_lse[k] - mx) * kLog2e);
@@ -2875,7 +2875,7 @@ mla_seqsplit_combine_kernel(const float* __restrict__ part_lse, const float* __r
     if (!ok) return;
     float mx = -INFINITY;
 #pragma unroll
-    for (int q = 0; q < kSeqMaxWorld; ++q) mx = fmaxf(mx, lq[q]);
+    for (int q = 0; q < kSeqMaxWorld; ++q) mx = max_nan(mx, lq[q]);
     float sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
     if (mx != -INFINITY) {
