@@ -66,33 +66,6 @@ constexpr int kMaxWorkers = 512;
 constexpr uint32_t kErrLoad = 0x301;
 constexpr uint64_t kWaitNs = 2000000000ull;
 
-template <int MT>
-struct Lay {
-  static constexpr int kRows = 16 * MT;
-  static constexpr int kStages = MT == 1 ? 3 : 5;
-  static constexpr int kCtasPerSm = MT == 1 ? 2 : 1;
-  static constexpr uint32_t kS = kStages * kStage;                        // [4][rows][kSPitch] float
-  static constexpr uint32_t kP = kS + 4 * kRows * kSPitch * 4;            // [rows][kPPitch] half
-  static constexpr uint32_t kAlpha = kP + kRows * kPPitch * 2;            // [rows] float
-  static constexpr uint32_t kInv = kAlpha + kRows * 4;                    // [rows] float
-  static constexpr uint32_t kBar = kInv + kRows * 4;                      // a barrier per stage
-  static constexpr uint32_t kMisc = kBar + 8 * 8;                         // abort flag, Walk of the lookups
-  static constexpr uint32_t kMap = kMisc + 64;                            // [kAhead] first cache row, KV head
-  static constexpr uint32_t kBytes = kMap + kAhead * 8 + 1024;            // + alignment slack
-};
-
-struct MmaParams {
-  CUtensorMap tm_codes;    // [rows][kv_heads][256] bytes, box 64 x 1 x 128
-  CUtensorMap tm_scales;   // [rows][kv_heads][16] halves, box 64 x 1 x 16
-  CUtensorMap tm_kpe;      // [rows][kv_heads][64], box 64 x 1 x 64
-  Int4Args a;
-  uint32_t* status;
-  int2* info;              // [units] of a split unit: its first piece's slot, its last worker; x < 0: not split
-  int g, groups;           // query heads per KV head; groups of 16 MT query rows
-  int num_rows;            // rows of the cache
-  float sl2;               // softmax scale x log2(e)
-};
-
 __device__ __forceinline__ int seq_rows(const Int4Args& a, int s) {
   int len = a.max_len;
   if (a.seqlens != nullptr) {
@@ -100,24 +73,6 @@ __device__ __forceinline__ int seq_rows(const Int4Args& a, int s) {
     len = len < 0 ? 0 : (len > a.max_len ? a.max_len : len);
   }
   return len;
-}
-
-// Bounded wait; once any wait of the CTA has given up every wait returns at once, so
-// that all threads still meet at every barrier and the launch ends.
-__device__ __forceinline__ void wait_full(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t* status,
-                                          uint32_t code) {
-  if (ptx::mbar_try_wait(bar, parity)) return;
-  const uint64_t t0 = ptx::globaltimer();
-  for (;;) {
-    for (int i = 0; i < 32; ++i)
-      if (ptx::mbar_try_wait(bar, parity)) return;
-    if (*abort != 0u) return;
-    if (ptx::globaltimer() - t0 > kWaitNs) {
-      *abort = 1u;
-      atomicCAS(status, 0u, code);
-      return;
-    }
-  }
 }
 
 // The tiles of a worker's range, in order: tile j of the unit `sub` (KV head and row
@@ -141,6 +96,53 @@ struct Walk {
     } while (nt == 0);
   }
 };
+
+template <int MT>
+struct Lay {
+  static constexpr int kRows = 16 * MT;
+  static constexpr int kStages = MT == 1 ? 3 : 5;
+  static constexpr int kCtasPerSm = MT == 1 ? 2 : 1;
+  static constexpr uint32_t kS = kStages * kStage;                        // [4][rows][kSPitch] float
+  static constexpr uint32_t kP = kS + 4 * kRows * kSPitch * 4;            // [rows][kPPitch] half
+  static constexpr uint32_t kAlpha = kP + kRows * kPPitch * 2;            // [rows] float
+  static constexpr uint32_t kInv = kAlpha + kRows * 4;                    // [rows] float
+  static constexpr uint32_t kBar = kInv + kRows * 4;                      // a barrier per stage
+  static constexpr uint32_t kMisc = kBar + 8 * 8;                         // abort flag, Walk of the lookups
+  static_assert(8 + sizeof(Walk) <= 48, "misc block");
+  static constexpr uint32_t kBad = kMisc + 48;                            // [2][2] rows of hide_rows, by tile parity
+  static constexpr uint32_t kMap = kMisc + 64;                            // [kAhead] first cache row, KV head
+  static constexpr uint32_t kBytes = kMap + kAhead * 8 + 1024;            // + alignment slack
+};
+
+struct MmaParams {
+  CUtensorMap tm_codes;    // [rows][kv_heads][256] bytes, box 64 x 1 x 128
+  CUtensorMap tm_scales;   // [rows][kv_heads][16] halves, box 64 x 1 x 16
+  CUtensorMap tm_kpe;      // [rows][kv_heads][64], box 64 x 1 x 64
+  Int4Args a;
+  uint32_t* status;
+  int2* info;              // [units] of a split unit: its first piece's slot, its last worker; x < 0: not split
+  int g, groups;           // query heads per KV head; groups of 16 MT query rows
+  int num_rows;            // rows of the cache
+  float sl2;               // softmax scale x log2(e)
+};
+
+// Bounded wait; once any wait of the CTA has given up every wait returns at once, so
+// that all threads still meet at every barrier and the launch ends.
+__device__ __forceinline__ void wait_full(uint32_t bar, uint32_t parity, volatile uint32_t* abort, uint32_t* status,
+                                          uint32_t code) {
+  if (ptx::mbar_try_wait(bar, parity)) return;
+  const uint64_t t0 = ptx::globaltimer();
+  for (;;) {
+    for (int i = 0; i < 32; ++i)
+      if (ptx::mbar_try_wait(bar, parity)) return;
+    if (*abort != 0u) return;
+    if (ptx::globaltimer() - t0 > kWaitNs) {
+      *abort = 1u;
+      atomicCAS(status, 0u, code);
+      return;
+    }
+  }
+}
 
 template <typename T>
 __device__ __forceinline__ void mma16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -181,6 +183,28 @@ template <typename T>
 __device__ __forceinline__ uint32_t to_h2(uint32_t w) {
   if constexpr (std::is_same<T, __half>::value) return w;
   else return Elt<__half>::pack2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
+// Rows that some of the tile's query rows do not see (a later position's, within the
+// length), [first, end) of the tile at `stage`, may hold anything, but their weight 0 times
+// a value past fp16 would be NaN.  After the scores are taken, a group with such a value gets the
+// scale 0 and its row a bit in `bad`: the query rows that do see it answer NaN instead.
+__device__ __noinline__ void hide_rows(uint8_t* stage, uint32_t* bad, int first, int end, int tid) {
+  for (int i = first * kI4Groups + tid; i < end * kI4Groups; i += kThreads) {
+    const int r = i / kI4Groups, g = i % kI4Groups;
+    __half* scale = reinterpret_cast<__half*>(stage + kCodeBytes + kRopeBytes) + i;
+    const float s = fabsf(__half2float(*scale));
+    if (s * 8.f < 65520.f) continue;   // (65520 and more round to infinity)
+    const uint4 w = *reinterpret_cast<const uint4*>(stage + (g >> 3) * (kCodeBytes / 2) + r * 128 +
+                                                    (((g & 7) ^ (r & 7)) << 4));
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+    int most = 0;                      // the group's largest |n - 8|
+    for (int k = 0; k < kI4Group; ++k) most = max(most, abs((int)((v[k >> 3] >> (4 * (k & 7))) & 15u) - 8));
+    if (s * (float)most < 65520.f) continue;
+    *scale = __ushort_as_half(0);
+    atomicOr(bad + (r >> 5), 1u << (r & 31));
+  }
+  ptx::fence_proxy_async_smem();
 }
 
 __device__ __forceinline__ float exp2_approx(float x) {
@@ -384,6 +408,11 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
         const uint32_t stage = st * kStage;
         uint8_t* scales = smem + st * kStage + kCodeBytes + kRopeBytes;
         const int valid = len - j * kTileR;
+        // rows of this tile that not every position sees: from its first position's length on
+        const int hidden = max(valid - (a.q_len - 1), 0);
+        const bool hides = a.q_len > 1 && hidden < kTileR;
+        uint32_t* bad = reinterpret_cast<uint32_t*>(smem + L::kBad) + 2 * (tile & 1);
+        if (hides && tid < 2) bad[tid] = 0u;
         if (valid < kTileR) {
           // rows past the length: a zero scale makes them zeros whatever the cache holds
           if (tid < 2 * kTileR && (tid >> 1) >= valid)
@@ -433,6 +462,7 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
         __syncthreads();
         // every warp is past the tile before: its stage takes the next load
         if (tid == 0 && tile > 0) fetch(tile - 1 + L::kStages);
+        if (hides) hide_rows(smem + stage, bad, hidden, min(valid, kTileR), tid);
         // ---- softmax: thread <-> row tid / 16 (+ 16 mt), columns 4 (tid % 16)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
@@ -475,6 +505,14 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
           if ((tid & 15) == 0) sAlpha[row] = alpha;
         }
         __syncthreads();
+        if (hides) {
+#pragma unroll
+          for (int mt = 0; mt < MT; ++mt) {
+            const int col = 4 * (tid & 15), seen = row_len[mt] - j * kTileR - col;
+            const uint32_t mine = bad[col >> 5] >> (col & 31);
+            if (seen > 0 && (mine & ((1u << min(seen, 4)) - 1u)) != 0u) l_run[mt] = __int_as_float(0x7fffffff);
+          }
+        }
         // ---- O += P.V, dims [64 warp, +64)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {

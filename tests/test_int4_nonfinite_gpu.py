@@ -103,3 +103,51 @@ def test_combine_of_nan_parts():
     assert out[0, 1].isnan().all() and total[0, 1].isnan() and out[0, 3].isnan().all() and total[0, 3].isnan()
     assert (out[0, 2] == 0).all() and torch.isneginf(total[0, 2])
     assert (out[0, 0] - 1).abs().max() < 1e-6 and abs(total[0, 0].item() - 1.0986123) < 1e-6
+
+
+@pytest.mark.parametrize("kernel", list(KERNELS))
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("ql, h, s", [(2, 16, 129), (3, 16, 200), (3, 40, 66), (5, 3, 64), (70, 1, 100), (4, 16, 3)])
+def test_rows_a_position_does_not_see_may_hold_anything(ql, h, s, dtype, kernel):
+    """The rows of a step's later positions: infinite or NaN scales and rope values, and values
+    past fp16's range, change nothing for the positions before them, to the bit; the
+    tensor-core kernels answer NaN or infinity to those that see them."""
+    _, _, codes, scales, pe, run = _call(2, ql, h, s, dtype, KERNELS[kernel], seed=ql + s)
+    clean, clean_lse = run()
+    for back, scale, rope in ((1, 65504.0, 0.0), (2, NAN, float("inf")), (3, float("inf"), NAN), (4, 9362.0, 0.0)):
+        if back >= min(ql, s):
+            continue
+        keep = scales.clone(), pe.clone(), codes.clone()
+        codes[0, s - back] = 0xff                # the largest code everywhere: 7 x the scale
+        scales[0, s - back, 0, 3::5] = scale     # (7 x 9362 rounds to infinity, 7 x 9352 does not)
+        if rope != 0.0:
+            pe[0, s - back, 0, 11] = rope
+        out, lse = run()
+        blind = ql - back                        # positions [0, blind) do not see the row
+        if kernel in ("auto", "pair") and s > 128:   # (pieces met in order of arrival: the last bit)
+            eps = torch.finfo(dtype).eps
+            assert ((out[0, :blind] - clean[0, :blind]).abs().float() <= eps * clean[0, :blind].abs().float() + 1e-6).all()
+        else:
+            assert torch.equal(out[0, :blind], clean[0, :blind]) and torch.equal(lse[0, :blind], clean_lse[0, :blind])
+        assert torch.isfinite(out[1]).all()
+        if kernel != "simt":
+            assert not torch.isfinite(out[0, blind:]).all(-1).any()
+        scales.copy_(keep[0]), pe.copy_(keep[1]), codes.copy_(keep[2])
+
+
+@pytest.mark.parametrize("kernel", ["auto", "pair", "mma16", "mma32"])
+def test_the_largest_values_fp16_holds_are_values(kernel):
+    """Scales above 8188 whose codes keep the values within fp16's range are ordinary values, for
+    the last positions' rows too."""
+    q, qp, codes, scales, pe, run = _call(1, 3, 16, 80, torch.float16, KERNELS[kernel], seed=9)
+    q.zero_()
+    codes[0, 70:] = 0xff
+    codes[0, 79] = 0x11
+    scales[0, 70:, 0, ::4] = 9352.0
+    ref, ref_lse = torch.empty_like(q), torch.empty(1, 3, 16, device="cuda")
+    MlaPagedDecodeKernel(1, 16, 80, cfg=KERNELS["simt"], q_len=3).decode_int4(q, qp, codes, scales, pe, None, ref, ref_lse)
+    out, lse = run()
+    assert torch.isfinite(ref).all() and torch.isfinite(out).all()
+    # weights and values rounded to fp16 once each, and the result: three times 2^-11 of the largest value
+    assert ((out.float() - ref.float()).abs() <= 3 * 2.0 ** -11 * 65504).all()
+    assert ((lse - ref_lse).abs() <= 1e-4).all()
