@@ -396,7 +396,8 @@ int32_t mla_decode_ext_int4kv(const void* q, const void* q_pe, const void* kv_co
  * q_len 0: new rows are packed, request after request (rows past num_tokens are not
  * added); q_len > 0: num_tokens = batch x q_len, n is at most q_len and request i's rows
  * are the last n of [i q_len, (i + 1) q_len), as mla_decode_ext's causal rule has a step's
- * rows.  new_seqlens may be cache_seqlens and new_free_pos may be free_pos (in place);
+ * rows (a request that got fewer rows than n is not lined up with that rule any more: see
+ * mla_extend_block_tables_whole).  new_seqlens may be cache_seqlens and new_free_pos may be free_pos (in place);
  * otherwise no two arrays overlap.  Workspace: mla_block_tables_workspace_bytes (16-byte
  * aligned; 0 with no error text: none).
  */
@@ -407,6 +408,20 @@ int32_t mla_extend_block_tables(int32_t* block_table, const int32_t* cache_seqle
                                 void* workspace, size_t workspace_bytes, int32_t batch, int32_t max_pages,
                                 int32_t page_size, int32_t num_pages, int32_t num_free, int32_t num_tokens,
                                 int32_t q_len, void* stream);
+/*
+ * The same for a decode step whose positions are to see their own rows (q_len >= 1):
+ * a request gets a place for all of its n rows or for none.  With fewer rows than asked
+ * for, mla_decode_ext's causal rule, which counts back from the sequence's last row, would
+ * show a position other rows than its own.  A request whose table row is too short keeps its
+ * length; from the first request on that does not find all the pages it lacks, nobody gets
+ * new pages (rows that fit in pages already held are placed).
+ */
+int32_t mla_extend_block_tables_whole(int32_t* block_table, const int32_t* cache_seqlens, const int32_t* new_lens,
+                                      const int32_t* free_pages, const int32_t* free_pos, int32_t* new_seqlens,
+                                      int32_t* new_free_pos, int32_t* slots, int32_t* positions, int32_t* cu_new,
+                                      void* workspace, size_t workspace_bytes, int32_t batch, int32_t max_pages,
+                                      int32_t page_size, int32_t num_pages, int32_t num_free, int32_t num_tokens,
+                                      int32_t q_len, void* stream);
 
 /*
  * Rotary positions.  No counterpart in the reference (its inputs come rotated).

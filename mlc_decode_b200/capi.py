@@ -33,7 +33,8 @@ EXPORTED_SYMBOLS = ("mla_abi_version", "mla_last_error", "mla_split_plan",
                     "mla_seqsplit_buffer_bytes", "mla_ipc_export", "mla_ipc_import", "mla_ipc_close",
                     "mla_seqsplit_exchange", "mla_seqsplit_decode", "mla_seqsplit_merge",
                     "mla_decode_int4kv_workspace_bytes", "mla_decode_ext_int4kv",
-                    "mla_block_tables_workspace_bytes", "mla_extend_block_tables", "mla_rotary",
+                    "mla_block_tables_workspace_bytes", "mla_extend_block_tables",
+                    "mla_extend_block_tables_whole", "mla_rotary",
                     "mla_cache_append", "mla_cache_gather")
 
 MLA_CACHE_MODEL = 0
@@ -165,6 +166,8 @@ def load(build_if_missing: bool = True):
         lib.mla_extend_block_tables.argtypes = [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, sz, i32, i32, i32, i32,
                                                 i32, i32, i32, vp]
         lib.mla_extend_block_tables.restype = i32
+        lib.mla_extend_block_tables_whole.argtypes = lib.mla_extend_block_tables.argtypes
+        lib.mla_extend_block_tables_whole.restype = i32
         lib.mla_rotary.argtypes = [vp, vp, vp, vp, f32, i32, i32, i32, i32, i32, i32, i64, i64, i64, i64, i32, vp]
         lib.mla_rotary.restype = i32
         lib.mla_cache_append.argtypes = [vp, vp, vp, vp, vp, vp, f32, vp, vp, f32, i32, i64, i32, i64, i64, i64, i64,
@@ -439,6 +442,13 @@ def block_tables_workspace_bytes(batch, num_tokens) -> int:
 def extend_block_tables(*args) -> None:
     """mla_extend_block_tables, its arguments in order (pointers are device addresses)."""
     rc = load().mla_extend_block_tables(*args)
+    if rc:
+        check(rc)
+
+
+def extend_block_tables_whole(*args) -> None:
+    """mla_extend_block_tables_whole, its arguments in order."""
+    rc = load().mla_extend_block_tables_whole(*args)
     if rc:
         check(rc)
 

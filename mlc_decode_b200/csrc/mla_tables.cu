@@ -38,6 +38,7 @@ struct TablesArgs {
   int* cu_new;               // [batch + 1] or nullptr
   int batch, max_pages, page, num_pages, num_free, num_tokens;
   int q_len;                 // 0: rows packed; else request i's rows are the last of [i q_len, (i + 1) q_len)
+  int whole;                 // a request gets all of its rows or none (q_len > 0)
 };
 
 // One request: first row in the packed list, rows held before, rows held after, and
@@ -67,7 +68,12 @@ __device__ long long block_scan(long long v, long long* s_warp) {
 // The records of every request, by one CTA; thread t owns requests [t per, (t + 1) per).
 // A request's lengths are read and its new length written by the same thread, so
 // new_seqlens may be seqlens.
+// With `whole` a request whose table row is too short asks for nothing, and one that does not
+// find all its pages takes none; nor do those behind it that need any, so that the pages
+// handed out are still a prefix of the sums.
 __device__ void plan(const TablesArgs& a, Record* rec, long long* s_warp) {
+  __shared__ int s_taken;   // with `whole`: pages handed out
+  if (threadIdx.x == 0) s_taken = 0;
   const int per = (a.batch + kThreads - 1) / kThreads;
   const int i0 = min((int)threadIdx.x * per, a.batch), i1 = min(i0 + per, a.batch);
   const long long cover = (long long)a.max_pages * a.page;
@@ -81,9 +87,11 @@ __device__ void plan(const TablesArgs& a, Record* rec, long long* s_warp) {
   auto cut = [&](long long v) { return (int)min(v, (long long)a.num_tokens); };
   long long pages = 0;
   for (int i = i0; i < i1; ++i) {
-    const int n = asked(i), cu = cut(at), rows = cut(at + n) - cu;
+    const int n = asked(i), cu = cut(at);
+    int rows = cut(at + n) - cu;
     at += n;
     const int len = old_len(i);
+    if (a.whole && len + (long long)rows > cover) rows = 0;
     rec[i] = Record{cu, len, rows, 0};   // end: the rows asked for, until the pages are known
     pages += page_count(min(len + (long long)rows, cover), a.page) - page_count(len, a.page);
   }
@@ -101,11 +109,18 @@ __device__ void plan(const TablesArgs& a, Record* rec, long long* s_warp) {
     r.first = pos0 + (int)min(taken, avail);
     r.end = (int)min(want, (long long)(held + got) * a.page);
     taken += take;
+    if (a.whole) {
+      if (got < take)
+        r.end = r.len;
+      else if (take > 0)
+        atomicMax(&s_taken, (int)taken);   // (at most avail)
+    }
     rec[i] = r;
     if (a.cu_new != nullptr) a.cu_new[i] = r.cu;
     a.new_seqlens[i] = r.end;
   }
-  if (threadIdx.x == kThreads - 1) *a.new_free_pos = pos0 + (int)min(incl, avail);
+  if (a.whole) __syncthreads();
+  if (threadIdx.x == kThreads - 1) *a.new_free_pos = pos0 + (a.whole ? s_taken : (int)min(incl, avail));
 }
 
 // Slot and position of row p of request i; p at a page's start also names the page in
@@ -185,6 +200,54 @@ __global__ void __launch_bounds__(kFillThreads) mla_tables_fill_kernel(TablesArg
 
 bool small(int batch, int num_tokens) { return batch <= kSmallBatch && num_tokens <= kSmallTokens; }
 
+
+int extend(const char* fn, TablesArgs a, void* workspace, size_t workspace_bytes, void* stream) {
+  const int batch = a.batch, max_pages = a.max_pages, page_size = a.page, num_pages = a.num_pages,
+            num_free = a.num_free, num_tokens = a.num_tokens, q_len = a.q_len;
+  if (batch < 1 || max_pages < 1 || page_size < 1 || num_pages < 1 || num_free < 0 || num_tokens < 0 || q_len < 0) {
+    set_error("%s: bad size (batch %d, max_pages %d, page_size %d, num_pages %d, num_free %d, num_tokens %d, "
+              "q_len %d)", fn, batch, max_pages, page_size, num_pages, num_free, num_tokens, q_len);
+    return MLA_ERR_ARG;
+  }
+  if ((long long)num_pages * page_size > INT32_MAX || (long long)max_pages * page_size > INT32_MAX) {
+    set_error("%s: num_pages x page_size and max_pages x page_size must stay below 2^31 rows (page_size %d, "
+              "num_pages %d, max_pages %d)", fn, page_size, num_pages, max_pages);
+    return MLA_ERR_ARG;
+  }
+  if (q_len > 0 && (long long)batch * q_len != num_tokens) {
+    set_error("%s: with q_len, num_tokens must be batch x q_len (%d x %d, got %d)", fn, batch, q_len, num_tokens);
+    return MLA_ERR_ARG;
+  }
+  if (!a.block_table || !a.seqlens || !a.new_lens || !a.free_pos || !a.new_seqlens || !a.new_free_pos ||
+      (num_free > 0 && !a.free_pages) || (num_tokens > 0 && (!a.slots || !a.positions))) {
+    set_error("%s: null pointer", fn);
+    return MLA_ERR_ARG;
+  }
+  const bool one = small(batch, num_tokens);
+  if (!one && (workspace == nullptr || workspace_bytes < (size_t)batch * sizeof(Record) ||
+               (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)) {
+    set_error("%s: workspace needs %zu bytes, 16-byte aligned (got %zu at %p)", fn, (size_t)batch * sizeof(Record),
+              workspace_bytes, workspace);
+    return MLA_ERR_WORKSPACE;
+  }
+  const cudaStream_t s = static_cast<cudaStream_t>(stream);
+  if (one) {
+    mla_tables_small_kernel<<<1, kThreads, 0, s>>>(a);
+  } else {
+    Record* rec = static_cast<Record*>(workspace);
+    mla_tables_plan_kernel<<<1, kThreads, 0, s>>>(a, rec);
+    const long long quads = ((long long)num_tokens + 3) / 4;
+    if (quads > 0)
+      mla_tables_fill_kernel<<<(unsigned)((quads + kFillThreads - 1) / kFillThreads), kFillThreads, 0, s>>>(a, rec);
+  }
+  const cudaError_t err = cudaGetLastError();
+  if (err != cudaSuccess) {
+    set_error("%s: launch failed: %s", fn, cudaGetErrorString(err));
+    return MLA_ERR_CUDA;
+  }
+  return MLA_OK;
+}
+
 }  // namespace
 }  // namespace mla
 
@@ -208,51 +271,27 @@ int32_t mla_extend_block_tables(int32_t* block_table, const int32_t* cache_seqle
                                 void* workspace, size_t workspace_bytes, int32_t batch, int32_t max_pages,
                                 int32_t page_size, int32_t num_pages, int32_t num_free, int32_t num_tokens,
                                 int32_t q_len, void* stream) {
-  const char* fn = "mla_extend_block_tables";
-  if (batch < 1 || max_pages < 1 || page_size < 1 || num_pages < 1 || num_free < 0 || num_tokens < 0 || q_len < 0) {
-    set_error("%s: bad size (batch %d, max_pages %d, page_size %d, num_pages %d, num_free %d, num_tokens %d, "
-              "q_len %d)", fn, batch, max_pages, page_size, num_pages, num_free, num_tokens, q_len);
+  return extend("mla_extend_block_tables",
+                TablesArgs{block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens, new_free_pos, slots,
+                           positions, cu_new, batch, max_pages, page_size, num_pages, num_free, num_tokens, q_len, 0},
+                workspace, workspace_bytes, stream);
+}
+
+int32_t mla_extend_block_tables_whole(int32_t* block_table, const int32_t* cache_seqlens, const int32_t* new_lens,
+                                      const int32_t* free_pages, const int32_t* free_pos, int32_t* new_seqlens,
+                                      int32_t* new_free_pos, int32_t* slots, int32_t* positions, int32_t* cu_new,
+                                      void* workspace, size_t workspace_bytes, int32_t batch, int32_t max_pages,
+                                      int32_t page_size, int32_t num_pages, int32_t num_free, int32_t num_tokens,
+                                      int32_t q_len, void* stream) {
+  const char* fn = "mla_extend_block_tables_whole";
+  if (q_len < 1) {
+    set_error("%s: q_len must be >= 1, got %d", fn, q_len);
     return MLA_ERR_ARG;
   }
-  if ((long long)num_pages * page_size > INT32_MAX || (long long)max_pages * page_size > INT32_MAX) {
-    set_error("%s: num_pages x page_size and max_pages x page_size must stay below 2^31 rows (page_size %d, "
-              "num_pages %d, max_pages %d)", fn, page_size, num_pages, max_pages);
-    return MLA_ERR_ARG;
-  }
-  if (q_len > 0 && (long long)batch * q_len != num_tokens) {
-    set_error("%s: with q_len, num_tokens must be batch x q_len (%d x %d, got %d)", fn, batch, q_len, num_tokens);
-    return MLA_ERR_ARG;
-  }
-  if (!block_table || !cache_seqlens || !new_lens || !free_pos || !new_seqlens || !new_free_pos ||
-      (num_free > 0 && !free_pages) || (num_tokens > 0 && (!slots || !positions))) {
-    set_error("%s: null pointer", fn);
-    return MLA_ERR_ARG;
-  }
-  const bool one = small(batch, num_tokens);
-  if (!one && (workspace == nullptr || workspace_bytes < (size_t)batch * sizeof(Record) ||
-               (reinterpret_cast<uintptr_t>(workspace) & 15u) != 0)) {
-    set_error("%s: workspace needs %zu bytes, 16-byte aligned (got %zu at %p)", fn, (size_t)batch * sizeof(Record),
-              workspace_bytes, workspace);
-    return MLA_ERR_WORKSPACE;
-  }
-  const TablesArgs a{block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens, new_free_pos, slots,
-                     positions, cu_new, batch, max_pages, page_size, num_pages, num_free, num_tokens, q_len};
-  const cudaStream_t s = static_cast<cudaStream_t>(stream);
-  if (one) {
-    mla_tables_small_kernel<<<1, kThreads, 0, s>>>(a);
-  } else {
-    Record* rec = static_cast<Record*>(workspace);
-    mla_tables_plan_kernel<<<1, kThreads, 0, s>>>(a, rec);
-    const long long quads = ((long long)num_tokens + 3) / 4;
-    if (quads > 0)
-      mla_tables_fill_kernel<<<(unsigned)((quads + kFillThreads - 1) / kFillThreads), kFillThreads, 0, s>>>(a, rec);
-  }
-  const cudaError_t err = cudaGetLastError();
-  if (err != cudaSuccess) {
-    set_error("%s: launch failed: %s", fn, cudaGetErrorString(err));
-    return MLA_ERR_CUDA;
-  }
-  return MLA_OK;
+  return extend(fn,
+                TablesArgs{block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens, new_free_pos, slots,
+                           positions, cu_new, batch, max_pages, page_size, num_pages, num_free, num_tokens, q_len, 1},
+                workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"

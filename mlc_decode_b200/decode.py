@@ -565,8 +565,9 @@ class MlaPagedDecodeKernel:
         request i keeps its last ``new_lens[i]`` (int32 [batch] on the device; None: all q_len).
         The cache is 16-bit, e4m3 (``kv_scale``) or 4-bit (``kv_scales``), as ``cache_append``
         has it.  ``block_table``, ``cache_seqlens`` and ``free_pos`` (see
-        ``extend_block_tables``) are updated in place; a request whose table row or free list
-        is full keeps its length.  With ``rotary`` q_pe (into this object's scratch, q_pe
+        ``extend_block_tables``, ``whole``) are updated in place; a request whose table row or
+        free list has no place for all of its new rows keeps its length, stores none of them, and
+        its ``out`` and ``lse`` are of no use.  With ``rotary`` q_pe (into this object's scratch, q_pe
         itself stays) and k_pe turn to their rows' positions.  Like the workspace, the scratch
         is this object's: calls of one object are serialised by the caller, and the first call
         on a device precedes any graph capture.
@@ -625,7 +626,7 @@ class MlaPagedDecodeKernel:
         slots, positions, all_new, turned = self._step_scratch(dev, dtype)
         paged.extend_block_tables(block_table, cache_seqlens, all_new if new_lens is None else new_lens, free_pages,
                                   free_pos, cache_seqlens, free_pos, slots, positions,
-                                  page_size=page_size, num_pages=num_pages, q_len=ql)
+                                  page_size=page_size, num_pages=num_pages, q_len=ql, whole=True)
         paged.cache_append(kv.view(b * ql, kvh, DIM), k_pe.view(b * ql, kvh, PE_DIM), slots, kv_cache, k_pe_cache,
                            kv_scale=kv_scale, kv_scales=kv_scales, rotary=rotary,
                            positions=None if rotary is None else positions)

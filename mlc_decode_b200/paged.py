@@ -25,7 +25,7 @@ _ROTARY_DTYPES = {**_DTYPES, torch.float32: capi.MLA_DTYPE_F32}
 
 
 def extend_block_tables(block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens, new_free_pos, slots,
-                        positions, page_size, num_pages, cu_new=None, q_len=0):
+                        positions, page_size, num_pages, cu_new=None, q_len=0, whole=False):
     """Give every request ``new_lens[i]`` more cache rows (mla_extend_block_tables).
 
     All tensors int32 on one device.  ``block_table`` [batch, max_pages] is extended in
@@ -35,7 +35,10 @@ def extend_block_tables(block_table, cache_seqlens, new_lens, free_pages, free_p
     ``new_free_pos`` [1], ``slots`` [num_tokens] (cache row of every new row, -1 where there is
     none), ``positions`` [num_tokens] (index in its sequence) and ``cu_new`` [batch + 1]
     (first new row of every request; optional).  New rows are packed, request after request,
-    or, with ``q_len``, the last rows of each request's q_len.  ``new_seqlens`` may be
+    or, with ``q_len``, the last rows of each request's q_len.  ``whole`` (with ``q_len``
+    only): a request gets all of its rows or none, as a decode over them needs it (its causal
+    rule counts back from the last row); from the first one on that does not find its pages
+    nobody gets new pages (mla_extend_block_tables_whole).  ``new_seqlens`` may be
     ``cache_seqlens`` and ``new_free_pos`` may be ``free_pos``; nothing else may overlap.
     """
     if not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
@@ -69,7 +72,8 @@ def extend_block_tables(block_table, cache_seqlens, new_lens, free_pages, free_p
     n, nf = slots.numel(), free_pages.numel()
     nbytes = capi.block_tables_workspace_bytes(b, n)
     ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
-    _on_device(dev, capi.extend_block_tables, block_table.data_ptr(), cache_seqlens.data_ptr(), new_lens.data_ptr(),
+    call = capi.extend_block_tables_whole if whole else capi.extend_block_tables
+    _on_device(dev, call, block_table.data_ptr(), cache_seqlens.data_ptr(), new_lens.data_ptr(),
                free_pages.data_ptr(), free_pos.data_ptr(), new_seqlens.data_ptr(), new_free_pos.data_ptr(),
                slots.data_ptr(), positions.data_ptr(), None if cu_new is None else cu_new.data_ptr(),
                None if ws is None else ws.data_ptr(), nbytes, b, max_pages, int(page_size), int(num_pages), nf, n,

@@ -51,14 +51,15 @@ def dequantise_int4(codes, scales):
     return n * np.repeat(scales.astype(np.float64), GROUP, axis=-1)
 
 
-def extend_tables(table, lens, new, free, free_pos, page, num_pages, num_tokens, q_len=0):
-    """mla_extend_block_tables, request by request and row by row."""
+def extend_tables(table, lens, new, free, free_pos, page, num_pages, num_tokens, q_len=0, whole=False):
+    """mla_extend_block_tables (``whole``: mla_extend_block_tables_whole), request by request
+    and row by row."""
     table = [list(r) for r in table]
     max_pages = len(table[0])
     cover = max_pages * page
     slots, positions = [-1] * num_tokens, [0] * num_tokens
     pos = min(max(free_pos, 0), len(free))
-    out_lens, cu, at = [], [0], 0
+    out_lens, cu, at, closed = [], [0], 0, False
     for i, (length, n) in enumerate(zip(lens, new)):
         length, n = min(max(length, 0), cover), max(n, 0)
         if q_len:
@@ -69,6 +70,12 @@ def extend_tables(table, lens, new, free, free_pos, page, num_pages, num_tokens,
             first, kept = at, max(0, min(n, num_tokens - at))
         held = -(-length // page)
         end = min(length + kept, cover)
+        if whole:
+            lacks = -(-end // page) - held
+            if length + kept > cover:
+                end = length
+            elif lacks and (closed or lacks > len(free) - pos):
+                closed, end = True, length
         got = 0
         while held + got < -(-end // page) and pos < len(free):
             table[i][held + got] = free[pos]
