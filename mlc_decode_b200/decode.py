@@ -623,6 +623,8 @@ class MlaPagedDecodeKernel:
             if (dev.index, dtype) not in self._ws:
                 _not_capturing("the workspace")
             self._workspace(dev, dtype)
+        if rotary is not None:
+            rotary.turns(dev)       # (uploaded by a first call, which a capture refuses)
         slots, positions, all_new, turned = self._step_scratch(dev, dtype)
         paged.extend_block_tables(block_table, cache_seqlens, all_new if new_lens is None else new_lens, free_pages,
                                   free_pos, cache_seqlens, free_pos, slots, positions,
