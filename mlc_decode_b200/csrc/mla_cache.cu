@@ -12,6 +12,7 @@
 // more, has one row and more warps (37 us for as many, 41 with the rope part turned; with
 // a slower quantisation 58, and 62 and 94 with two and four rows a warp).
 #include <cuda_fp8.h>
+#include <math.h>
 #include <string.h>
 
 #include <type_traits>
@@ -317,7 +318,7 @@ int run(const char* fn, const CacheArgs& a, bool append, int form, int dtype, vo
     set_error("%s: unknown cache form %d", fn, form);
     return MLA_ERR_ARG;
   }
-  if (form == MLA_CACHE_FP8 && (!(a.kv_scale > 0.f) || a.kv_scale > 3.4e38f)) {
+  if (form == MLA_CACHE_FP8 && (!(a.kv_scale > 0.f) || !isfinite(a.kv_scale))) {
     set_error("%s: kv_scale must be finite and > 0", fn);
     return MLA_ERR_ARG;
   }

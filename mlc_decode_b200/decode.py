@@ -10,6 +10,7 @@ allocated on first use and reused, and passes it through the C ABI.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 import os
 import threading
@@ -608,8 +609,10 @@ class MlaPagedDecodeKernel:
         num_pages, page_size = kv_cache.shape[:2]
         if num_pages * page_size >= (1 << 31) - 256:
             raise ValueError(f"the cache must hold fewer than 2^31 - 256 rows, got {num_pages * page_size}")
-        if kv_scale is not None and not (kv_scale > 0 and math.isfinite(kv_scale)):
-            raise ValueError(f"kv_scale must be finite and > 0, got {kv_scale}")
+        if kv_scale is not None:
+            scale = ctypes.c_float(float(kv_scale)).value      # as the kernels take it
+            if not (scale > 0 and math.isfinite(scale)):
+                raise ValueError(f"kv_scale must be finite and > 0 in float32, got {kv_scale}")
         for name, t in (("q", q), ("q_pe", q_pe), ("out", out), ("kv", kv), ("k_pe", k_pe), ("kv_cache", kv_cache),
                         ("k_pe_cache", k_pe_cache), ("kv_scales", kv_scales)):
             if t is not None and t.data_ptr() % 16:

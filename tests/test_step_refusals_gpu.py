@@ -31,6 +31,14 @@ def _args(b, h, form):
     return a
 
 
+@pytest.mark.parametrize("scale", [1e39, 1e-50, float("nan"), -1.0])
+def test_scales_outside_float32(scale):
+    a = _args(2, 16, "fp8")
+    with pytest.raises(ValueError, match="kv_scale"):
+        MlaPagedDecodeKernel(2, 16, 128).step(**{**a, "kv_scale": scale})
+    assert a["cache_seqlens"].tolist() == [0, 0] and a["free_pos"].item() == 0 and (a["block_table"] == -1).all()
+
+
 @pytest.mark.parametrize("form", ["model", "fp8", "int4"])
 def test_a_rotary_first_met_in_a_capture(form):
     a = _args(2, 16, form)

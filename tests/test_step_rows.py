@@ -41,3 +41,12 @@ def test_the_rule_by_hand():
     # a table row that is too short is refused by itself: the next request still finds its page
     got = P.extend_tables([[3], [0]], [63, 0], [2, 2], [7], 0, 64, 8, 4, 2, whole=True)
     assert got[:4] == ([[3], [7]], [63, 2], 1, [-1, -1, 7 * 64, 7 * 64 + 1])
+
+
+def test_append_takes_every_float32_scale():
+    """What the decode takes as an e4m3 scale the append takes too (no rows: nothing launches)."""
+    lib = capi.load()
+    for scale, status in ((3.4028e38, 0), (1e-45, 0), (1e39, 1), (1e-50, 1), (-1.0, 1)):
+        got = lib.mla_cache_append(PTR, PTR, PTR, PTR, None, PTR, scale, None, None, 1.0, 0, 0, 1, 128, 512, 512, 64, 64,
+                                   1, 1, None)
+        assert got == status, scale
