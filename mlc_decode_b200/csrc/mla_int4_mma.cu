@@ -492,7 +492,7 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
             m_run[mt] = m_new;
           }
           // a query row that has seen nothing yet: every weight 0
-          const float ms = m_run[mt] == -INFINITY ? 0.f : m_run[mt] * p.sl2;
+          const float ms = m_run[mt] == -INFINITY ? 0.f : fmaf(m_run[mt], p.sl2, -kI4WeightLog2);
           float ls = 0.f;
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
@@ -568,7 +568,7 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
         for (int off = 8; off > 0; off >>= 1) l += __shfl_xor_sync(0xffffffffu, l, off);
         const int row = 16 * mt + (tid >> 4), r = r_base + row;
         if ((tid & 15) == 0) {
-          const float lse = l != 0.f ? (m_run[mt] * p.sl2 + log2f(l)) * kLn2 : -INFINITY;
+          const float lse = l != 0.f ? (m_run[mt] * p.sl2 + (log2f(l) - kI4WeightLog2)) * kLn2 : -INFINITY;
           sInv[row] = l != 0.f ? 1.f / l : 0.f;
           if (!whole)
             a.part_lse[slot * L::kRows + row] = lse;

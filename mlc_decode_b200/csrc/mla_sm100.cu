@@ -1844,6 +1844,7 @@ __device__ __forceinline__ void softmax_epilogue(const Params& p, const Ctx& c, 
   const uint32_t s_free0_leader = ptx::mapa(ptx::smem_u32(&bars->s_free[0]), 0);
   const uint32_t p_full0_leader = ptx::mapa(ptx::smem_u32(&bars->p_full[0]), 0);
   const uint32_t o_free_leader = ptx::mapa(ptx::smem_u32(&bars->o_free), 0);
+  constexpr float kWeightLog2 = Io<T>::kKv4 ? kI4WeightLog2 : 0.f;
   float sl2 = p.sl2;       // FP8: per piece, times this row's s / a
   float qinv_next = 1.f;   // FP8: s / a of the piece whose Q was quantized last
   uint32_t gi = 0;
@@ -2026,7 +2027,7 @@ __device__ __forceinline__ void softmax_epilogue(const Params& p, const Ctx& c, 
         l *= alpha;
         m_run = m_new;
       }
-      const float ms = m_run * sl2;
+      const float ms = m_run * sl2 - kWeightLog2;
       uint32_t phi[32], plo[32];
       float ls = 0.f;
 #pragma unroll
@@ -2094,7 +2095,7 @@ __device__ __forceinline__ void softmax_epilogue(const Params& p, const Ctx& c, 
     if (!sync4(lx, n_lx)) return;
     const float ltot = l + xl[L ^ 64];
     const float inv = (kK8 ? p.kv_scale : 1.f) / ltot;   // FP8: V's scale, folded here
-    const float lse = (m_run * sl2 + log2f(ltot)) * kLn2;
+    const float lse = (m_run * sl2 + (log2f(ltot) - kWeightLog2)) * kLn2;
     const int head = 64 * (int)rank + m;                   // row within the head group
     const int hglob = vseq_head0(p, pc.bb) + head;         // head within the sequence
     const size_t orow_g = (size_t)vseq_seq(p, pc.bb) * p.heads + hglob;

@@ -5,6 +5,13 @@
 
 namespace mla {
 
+// The 4-bit kernels' softmax weights are fp16 and as large as 2^8 beside a row's running
+// maximum (which moves only when it grows by more).  They carry a factor of 2^7, which
+// 1 / l takes out again: the largest is 2^15, and a weight keeps its eleven bits down to
+// 2^-21 of the maximum's and vanishes below 2^-32 (2^-14 and 2^-25 without: one dominant row
+// beside 20,000 of weight 2^-24.6 gave those half as much again).
+constexpr float kI4WeightLog2 = 7.f;
+
 // Groups of 128 heads per sequence: the tensor-core kernel's work units.
 int head_groups(int heads);
 
