@@ -135,7 +135,8 @@ class Rotary:
 
     ``rot(x, positions, out, offset=0)``: x, out [tokens, heads, head_dim] in float16,
     bfloat16 or float32 (any token and head strides, last dim contiguous), positions int32
-    [tokens]; dims [offset, offset + rot_dim) turn, the others are copied; out may be x.
+    [tokens]; dims [offset, offset + rot_dim) turn, the others are copied; out may be x, or have no
+    element in common with it (slices of one buffer with the same strides will do).
     ``interleaved``: pairs are dims (2 i, 2 i + 1), else (i, i + rot_dim / 2).  ``scaling``: see
     ``rotary_frequencies``.  The frequencies are uploaded by the first call on a device (make
     it, or ``rot.turns(device)``, before a graph capture: a capture refuses).
@@ -194,19 +195,42 @@ class Rotary:
             xs = os_ = (h * d, d)
             meet = xp != op and abs(xp - op) < n * h * d * dtype.itemsize
         else:
-            xs, os_ = x.stride(), out.stride()
-            meet = xs != os_ if xp == op else _ranges_meet(x, out)
+            xs, os_ = _strides(x), _strides(out)
+            meet = xs != os_ if xp == op else _share_elements(x, out)
         if meet:
             raise ValueError("out must be x itself or must not overlap it")
         _on_device(dev, capi.rotary, xp, op, positions.data_ptr(), self.turns(dev).data_ptr(), self.gain, n, h, d,
                    self.rot_dim, int(offset), self.interleaved, xs[0], xs[1], os_[0], os_[1], _ROTARY_DTYPES[dtype])
 
 
-def _ranges_meet(a, b):
-    a0, b0 = a.data_ptr(), b.data_ptr()
-    first, low, high = (a, a0, b0) if a0 < b0 else (b, b0, a0)
-    last = sum((s - 1) * st for s, st in zip(first.shape, first.stride()))
-    return high < low + (last + 1) * first.element_size()
+def _strides(t):
+    """Token and head stride; of a dimension of one entry any stride will do."""
+    (n, h, _), (sn, sh, _) = t.shape, t.stride()
+    return sn if n > 1 else 0, sh if h > 1 else 0
+
+
+def _share_elements(a, b):
+    """Whether two 3-D tensors of one shape and type (last dim contiguous) have an element in
+    common.  Exact where their strides are the same, as those of slices of one buffer are; True
+    where it would take more to tell."""
+    apart = (b.data_ptr() - a.data_ptr()) // a.element_size()
+    dims = sorted(((sa, sb, n) for sa, sb, n in zip(a.stride()[:2], b.stride()[:2], a.shape[:2]) if n > 1), reverse=True)
+
+    def meet(apart, dims):       # rows of a from 0, of b from `apart`
+        ends = [sum((n - 1) * d[k] for *d, n in dims) + a.shape[2] for k in (0, 1)]
+        if apart >= ends[0] or -apart >= ends[1]:
+            return False
+        if not dims:
+            return True
+        (sa, sb, n), inner = dims[0], dims[1:]
+        if sa != sb or sa == 0:
+            return True
+        # entries i apart along the outermost dim whose inner extents overlap
+        ends = [e - (n - 1) * sa for e in ends]
+        low, high = max(-((apart + ends[1] - 1) // sa), 1 - n), min((ends[0] - 1 - apart) // sa, n - 1)
+        return high - low > 16 or any(meet(apart + i * sa, inner) for i in range(low, high + 1))
+
+    return meet(apart, dims)
 
 
 def _check_rows(name, t, shape, dtype, device, written=False, align=1):
@@ -236,12 +260,6 @@ def _check_rows(name, t, shape, dtype, device, written=False, align=1):
             if s < need:
                 raise ValueError(f"{name}: rows overlap (strides {t.stride()})")
             need = s * (size - 1) + need
-
-
-def _strides(t):
-    """Token and head stride; of a dimension of one entry any stride will do."""
-    (n, h, _), (sn, sh, _) = t.shape, t.stride()
-    return sn if n > 1 else 0, sh if h > 1 else 0
 
 
 def _check_cache(kv_cache, k_pe_cache, kv_scale, kv_scales, dtype, device):
