@@ -2616,7 +2616,9 @@ mla_pair_combine_kernel(const float* __restrict__ part_lse, const float* __restr
   __shared__ float4 s_acc[kCombineGroups - 1][128];
   const int head = blockIdx.x, bb = blockIdx.y;
   ptx::grid_dep_wait();   // the decode kernel's partials are complete and visible
-  const TileMap m = tile_map(cu, nt, total_fixed, vbatch, pairs);
+  TileMap m = tile_map(cu, nt, total_fixed, vbatch, pairs);
+  if (m.whole) return;   // nothing is split
+  m.whole = false;       // (known from here on: 1.5 us less at 8 sequences of 8 pieces)
   if (m.first(bb) == m.first(bb + 1)) return;   // empty sequence (written by the plan kernel)
   int pf, pl;
   pairs_of_sequence(m, bb, &pf, &pl);
@@ -2642,8 +2644,9 @@ mla_ragged_combine_kernel(const float* __restrict__ part_lse, const float* __res
   __shared__ int s_list[kMaxPairs];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   ptx::grid_dep_wait();
-  const TileMap m = tile_map(cu, 0, 0u, vbatch, pairs);
+  TileMap m = tile_map(cu, 0, 0u, vbatch, pairs);
   if (m.whole) return;
+  m.whole = false;
   auto wide = [&](int v) -> bool {
     if (v >= vbatch || m.first(v) == m.first(v + 1)) return false;
     int pf, pl;
