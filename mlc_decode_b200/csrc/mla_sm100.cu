@@ -2157,16 +2157,17 @@ __device__ __forceinline__ void softmax_epilogue(const Params& p, const Ctx& c, 
       // this CTA completes a split sequence: merge every piece into `out`
       __threadfence();
       const int own = pair;
+      // every pair after the first starts its range inside the sequence: its first piece
+      const size_t slot0 = pair_slot(tm, pf, pc.bb);
+      auto mslot = [&](int pp) -> size_t { return pp == pf ? slot0 : (size_t)pp * 2; };
       float mx = lse;
       for (int pp = pf; pp <= pl; ++pp)
         if (pp != own)
-          mx = fmaxf(mx, __ldcg(p.part_lse + pair_slot(tm, pp, pc.bb) *
-                                                kHeads + head));
+          mx = fmaxf(mx, __ldcg(p.part_lse + mslot(pp) * kHeads + head));
       float sum = exp2f((lse - mx) * kLog2e);
       for (int pp = pf; pp <= pl; ++pp)
         if (pp != own)
-          sum += exp2f((__ldcg(p.part_lse + pair_slot(tm, pp, pc.bb) *
-                                               kHeads + head) - mx) * kLog2e);
+          sum += exp2f((__ldcg(p.part_lse + mslot(pp) * kHeads + head) - mx) * kLog2e);
       const float big = mx + logf(sum);
       if (!has_next) {
         // Last piece of this pair: the rings and the Q/P buffers are idle.  O of
@@ -2187,7 +2188,7 @@ __device__ __forceinline__ void softmax_epilogue(const Params& p, const Ctx& c, 
         const uint32_t mstage = ptx::smem_u32(smem);
         for (int pp = pf; pp <= pl; ++pp) {
           if (pp == own) continue;
-          const size_t sl = pair_slot(tm, pp, pc.bb);
+          const size_t sl = mslot(pp);
           const float w = exp2f((__ldcg(p.part_lse + sl * kHeads + head) - big) * kLog2e);
           if (L == 0) {
             ptx::fence_proxy_async_all();
@@ -2236,7 +2237,7 @@ __device__ __forceinline__ void softmax_epilogue(const Params& p, const Ctx& c, 
           for (int k = 0; k < 32; ++k) acc[k] = __uint_as_float(o[k]) * w_own;
           for (int pp = pf; pp <= pl; ++pp) {
             if (pp == own) continue;
-            const size_t sl = pair_slot(tm, pp, pc.bb);
+            const size_t sl = mslot(pp);
             const float w = exp2f((__ldcg(p.part_lse + sl * kHeads + head) - big) * kLog2e);
             const float4* src = reinterpret_cast<const float4*>(p.part_o + (sl * kHeads + head) * kDim + d0);
 #pragma unroll
