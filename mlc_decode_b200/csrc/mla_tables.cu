@@ -38,7 +38,6 @@ struct TablesArgs {
   int* cu_new;               // [batch + 1] or nullptr
   int batch, max_pages, page, num_pages, num_free, num_tokens;
   int q_len;                 // 0: rows packed; else request i's rows are the last of [i q_len, (i + 1) q_len)
-  int whole;                 // a request gets all of its rows or none (q_len > 0)
 };
 
 // One request: first row in the packed list, rows held before, rows held after, and
@@ -68,12 +67,13 @@ __device__ long long block_scan(long long v, long long* s_warp) {
 // The records of every request, by one CTA; thread t owns requests [t per, (t + 1) per).
 // A request's lengths are read and its new length written by the same thread, so
 // new_seqlens may be seqlens.
-// With `whole` a request whose table row is too short asks for nothing, and one that does not
-// find all its pages takes none; nor do those behind it that need any, so that the pages
-// handed out are still a prefix of the sums.
+// With kWhole (q_len > 0) a request gets all of its rows or none: one whose table row is too short
+// asks for nothing, and one that does not find all its pages takes none; nor do those behind
+// it that need any, so that the pages handed out are still a prefix of the sums.
+template <bool kWhole>
 __device__ void plan(const TablesArgs& a, Record* rec, long long* s_warp) {
-  __shared__ int s_taken;   // with `whole`: pages handed out
-  if (threadIdx.x == 0) s_taken = 0;
+  __shared__ int s_taken;   // kWhole: pages handed out
+  if (kWhole && threadIdx.x == 0) s_taken = 0;
   const int per = (a.batch + kThreads - 1) / kThreads;
   const int i0 = min((int)threadIdx.x * per, a.batch), i1 = min(i0 + per, a.batch);
   const long long cover = (long long)a.max_pages * a.page;
@@ -91,7 +91,7 @@ __device__ void plan(const TablesArgs& a, Record* rec, long long* s_warp) {
     int rows = cut(at + n) - cu;
     at += n;
     const int len = old_len(i);
-    if (a.whole && len + (long long)rows > cover) rows = 0;
+    if (kWhole && len + (long long)rows > cover) rows = 0;
     rec[i] = Record{cu, len, rows, 0};   // end: the rows asked for, until the pages are known
     pages += page_count(min(len + (long long)rows, cover), a.page) - page_count(len, a.page);
   }
@@ -109,7 +109,7 @@ __device__ void plan(const TablesArgs& a, Record* rec, long long* s_warp) {
     r.first = pos0 + (int)min(taken, avail);
     r.end = (int)min(want, (long long)(held + got) * a.page);
     taken += take;
-    if (a.whole) {
+    if (kWhole) {
       if (got < take)
         r.end = r.len;
       else if (take > 0)
@@ -119,8 +119,8 @@ __device__ void plan(const TablesArgs& a, Record* rec, long long* s_warp) {
     if (a.cu_new != nullptr) a.cu_new[i] = r.cu;
     a.new_seqlens[i] = r.end;
   }
-  if (a.whole) __syncthreads();
-  if (threadIdx.x == kThreads - 1) *a.new_free_pos = pos0 + (a.whole ? s_taken : (int)min(incl, avail));
+  if (kWhole) __syncthreads();
+  if (threadIdx.x == kThreads - 1) *a.new_free_pos = pos0 + (kWhole ? s_taken : (int)min(incl, avail));
 }
 
 // Slot and position of row p of request i; p at a page's start also names the page in
@@ -180,17 +180,19 @@ __device__ void fill4(const TablesArgs& a, const Record* rec, int k) {
   }
 }
 
+template <bool kWhole>
 __global__ void __launch_bounds__(kThreads) mla_tables_small_kernel(TablesArgs a) {
   __shared__ Record rec[kSmallBatch];
   __shared__ long long s_warp[kThreads / 32];
-  plan(a, rec, s_warp);
+  plan<kWhole>(a, rec, s_warp);
   __syncthreads();
   for (int k = 4 * threadIdx.x; k < a.num_tokens; k += 4 * kThreads) fill4(a, rec, k);
 }
 
+template <bool kWhole>
 __global__ void __launch_bounds__(kThreads) mla_tables_plan_kernel(TablesArgs a, Record* rec) {
   __shared__ long long s_warp[kThreads / 32];
-  plan(a, rec, s_warp);
+  plan<kWhole>(a, rec, s_warp);
 }
 
 __global__ void __launch_bounds__(kFillThreads) mla_tables_fill_kernel(TablesArgs a, const Record* rec) {
@@ -201,7 +203,8 @@ __global__ void __launch_bounds__(kFillThreads) mla_tables_fill_kernel(TablesArg
 bool small(int batch, int num_tokens) { return batch <= kSmallBatch && num_tokens <= kSmallTokens; }
 
 
-int extend(const char* fn, TablesArgs a, void* workspace, size_t workspace_bytes, void* stream) {
+template <bool kWhole>
+int extend(const char* fn, const TablesArgs& a, void* workspace, size_t workspace_bytes, void* stream) {
   const int batch = a.batch, max_pages = a.max_pages, page_size = a.page, num_pages = a.num_pages,
             num_free = a.num_free, num_tokens = a.num_tokens, q_len = a.q_len;
   if (batch < 1 || max_pages < 1 || page_size < 1 || num_pages < 1 || num_free < 0 || num_tokens < 0 || q_len < 0) {
@@ -232,10 +235,10 @@ int extend(const char* fn, TablesArgs a, void* workspace, size_t workspace_bytes
   }
   const cudaStream_t s = static_cast<cudaStream_t>(stream);
   if (one) {
-    mla_tables_small_kernel<<<1, kThreads, 0, s>>>(a);
+    mla_tables_small_kernel<kWhole><<<1, kThreads, 0, s>>>(a);
   } else {
     Record* rec = static_cast<Record*>(workspace);
-    mla_tables_plan_kernel<<<1, kThreads, 0, s>>>(a, rec);
+    mla_tables_plan_kernel<kWhole><<<1, kThreads, 0, s>>>(a, rec);
     const long long quads = ((long long)num_tokens + 3) / 4;
     if (quads > 0)
       mla_tables_fill_kernel<<<(unsigned)((quads + kFillThreads - 1) / kFillThreads), kFillThreads, 0, s>>>(a, rec);
@@ -271,10 +274,9 @@ int32_t mla_extend_block_tables(int32_t* block_table, const int32_t* cache_seqle
                                 void* workspace, size_t workspace_bytes, int32_t batch, int32_t max_pages,
                                 int32_t page_size, int32_t num_pages, int32_t num_free, int32_t num_tokens,
                                 int32_t q_len, void* stream) {
-  return extend("mla_extend_block_tables",
-                TablesArgs{block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens, new_free_pos, slots,
-                           positions, cu_new, batch, max_pages, page_size, num_pages, num_free, num_tokens, q_len, 0},
-                workspace, workspace_bytes, stream);
+  const TablesArgs a{block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens, new_free_pos, slots,
+                     positions, cu_new, batch, max_pages, page_size, num_pages, num_free, num_tokens, q_len};
+  return extend<false>("mla_extend_block_tables", a, workspace, workspace_bytes, stream);
 }
 
 int32_t mla_extend_block_tables_whole(int32_t* block_table, const int32_t* cache_seqlens, const int32_t* new_lens,
@@ -288,10 +290,9 @@ int32_t mla_extend_block_tables_whole(int32_t* block_table, const int32_t* cache
     set_error("%s: q_len must be >= 1, got %d", fn, q_len);
     return MLA_ERR_ARG;
   }
-  return extend(fn,
-                TablesArgs{block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens, new_free_pos, slots,
-                           positions, cu_new, batch, max_pages, page_size, num_pages, num_free, num_tokens, q_len, 1},
-                workspace, workspace_bytes, stream);
+  const TablesArgs a{block_table, cache_seqlens, new_lens, free_pages, free_pos, new_seqlens, new_free_pos, slots,
+                     positions, cu_new, batch, max_pages, page_size, num_pages, num_free, num_tokens, q_len};
+  return extend<true>(fn, a, workspace, workspace_bytes, stream);
 }
 
 }  // extern "C"
