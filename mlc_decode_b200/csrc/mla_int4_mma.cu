@@ -213,7 +213,8 @@ __device__ __forceinline__ float exp2_approx(float x) {
   return y;
 }
 
-template <typename T, int MT>
+// kHide: sequences of several positions, whose last rows not all of them see.
+template <typename T, int MT, bool kHide>
 __global__ void __launch_bounds__(kThreads, Lay<MT>::kCtasPerSm)
 mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
   using L = Lay<MT>;
@@ -410,7 +411,7 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
         const int valid = len - j * kTileR;
         // rows of this tile that not every position sees: from its first position's length on
         const int hidden = max(valid - (a.q_len - 1), 0);
-        const bool hides = a.q_len > 1 && hidden < kTileR;
+        const bool hides = kHide && hidden < kTileR;
         uint32_t* bad = reinterpret_cast<uint32_t*>(smem + L::kBad) + 2 * (tile & 1);
         if (hides && tid < 2) bad[tid] = 0u;
         if (valid < kTileR) {
@@ -731,10 +732,14 @@ cudaError_t device_facts(int* sms) {
     auto grant = [&](const void* f, uint32_t bytes) {
       if (err == cudaSuccess) err = cudaFuncSetAttribute(f, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
     };
-    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__half, 1>), Lay<1>::kBytes);
-    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__nv_bfloat16, 1>), Lay<1>::kBytes);
-    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__half, 2>), Lay<2>::kBytes);
-    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__nv_bfloat16, 2>), Lay<2>::kBytes);
+    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__half, 1, false>), Lay<1>::kBytes);
+    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__half, 1, true>), Lay<1>::kBytes);
+    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__nv_bfloat16, 1, false>), Lay<1>::kBytes);
+    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__nv_bfloat16, 1, true>), Lay<1>::kBytes);
+    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__half, 2, false>), Lay<2>::kBytes);
+    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__half, 2, true>), Lay<2>::kBytes);
+    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__nv_bfloat16, 2, false>), Lay<2>::kBytes);
+    grant(reinterpret_cast<const void*>(mla_int4_mma_kernel<__nv_bfloat16, 2, true>), Lay<2>::kBytes);
     if (err != cudaSuccess) return err;
     d.ready = true;
   }
@@ -799,7 +804,10 @@ inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 template <typename T, int MT>
 cudaError_t launch_typed(const MmaParams& p, int workers, cudaStream_t stream) {
   using L = Lay<MT>;
-  mla_int4_mma_kernel<T, MT><<<workers, kThreads, L::kBytes, stream>>>(p);
+  if (p.a.q_len > 1)
+    mla_int4_mma_kernel<T, MT, true><<<workers, kThreads, L::kBytes, stream>>>(p);
+  else
+    mla_int4_mma_kernel<T, MT, false><<<workers, kThreads, L::kBytes, stream>>>(p);
   cudaError_t err = cudaGetLastError();
   if (err != cudaSuccess) return err;
   const long long items = (long long)p.a.batch * p.a.kv_heads * p.groups * L::kRows;
