@@ -357,15 +357,20 @@ int32_t mla_decode_ext_fp8kv(const void* q, const void* q_pe, const void* kv_fp8
  *   kv_scales  [..., kv_heads, 16] float16
  *   k_pe_cache [..., kv_heads, 64] in `dtype`
  * 416 bytes a row instead of 1,152.  Everything else (q, q_pe, out, lse, paging, lengths,
- * query positions, KV heads, cfg) as in mla_decode_ext.  Rows past a sequence's length
- * are not read; a row on a page outside [0, num_pages) reads as zeros.
+ * query positions, KV heads, cfg) as in mla_decode_ext.  Rows that a query row does not see
+ * (past the sequence's length, or a later position's) may be read but change nothing,
+ * whatever they hold; a row on a page outside [0, num_pages) reads as zeros.
  * The tensor-core kernels take the products in float16 with float32 sums: a row's value
  * (n - 8) s (the warp-level kernel's scores take n - 8 itself), a softmax weight and a
  * bfloat16 query are rounded to float16 once each, and queries and values must lie within
- * its range (the CUDA-core kernel, cfg kernel
- * MLA_KERNEL_SIMT, computes in float32).  cfg block_H, query rows per CTA, chooses
- * between them: up to 16 or 32 the warp-level kernel, more the CTA-pair kernel, 0 the
- * faster one for the shape.
+ * its range: a query row with a larger value, or one that sees a row with a larger value,
+ * is infinite or NaN (in the dims concerned at least), as it is when a value is NaN.  (mla_cache_append stores values up to
+ * 7 x 65504; the CUDA-core kernel, cfg kernel MLA_KERNEL_SIMT, computes in float32.)
+ * A stored weight has eleven bits down to 2^-21 of the row's largest and vanishes below 2^-32.
+ * cfg block_H, query rows per CTA, chooses between them: up to 16 or 32 the warp-level
+ * kernel, more the CTA-pair kernel, 0 the faster one for the shape at lengths near
+ * max_seqlen_kv (lengths are on the device: a caller whose sequences are far shorter than
+ * their room may choose better).
  * Workspace: mla_decode_int4kv_workspace_bytes (256-byte aligned, zero before the first
  * call with it, left ready by every call); 0 with no error text means none is needed.
  */

@@ -9,8 +9,10 @@
 // lane's eight codes are one 32-bit word and a warp stores whole 128-byte lines; lane l
 // also turns rope pair l.  A gather long enough to fill the GPU has the loads of two rows
 // in flight per warp (131072 4-bit rows 39 us, 41 with one); an append, which computes
-// more, has one row and more warps (37 us for as many, 41 with the rope part turned; with
-// a slower quantisation 58, and 62 and 94 with two and four rows a warp).
+// more, has one row and more warps (37 us for as many, 41 with the rope part turned;
+// two and four rows a warp were timed with a slower quantisation only: 62 and 94 against 58).
+// As many rotated 16-bit rows take 48 us, e4m3 rows 41, their gathers 48 and 39 (at 6.4 TB/s:
+// 47 and 36.5).
 #include <cuda_fp8.h>
 #include <math.h>
 #include <string.h>

@@ -579,7 +579,8 @@ int32_t mla_selftest_wait_timeout(uint32_t* status, uint64_t* result, uint64_t l
 // ---------------------------------------------------------------------------
 // Ragged / paged decode (per-sequence KV lengths, optional page table).
 // Workspace: [status 256 B][counters u32 x batch x groups x 4, padded][tile prefix
-// sums u32 x (batch x groups + 1), padded][partial LSE][partial O].
+// sums u32 x (batch x groups + 1) and the plan's whole-sequence word, padded][partial
+// LSE][partial O].
 // ---------------------------------------------------------------------------
 namespace mla {
 namespace {

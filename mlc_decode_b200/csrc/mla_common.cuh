@@ -146,7 +146,8 @@ struct DecodeArgs {
   const int* seqlens;      // [batch] or nullptr
   const int* block_table;  // [batch][max_pages] or nullptr (contiguous [batch, seqlen_kv] rows)
   int page_size, num_pages, max_pages;
-  uint32_t* cu_tiles;      // workspace: flattened-tile prefix sums (batch x head groups + 1)
+  uint32_t* cu_tiles;      // workspace: flattened-tile prefix sums (batch x head groups + 1), then the
+                           // plan's word whether every sequence has a pair of its own
   int batch, heads, seqlen_kv, dtype;
   // query positions per sequence (causal within the step) and KV heads (query
   // heads [i*h/kv_heads, (i+1)*h/kv_heads) read KV head i); 0 means 1.

@@ -14,8 +14,8 @@ inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 enum Int4Kernel { kSimt, kPair, kMma };
 
 // Which of the two tensor-core kernels, by the time each is expected to take in us for
-// sequences of the maximal length (fits to measured calls, one B200; rows = query rows
-// per KV head):
+// sequences of the maximal length, the one the host knows (fits to measured calls, one
+// B200; rows = query rows per KV head):
 //   warp-level, 16 rows a CTA and two CTAs an SM: 16 + 4.0 per round of 64-row tiles;
 //   32 rows and one CTA: 16 + 3.1 per round;
 //   pair kernel, 128 rows a pair: 30 + 2.9 per round of 128-row tiles, and 15 or 45 to merge

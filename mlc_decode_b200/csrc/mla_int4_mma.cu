@@ -15,11 +15,12 @@
 //   B fragment of two k-steps, with the dims of Q's A fragment (kept in registers)
 //   permuted to match.  The two k-steps are one scale group: their MMAs take the bare
 //   codes n - 8 and a float32 product with the scale follows, so the scores have no
-//   rounding of the row values (values rounded to fp16 first: 130 us instead of 133 at
+//   rounding of the row values (values rounded to fp16 first: 121 us instead of 125 at
 //   b128 h16 s4096, and an error of 2e-4 in the log-sum-exp of short sequences).  For P.V the
-//   values are rounded to fp16 once, as the weights are, and the words of two rows are interleaved by 16-bit halves,
-//   so that a field pair is one dim of two neighbouring rows; column n of block e is dim
-//   8 n + e of the warp's 64, which leaves each thread with 16 neighbouring output dims.
+//   values are rounded to fp16 once, as the weights are (kI4WeightLog2), and the words of
+//   two rows are interleaved by 16-bit halves, so that a field pair is one dim of two
+//   neighbouring rows; column n of block e is dim 8 n + e of the warp's 64, which leaves
+//   each thread with 16 neighbouring output dims.
 // * Eight warps: for S two row halves x four quarters of the dims (the quarters' sums
 //   meet in shared memory), for P.V 64 output dims each.  The 128-byte TMA swizzle makes
 //   both access patterns free of bank conflicts.
@@ -28,8 +29,9 @@
 //   Every CTA sums the lengths itself: no plan launch.
 //
 // Bound: the issue slots of the widening (13 instructions per 8 codes, once for S and
-// once for P.V) with the latencies that 16 warps an SM leave uncovered (issue slots 55 %,
-// integer pipe 45 %, tensor pipe 30 % busy at b128 h16 s4096: 121 us, 1.8 TB/s).
+// once for P.V) with the latencies that 16 warps an SM leave uncovered (issue slots 56 %,
+// integer pipe 43 %, tensor pipe 29 % busy at b128 h16 s4096, bf16: 124 us, 1.8 TB/s; fp16,
+// whose registers spill 64 bytes: 133 us).
 // S of the next tile beside P.V of this one between the same two barriers: no faster.
 #include <cuda.h>
 #include <cudaTypedefs.h>

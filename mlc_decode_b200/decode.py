@@ -486,7 +486,9 @@ class MlaPagedDecodeKernel:
         (leading dims as ``__call__``'s kv_cache) hold the rows as ``cache_append`` writes
         them: 16 groups of 32 dims, each dim (code - 8) x its group's scale.  q, q_pe,
         k_pe_cache and out keep the model's type; bfloat16 queries and the rows' values must
-        lie within fp16's range (the scores are fp16 products with fp32 sums).  The first call
+        lie within fp16's range (the scores are fp16 products with fp32 sums; what leaves it
+        comes out infinite or NaN).  Rows a position does not see change nothing, whatever
+        they hold.  The first call
         on a device makes the workspace and precedes any graph capture.
         """
         b, h, smax, ql, kvh = self.batch, self.heads, self.max_seqlen_kv, self.q_len, self.kv_heads
