@@ -467,17 +467,14 @@ class MlaPagedDecodeKernel:
             _check_tensor("lse", lse, qshape, torch.float32, dev)
             lse_ptr = lse.data_ptr()
         ws = self._workspace(dev, dtype)
-        with torch.cuda.device(dev):
-            stream = torch.cuda.current_stream(dev).cuda_stream
         if fp8:
-            capi.decode_ext_fp8kv(q.data_ptr(), q_pe.data_ptr(), kv_cache.data_ptr(), k_pe_cache.data_ptr(),
-                                  float(kv_scale), bt_ptr, sl_ptr, out.data_ptr(), lse_ptr, ws.data_ptr(), ws.numel(),
-                                  b, ql, h, kvh, smax, page_size, num_pages, max_pages, _DTYPES[dtype], self._ccfg,
-                                  stream)
+            _on_device(dev, capi.decode_ext_fp8kv, q.data_ptr(), q_pe.data_ptr(), kv_cache.data_ptr(),
+                       k_pe_cache.data_ptr(), float(kv_scale), bt_ptr, sl_ptr, out.data_ptr(), lse_ptr, ws.data_ptr(),
+                       ws.numel(), b, ql, h, kvh, smax, page_size, num_pages, max_pages, _DTYPES[dtype], self._ccfg)
         else:
-            capi.decode_ext(q.data_ptr(), q_pe.data_ptr(), kv_cache.data_ptr(), k_pe_cache.data_ptr(), bt_ptr,
-                            sl_ptr, out.data_ptr(), lse_ptr, ws.data_ptr(), ws.numel(), b, ql, h, kvh, smax,
-                            page_size, num_pages, max_pages, _DTYPES[dtype], self._ccfg, stream)
+            _on_device(dev, capi.decode_ext, q.data_ptr(), q_pe.data_ptr(), kv_cache.data_ptr(), k_pe_cache.data_ptr(),
+                       bt_ptr, sl_ptr, out.data_ptr(), lse_ptr, ws.data_ptr(), ws.numel(), b, ql, h, kvh, smax,
+                       page_size, num_pages, max_pages, _DTYPES[dtype], self._ccfg)
 
     def decode_int4(self, q, q_pe, kv_codes, kv_scales, k_pe_cache, cache_seqlens, out, lse=None, block_table=None):
         """``__call__`` over a latent cache held in 4 bits (mla_decode_ext_int4kv).
