@@ -167,7 +167,7 @@ __device__ void fill4(const TablesArgs& a, const Record* rec, int k) {
     pos[e] = (int)min(p, (long long)INT_MAX);
     slot[e] = place(a, rec[i], i, pos[e]);
   }
-  if (k + 4 <= a.num_tokens && ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0) {
+  if (a.num_tokens - k >= 4 && ((reinterpret_cast<uintptr_t>(a.slots) | reinterpret_cast<uintptr_t>(a.positions)) & 15) == 0) {
     *reinterpret_cast<int4*>(a.slots + k) = make_int4(slot[0], slot[1], slot[2], slot[3]);
     *reinterpret_cast<int4*>(a.positions + k) = make_int4(pos[0], pos[1], pos[2], pos[3]);
   } else {
