@@ -94,8 +94,9 @@ int plan_call(const char* fn, int batch, int q_len, int heads, int kv_heads, int
   p->kernel = kSimt;
   p->splits = int4_simt_splits((int)qb, heads / kv_heads, max_seqlen_kv, asked);
   const size_t rows = p->splits > 1 ? (size_t)p->splits * batch * q_len * heads : 0;
-  p->lse_off = 0;
-  p->o_off = align_up(rows * sizeof(float), 256);
+  // (a status word as in the other kernels' workspaces, which this kernel leaves zero)
+  p->lse_off = rows > 0 ? 256 : 0;
+  p->o_off = p->lse_off + align_up(rows * sizeof(float), 256);
   p->total = p->o_off + rows * kDim * sizeof(float);
   return MLA_OK;
 }
