@@ -58,6 +58,12 @@ def _on_device(device, call, *args):
             call(*args, torch._C._cuda_getCurrentRawStream(index))
 
 
+def _index_of(device):
+    """A device's index; of "cuda" without one, the current device's."""
+    device = torch.device(device)
+    return torch.cuda.current_device() if device.type == "cuda" and device.index is None else device.index
+
+
 def _not_capturing(what):
     """A buffer made inside a graph capture holds its first values only once the graph has
     run: an eager call before that would read whatever the memory held."""
@@ -270,7 +276,7 @@ class MlaDecodeKernel:
         """Status word the tensor-core kernel leaves in the workspace (0 = no timeout)."""
         if self._grouped is not None:
             return self._grouped.device_status(device, dtype)
-        ws = self._ws.get((torch.device(device).index, dtype))
+        ws = self._ws.get((_index_of(device), dtype))
         if ws is None or ws.numel() < 4:
             return 0
         return int(ws[:4].view(torch.int32).item())
@@ -306,7 +312,7 @@ class MlaDecodeKernel:
 
 
 def _clock_probe(ws_map, device, dtype):
-    ws = ws_map.get((torch.device(device).index, dtype))
+    ws = ws_map.get((_index_of(device), dtype))
     if ws is None or ws.numel() < 32:
         return (0, 0, 0)
     v = ws[8:32].view(torch.int64).tolist()
@@ -418,7 +424,7 @@ class MlaPagedDecodeKernel:
 
     def device_status(self, device, dtype) -> int:
         """Status word the kernels leave in the workspaces (0 = no timeout)."""
-        index = torch.device(device).index
+        index = _index_of(device)
         for key in ((index, dtype), (index, dtype, "int4")):
             ws = self._ws.get(key)
             if ws is not None and ws.numel() >= 4 and int(ws[:4].view(torch.int32).item()) != 0:
