@@ -361,8 +361,9 @@ int32_t mla_decode_ext_fp8kv(const void* q, const void* q_pe, const void* kv_fp8
  * (past the sequence's length, or a later position's) may be read but change nothing,
  * whatever they hold; a row on a page outside [0, num_pages) reads as zeros.
  * The tensor-core kernels take the products in float16 with float32 sums: a row's value
- * (n - 8) s (the warp-level kernel's scores take n - 8 itself), a softmax weight and a
- * bfloat16 query are rounded to float16 once each, and queries and values must lie within
+ * (n - 8) s (the warp-level kernel's scores take n - 8 itself), a softmax weight (two
+ * parts in the warp-level kernel's float16 calls) and a bfloat16 query are rounded to
+ * float16 once each, and queries and values must lie within
  * its range: a query row with a larger value, or one that sees a row with a larger value,
  * is infinite or NaN (in the dims concerned at least), as it is when a value is NaN.  (mla_cache_append stores values up to
  * 7 x 65504; the CUDA-core kernel, cfg kernel MLA_KERNEL_SIMT, computes in float32.)

@@ -17,7 +17,10 @@
 //   codes n - 8 and a float32 product with the scale follows, so the scores have no
 //   rounding of the row values (values rounded to fp16 first: 121 us instead of 125 at
 //   b128 h16 s4096, and an error of 2e-4 in the log-sum-exp of short sequences).  For P.V the
-//   values are rounded to fp16 once, as the weights are (kI4WeightLog2), and the words of
+//   values are rounded to fp16 once, and so are the weights (kI4WeightLog2) of a bf16 call,
+//   whose result rounds eight times as coarsely; a fp16 call's weights are two fp16 parts with
+//   an MMA each (root-mean-square error 1.25 to 1.38 times the result's own rounding instead of
+//   1.40 to 1.52; 145 us instead of 133 at b128 h16 s4096).  The words of
 //   two rows are interleaved by 16-bit halves, so that a field pair is one dim of two
 //   neighbouring rows; column n of block e is dim 8 n + e of the warp's 64, which leaves
 //   each thread with 16 neighbouring output dims.
@@ -30,8 +33,8 @@
 //
 // Bound: the issue slots of the widening (13 instructions per 8 codes, once for S and
 // once for P.V) with the latencies that 16 warps an SM leave uncovered (issue slots 56 %,
-// integer pipe 43 %, tensor pipe 29 % busy at b128 h16 s4096, bf16: 124 us, 1.8 TB/s; fp16,
-// whose registers spill 64 bytes: 133 us).
+// integer pipe 43 %, tensor pipe 29 % busy at b128 h16 s4096, bf16: 124 us, 1.8 TB/s; the
+// fp16 instance spills 40 bytes).
 // S of the next tile beside P.V of this one between the same two barriers: no faster.
 #include <cuda.h>
 #include <cudaTypedefs.h>
@@ -105,8 +108,8 @@ struct Lay {
   static constexpr int kStages = MT == 1 ? 3 : 5;
   static constexpr int kCtasPerSm = MT == 1 ? 2 : 1;
   static constexpr uint32_t kS = kStages * kStage;                        // [4][rows][kSPitch] float
-  static constexpr uint32_t kP = kS + 4 * kRows * kSPitch * 4;            // [rows][kPPitch] half
-  static constexpr uint32_t kAlpha = kP + kRows * kPPitch * 2;            // [rows] float
+  static constexpr uint32_t kP = kS + 4 * kRows * kSPitch * 4;            // [2][rows][kPPitch] half: parts of P
+  static constexpr uint32_t kAlpha = kP + 2 * kRows * kPPitch * 2;        // [rows] float
   static constexpr uint32_t kInv = kAlpha + kRows * 4;                    // [rows] float
   static constexpr uint32_t kBar = kInv + kRows * 4;                      // a barrier per stage
   static constexpr uint32_t kMisc = kBar + 8 * 8;                         // abort flag, Walk of the lookups
@@ -220,6 +223,7 @@ template <typename T, int MT, bool kHide>
 __global__ void __launch_bounds__(kThreads, Lay<MT>::kCtasPerSm)
 mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
   using L = Lay<MT>;
+  constexpr bool kTwoParts = std::is_same<T, __half>::value;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   // (aligned by an offset: a pointer rounded as an integer would make every access generic)
   uint8_t* smem = smem_raw + ((1024u - (ptx::smem_u32(smem_raw) & 1023u)) & 1023u);
@@ -347,6 +351,14 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
     const int tq = warp >> 2, dq = warp & 3;         // S: row half, quarter of the dims
     float* sS = reinterpret_cast<float*>(smem + L::kS);
     __half* sP = reinterpret_cast<__half*>(smem + L::kP);
+    // A fragment of k-step ks, weights of 16 rows from row `row`
+    auto load_p = [&](int row, int ks, uint32_t (&o)[4]) {
+      const __half* pr = sP + (row + qr) * kPPitch + 16 * ks + 2 * t;
+      o[0] = *reinterpret_cast<const uint32_t*>(pr);
+      o[1] = *reinterpret_cast<const uint32_t*>(pr + 8 * kPPitch);
+      o[2] = *reinterpret_cast<const uint32_t*>(pr + 8);
+      o[3] = *reinterpret_cast<const uint32_t*>(pr + 8 * kPPitch + 8);
+    };
     float* sAlpha = reinterpret_cast<float*>(smem + L::kAlpha);
     float* sInv = reinterpret_cast<float*>(smem + L::kInv);
     const int rows_all = a.q_len * p.g;              // query rows of a unit's KV head
@@ -503,8 +515,13 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
             ls += v[e];
           }
           l_run[mt] = fmaf(l_run[mt], alpha, ls);
-          *reinterpret_cast<uint2*>(sP + row * kPPitch + col) =
-              make_uint2(Elt<__half>::pack2(v[0], v[1]), Elt<__half>::pack2(v[2], v[3]));
+          const uint2 hi = make_uint2(Elt<__half>::pack2(v[0], v[1]), Elt<__half>::pack2(v[2], v[3]));
+          *reinterpret_cast<uint2*>(sP + row * kPPitch + col) = hi;
+          if constexpr (kTwoParts) {
+            const float2 h0 = Elt<__half>::to2(hi.x), h1 = Elt<__half>::to2(hi.y);
+            *reinterpret_cast<uint2*>(sP + (L::kRows + row) * kPPitch + col) =
+                make_uint2(Elt<__half>::pack2(v[0] - h0.x, v[1] - h0.y), Elt<__half>::pack2(v[2] - h1.x, v[3] - h1.y));
+          }
           if ((tid & 15) == 0) sAlpha[row] = alpha;
         }
         __syncthreads();
@@ -534,13 +551,7 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
         for (int ks = 0; ks < 4; ++ks) {
           uint32_t pf[MT][4];
 #pragma unroll
-          for (int mt = 0; mt < MT; ++mt) {
-            const __half* pr = sP + (16 * mt + qr) * kPPitch + 16 * ks + 2 * t;
-            pf[mt][0] = *reinterpret_cast<const uint32_t*>(pr);
-            pf[mt][1] = *reinterpret_cast<const uint32_t*>(pr + 8 * kPPitch);
-            pf[mt][2] = *reinterpret_cast<const uint32_t*>(pr + 8);
-            pf[mt][3] = *reinterpret_cast<const uint32_t*>(pr + 8 * kPPitch + 8);
-          }
+          for (int mt = 0; mt < MT; ++mt) load_p(16 * mt, ks, pf[mt]);
           uint32_t f[2][2][4];   // [rows 2 t and 2 t + 8][even, odd dims][pair]
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -558,6 +569,15 @@ mla_int4_mma_kernel(const __grid_constant__ MmaParams p) {
           for (int e = 0; e < 8; ++e)
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) mma16816<__half>(acc[mt][e], pf[mt], f[0][e & 1][e >> 1], f[1][e & 1][e >> 1]);
+          if constexpr (kTwoParts) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) load_p(L::kRows + 16 * mt, ks, pf[mt]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+#pragma unroll
+              for (int mt = 0; mt < MT; ++mt)
+                mma16816<__half>(acc[mt][e], pf[mt], f[0][e & 1][e >> 1], f[1][e & 1][e >> 1]);
+          }
         }
       }
       // ---- end of the piece: normalise, write the result or a partial

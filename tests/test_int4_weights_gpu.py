@@ -44,3 +44,30 @@ def test_many_small_weights_beside_a_dominant_one(e, dtype, kernel):
     tol = (s - 1) * max(2.0 ** -32, w * 2.0 ** -11) + (torch.finfo(dtype).eps / 2 + sums + scores) * ref
     assert (out.double() - ref).abs().max().item() <= tol, (out[0, 0, 0].item(), ref)
     assert (lse.double() - ref_lse).abs().max().item() <= sums + scores
+
+
+@pytest.mark.parametrize("kernel", ["mma16", "mma32"])
+@pytest.mark.parametrize("b, h, s", [(8, 96, 500), (16, 64, 1000), (4, 16, 300)])
+def test_fp16_results_are_near_their_own_rounding(b, h, s, kernel):
+    """fp16 results of the warp-level kernel: the weights are taken in two parts, so what is left
+    beside the result's own rounding is the values', (n - 8) s to fp16.  Each value's relative error
+    has at most the result's spread (some products are exact), and results are sums of values with
+    independent errors: at most sqrt(2) times the result's rounding in the root mean square, and 3 %
+    for the sample (weights in one part: 1.46 to 1.52)."""
+    g = torch.Generator(device="cuda").manual_seed(b * h)
+    dt = torch.float16
+    x = torch.randn(b, s, 16, 32, generator=g, device="cuda")
+    scales = (x.abs().amax(-1) / 7).half()
+    n = (x / scales.float().unsqueeze(-1)).round().clamp(-8, 7)
+    nib = [0, 2, 4, 6, 1, 3, 5, 7]
+    c = (n + 8).to(torch.uint8).view(b, s, 64, 8)[..., nib].view(b, s, 64, 4, 2)
+    codes = (c[..., 0] | (c[..., 1] << 4)).reshape(b, s, 1, 256).contiguous()
+    rows = (n.double() * scales.double().unsqueeze(-1)).view(b, s, 512)
+    q, qp = torch.randn(b, h, 512, generator=g, device="cuda").to(dt), torch.randn(b, h, 64, generator=g, device="cuda").to(dt)
+    pe = torch.randn(b, s, 1, 64, generator=g, device="cuda").to(dt)
+    scores = (q.double() @ rows.transpose(1, 2) + qp.double() @ pe[:, :, 0].double().transpose(1, 2)) * SCALE
+    ref = torch.softmax(scores, -1) @ rows
+    out = torch.empty_like(q)
+    MlaPagedDecodeKernel(b, h, s, cfg=KERNELS[kernel]).decode_int4(q, qp, codes, scales.view(b, s, 1, 16), pe, None, out)
+    own = (ref.half().double() - ref).norm()
+    assert (out.double() - ref).norm() <= 1.03 * math.sqrt(2) * own, ((out.double() - ref).norm() / own).item()
