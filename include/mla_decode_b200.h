@@ -363,10 +363,10 @@ int32_t mla_decode_ext_fp8kv(const void* q, const void* q_pe, const void* kv_fp8
  * The tensor-core kernels take the products in float16 with float32 sums: a row's value
  * (n - 8) s (the warp-level kernel's scores take n - 8 itself), a softmax weight (two
  * parts in the warp-level kernel's float16 calls) and a bfloat16 query are rounded to
- * float16 once each, and queries and values must lie within
- * its range: a query row with a larger value, or one that sees a row with a larger value,
- * is infinite or NaN (in the dims concerned at least), as it is when a value is NaN.  (mla_cache_append stores values up to
- * 7 x 65504; the CUDA-core kernel, cfg kernel MLA_KERNEL_SIMT, computes in float32.)
+ * float16 once each, and queries and values must lie within its range: a query row with a
+ * larger value, or one that sees a row with a larger value, is infinite or NaN (in the dims
+ * concerned at least), as it is when a value is NaN.  (mla_cache_append stores values up
+ * to 7 x 65504; the CUDA-core kernel, cfg kernel MLA_KERNEL_SIMT, computes in float32.)
  * A stored weight has eleven bits down to 2^-21 of the row's largest and vanishes below 2^-32.
  * cfg block_H, query rows per CTA, chooses between them: up to 16 or 32 the warp-level
  * kernel, more the CTA-pair kernel, 0 the faster one for the shape at lengths near
@@ -403,7 +403,8 @@ int32_t mla_decode_ext_int4kv(const void* q, const void* q_pe, const void* kv_co
  * added); q_len > 0: num_tokens = batch x q_len, n is at most q_len and request i's rows
  * are the last n of [i q_len, (i + 1) q_len), as mla_decode_ext's causal rule has a step's
  * rows (a request that got fewer rows than n is not lined up with that rule any more: see
- * mla_extend_block_tables_whole).  new_seqlens may be cache_seqlens and new_free_pos may be free_pos (in place);
+ * mla_extend_block_tables_whole).  new_seqlens may be cache_seqlens and new_free_pos may
+ * be free_pos (in place);
  * otherwise no two arrays overlap.  Workspace: mla_block_tables_workspace_bytes (16-byte
  * aligned; 0 with no error text: none).
  */
